@@ -357,6 +357,111 @@ LCA_API int lca_swa_backward(const void* q, const void* k, const void* v, const 
                              const int64_t* global_tokens, int64_t num_global_tokens, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Paged KV cache held in 4 bits, for serving (no counterpart in the reference, which has no
+ * cache).  A pool holds `num_pages` pages of `page_size` tokens (a multiple of 16) for every
+ * KV head, (head_dim + 8) bytes a token and head: num_pages * kv_heads * page_size *
+ * (head_dim + 8) bytes, 16-byte aligned.  Piece (page, head) is page_size / 16 blocks of 16
+ * tokens, each
+ *     K codes [16][head_dim / 2] | V codes [16][head_dim / 2] | K words [16] | V words [16]
+ * where bits 4j .. 4j+3 of 32-bit word i of a code row hold element 8i + j, and a row's word is
+ * its fp32 scale with the zero point z in the low four bits: an element is scale * (code - z).
+ * A row is stored with lo = min(row, 0), hi = max(row, 0), scale = hi * (1/15) - lo * (1/15)
+ * (low four bits cleared), z = rint(-lo * (1 / scale)), code = clamp(rint(x * (1 / scale)) + z,
+ * 0, 15), all in fp32.  A row whose scale is below the smallest normal fp32 number is stored as
+ * zeros; a row with an infinity or a NaN reads back as NaN.
+ *
+ * A slot is page * page_size + (position within the page).  Request b's token at position p is
+ * in page block_table[b][p / page_size].  All the arrays of lengths, tables and slots are int32
+ * on the device; no call reads them on the host, so a serving step can be captured into a graph
+ * and replayed with other lengths.
+ */
+
+/* Most requests of one layout or release call. */
+#define LCA_MAX_REQUESTS 8192
+/* Most distinct global tokens of one lca_swa_forward_cached call. */
+#define LCA_MAX_CACHED_GLOBALS 1024
+
+/*
+ * Block tables and slot maps from request lengths.  Request b holds seq_lens[b] tokens and gets
+ * new_lens[b] more (negative lengths count as 0); the new tokens of all requests are packed one
+ * request after the other into num_tokens rows.  A request is placed whole or not at all:
+ * its rows must lie inside num_tokens, its pages inside its table row (table_width), and the
+ * new pages it needs must be left of the free ones, which are taken from the end of
+ * free_pages[0 .. *free_count) in request order (one that does not fit keeps its share of that
+ * order, so a later request that needs pages does not fit either).  Writes
+ *   block_table      the entries of the new pages (the others stay as they were)
+ *   slots, positions [num_tokens]; -1 for rows of a request that was not placed and for rows
+ *                    behind the last request's; 16-byte aligned.  The slot is also -1 where an
+ *                    entry of the table is negative.
+ *   cu_seqlens       [batch + 1] row offsets of the requests, at most num_tokens
+ *   kv_lens          [batch] cached plus new tokens; 0 for a request that was not placed, whose
+ *                    rows then attend to nothing
+ *   placed           [batch] new tokens placed (new_lens or 0)
+ *   next_seq_lens, next_free_count   the state after this step; distinct from seq_lens and
+ *                    free_count
+ * free_capacity is the length of free_pages; *free_count is clamped to it.
+ */
+LCA_API int lca_kv_layout(int32_t* block_table, int64_t batch, int64_t table_width, const int32_t* seq_lens,
+                          const int32_t* new_lens, const int32_t* free_pages, int64_t free_capacity,
+                          const int32_t* free_count, int64_t page_size, int64_t num_tokens, int32_t* slots,
+                          int32_t* positions, int32_t* cu_seqlens, int32_t* kv_lens, int32_t* placed,
+                          int32_t* next_seq_lens, int32_t* next_free_count, void* stream);
+
+/* The inverse: puts the pages of every request with release[b] != 0 at the end of the free
+ * list, in request order, and sets its length to 0.  Pages beyond free_capacity are dropped. */
+LCA_API int lca_kv_release(const int32_t* block_table, int64_t batch, int64_t table_width, const int32_t* seq_lens,
+                           const uint8_t* release, int32_t* free_pages, int64_t free_capacity,
+                           const int32_t* free_count, int64_t page_size, int32_t* next_seq_lens,
+                           int32_t* next_free_count, void* stream);
+
+/*
+ * Quantise the rows k, v [num_tokens][kv_heads][head_dim] (fp16 or bf16; strides in elements, the
+ * last dimension contiguous, any alignment of whole elements) into the slots given.  A slot
+ * outside the pool (-1) is skipped.  Slots of one call are distinct; which row a slot given twice
+ * holds afterwards is not specified.
+ */
+LCA_API int lca_kv4_append(void* pool, int64_t num_pages, int64_t kv_heads, int64_t page_size, int64_t head_dim,
+                           const void* k, const void* v, int dtype, int64_t k_token_stride, int64_t k_head_stride,
+                           int64_t v_token_stride, int64_t v_head_stride, const int32_t* slots, int64_t num_tokens,
+                           void* stream);
+
+/* The values held in the slots given, k, v [num_tokens][kv_heads][head_dim] contiguous and 16-byte
+ * aligned, in out_dtype (fp32, fp16 or bf16; rounded once).  A slot outside the pool reads as
+ * zeros. */
+LCA_API int lca_kv4_read(const void* pool, int64_t num_pages, int64_t kv_heads, int64_t page_size, int64_t head_dim,
+                         const int32_t* slots, int64_t num_tokens, void* k, void* v, int out_dtype, void* stream);
+
+/*
+ * Causal sliding-window + global-token attention of new tokens over the cache.  Request b's query
+ * rows are [cu_seqlens[b], cu_seqlens[b + 1]); they are the last tokens of its kv_lens[b] cached
+ * ones, so row i of them is at position p = kv_lens[b] - (its row count) + i.  Key j of the request
+ * is visible to it iff j <= p and (p - j <= window_size, or j or p is a global token): the causal
+ * form of lca_swa_forward's mask.  A window_size of at least the longest length is plain causal
+ * attention.
+ *   q       [num_rows][heads][head_dim] fp16 or bf16, 16-byte aligned, strides in elements (multiples
+ *           of 8), last dimension contiguous; query head h reads KV head h / (heads / kv_heads)
+ *   out     [num_rows][heads][head_dim] contiguous, out_dtype, 16-byte aligned
+ *   lse     [heads][num_rows] fp32 natural-log log-sum-exp, or NULL
+ * A row that sees nothing (its position is negative) gets zeros and an LSE of -inf.  Rows outside
+ * [cu_seqlens[0], cu_seqlens[batch]) are left as they were.  Lengths are clamped to the table's
+ * capacity (table_width * page_size); a key whose page id is outside the pool is not visible.
+ * global_tokens: HOST array of positions in [0, capacity), any order, duplicates allowed, at most
+ * LCA_MAX_CACHED_GLOBALS distinct ones; one at or behind a request's length has no effect yet.
+ * workspace: lca_swa_cached_workspace_size bytes of scratch, 256-byte aligned (NULL when 0); not
+ * to be shared by calls that can run concurrently.
+ */
+LCA_API int lca_swa_cached_workspace_size(int64_t num_rows, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t batch, int64_t capacity, int64_t window_size,
+                                          int64_t num_unique_global, size_t* out_bytes);
+LCA_API int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                   int64_t num_rows, int64_t heads, const void* pool, int64_t num_pages,
+                                   int64_t kv_heads, int64_t page_size, int64_t head_dim, const int32_t* block_table,
+                                   int64_t batch, int64_t table_width, const int32_t* kv_lens,
+                                   const int32_t* cu_seqlens, int64_t window_size, const int64_t* global_tokens,
+                                   int64_t num_global_tokens, float scale, void* out, int out_dtype, float* lse,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
 /*
  * Measurement hook (no counterpart in the reference): when both events are non-NULL,
  * subsequent lca_swa_forward calls made on THIS thread record `before_main` immediately

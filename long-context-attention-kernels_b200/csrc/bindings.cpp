@@ -208,6 +208,174 @@ int device_error() {
     return code;
 }
 
+// ------------------------------------------------------------------ paged 4-bit KV cache
+// (include/lca.h lca_kv_* / lca_kv4_* / lca_swa_forward_cached; no counterpart in the reference)
+
+void check_ints(const torch::Tensor& t, const char* name, int64_t dim, const torch::Device& device) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.dim() == dim, name,
+                " must be a contiguous int32 CUDA tensor with ", dim, " dimension(s)");
+    TORCH_CHECK(t.device() == device, name, " must be on the same device as the others");
+}
+
+struct PoolShape {
+    int64_t pages, kv_heads, page_size, head_dim;
+};
+
+PoolShape check_pool(const torch::Tensor& pool) {
+    TORCH_CHECK(pool.is_cuda() && pool.scalar_type() == torch::kUInt8 && pool.is_contiguous() && pool.dim() == 4,
+                "pool must be a contiguous uint8 CUDA tensor [pages, kv_heads, page_size, head_dim + 8]");
+    return {pool.size(0), pool.size(1), pool.size(2), pool.size(3) - 8};
+}
+
+int type_code(c10::ScalarType t, const char* name) {
+    TORCH_CHECK(t == torch::kFloat32 || t == torch::kFloat16 || t == torch::kBFloat16, name,
+                " must be float32, float16 or bfloat16");
+    return t == torch::kFloat32 ? LCA_DTYPE_F32 : (t == torch::kBFloat16 ? LCA_DTYPE_BF16 : LCA_DTYPE_F16);
+}
+
+void* current_stream() { return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream()); }
+
+std::vector<torch::Tensor> kv_cache_layout(torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor new_lens,
+                                           torch::Tensor free_pages, torch::Tensor free_count, int64_t page_size,
+                                           int64_t num_tokens) {
+    const auto device = block_table.device();
+    check_ints(block_table, "block_table", 2, device);
+    check_ints(seq_lens, "seq_lens", 1, device);
+    check_ints(new_lens, "new_lens", 1, device);
+    check_ints(free_pages, "free_pages", 1, device);
+    check_ints(free_count, "free_count", 1, device);
+    const int64_t batch = block_table.size(0);
+    TORCH_CHECK(seq_lens.size(0) == batch && new_lens.size(0) == batch,
+                "seq_lens and new_lens need one length per row of block_table (", batch, ")");
+    TORCH_CHECK(free_count.size(0) == 1, "free_count must hold one value");
+    TORCH_CHECK(num_tokens >= 0, "num_tokens must be >= 0 (got ", num_tokens, ")");
+    c10::cuda::CUDAGuard guard(device);
+    const int64_t pad = (num_tokens + 3) / 4 * 4;  // slots and positions on 16-byte boundaries
+    auto all = torch::empty({2 * pad + 4 * batch + 2}, block_table.options());
+    int32_t* at = all.data_ptr<int32_t>();
+    int32_t *slots = at, *positions = at + pad, *kv_lens = at + 2 * pad, *placed = kv_lens + batch,
+            *next = placed + batch, *count = next + batch, *cu = count + 1;
+    raise_status(lca_kv_layout(block_table.data_ptr<int32_t>(), batch, block_table.size(1), seq_lens.data_ptr<int32_t>(),
+                               new_lens.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(), free_pages.size(0),
+                               free_count.data_ptr<int32_t>(), page_size, num_tokens, slots, positions, cu, kv_lens,
+                               placed, next, count, current_stream()),
+                 "kv_cache_layout");
+    auto part = [&](int32_t* from, int64_t n) { return all.narrow(0, from - at, n); };
+    return {part(slots, num_tokens), part(positions, num_tokens), part(cu, batch + 1), part(kv_lens, batch),
+            part(placed, batch),     part(next, batch),           part(count, 1),      part(next, batch + 1)};
+}
+
+std::vector<torch::Tensor> kv_cache_release(torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor release,
+                                            torch::Tensor free_pages, torch::Tensor free_count, int64_t page_size) {
+    const auto device = block_table.device();
+    check_ints(block_table, "block_table", 2, device);
+    check_ints(seq_lens, "seq_lens", 1, device);
+    check_ints(free_pages, "free_pages", 1, device);
+    check_ints(free_count, "free_count", 1, device);
+    const int64_t batch = block_table.size(0);
+    TORCH_CHECK(release.is_cuda() && release.scalar_type() == torch::kBool && release.is_contiguous() &&
+                    release.dim() == 1 && release.device() == device,
+                "release must be a contiguous bool CUDA tensor with one value per request");
+    TORCH_CHECK(seq_lens.size(0) == batch && release.size(0) == batch,
+                "seq_lens and release need one value per row of block_table (", batch, ")");
+    TORCH_CHECK(free_count.size(0) == 1, "free_count must hold one value");
+    c10::cuda::CUDAGuard guard(device);
+    auto next = torch::empty({batch + 1}, block_table.options());
+    int32_t* at = next.data_ptr<int32_t>();
+    raise_status(lca_kv_release(block_table.data_ptr<int32_t>(), batch, block_table.size(1),
+                                seq_lens.data_ptr<int32_t>(), reinterpret_cast<const uint8_t*>(release.data_ptr<bool>()),
+                                free_pages.data_ptr<int32_t>(), free_pages.size(0), free_count.data_ptr<int32_t>(),
+                                page_size, at, at + batch, current_stream()),
+                 "kv_cache_release");
+    return {next.narrow(0, 0, batch), next.narrow(0, batch, 1), next};
+}
+
+void kv_cache_append(torch::Tensor pool, torch::Tensor k, torch::Tensor v, torch::Tensor slots) {
+    const PoolShape s = check_pool(pool);
+    check_ints(slots, "slots", 1, pool.device());
+    for (const torch::Tensor* t : {&k, &v}) {
+        TORCH_CHECK(t->is_cuda() && t->device() == pool.device() &&
+                        (t->scalar_type() == torch::kFloat16 || t->scalar_type() == torch::kBFloat16) &&
+                        t->scalar_type() == k.scalar_type(),
+                    "k and v must be CUDA tensors of one type, fp16 or bf16, on the pool's device");
+        TORCH_CHECK(t->dim() == 3 && t->size(0) == slots.size(0) && t->size(1) == s.kv_heads && t->size(2) == s.head_dim,
+                    "k and v must be [tokens, kv_heads, head_dim] = [", slots.size(0), ", ", s.kv_heads, ", ", s.head_dim,
+                    "], as the slots and the pool have them");
+        TORCH_CHECK(t->size(0) == 0 || t->stride(2) == 1, "the last dimension of k and v must be contiguous");
+    }
+    c10::cuda::CUDAGuard guard(pool.device());
+    raise_status(lca_kv4_append(pool.data_ptr(), s.pages, s.kv_heads, s.page_size, s.head_dim, k.data_ptr(), v.data_ptr(),
+                                type_code(k.scalar_type(), "k"), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                slots.data_ptr<int32_t>(), slots.size(0), current_stream()),
+                 "kv_cache_append");
+}
+
+std::vector<torch::Tensor> kv_cache_read(torch::Tensor pool, torch::Tensor slots, c10::ScalarType out_dtype) {
+    const PoolShape s = check_pool(pool);
+    check_ints(slots, "slots", 1, pool.device());
+    const int code = type_code(out_dtype, "out_dtype");
+    c10::cuda::CUDAGuard guard(pool.device());
+    auto k = torch::empty({slots.size(0), s.kv_heads, s.head_dim}, pool.options().dtype(out_dtype));
+    auto v = torch::empty_like(k);
+    raise_status(lca_kv4_read(pool.data_ptr(), s.pages, s.kv_heads, s.page_size, s.head_dim, slots.data_ptr<int32_t>(),
+                              slots.size(0), k.data_ptr(), v.data_ptr(), code, current_stream()),
+                 "kv_cache_read");
+    return {k, v};
+}
+
+std::vector<torch::Tensor> sliding_window_attention_cached(torch::Tensor Q, torch::Tensor pool,
+                                                           torch::Tensor block_table, torch::Tensor kv_lens,
+                                                           torch::Tensor cu_seqlens, int64_t window_size,
+                                                           std::vector<int64_t> global_tokens, double scale,
+                                                           c10::ScalarType out_dtype, bool want_lse,
+                                                           c10::optional<torch::Tensor> out) {
+    const PoolShape s = check_pool(pool);
+    const auto device = pool.device();
+    check_ints(block_table, "block_table", 2, device);
+    check_ints(kv_lens, "kv_lens", 1, device);
+    check_ints(cu_seqlens, "cu_seqlens", 1, device);
+    const int64_t batch = block_table.size(0);
+    TORCH_CHECK(kv_lens.size(0) == batch && cu_seqlens.size(0) == batch + 1,
+                "kv_lens needs one length, and cu_seqlens one offset and a last one, per row of block_table (", batch, ")");
+    TORCH_CHECK(Q.is_cuda() && Q.device() == device &&
+                    (Q.scalar_type() == torch::kFloat16 || Q.scalar_type() == torch::kBFloat16),
+                "Q must be an fp16 or bf16 CUDA tensor on the pool's device");
+    TORCH_CHECK(Q.dim() == 3 && Q.size(2) == s.head_dim, "Q must be [rows, heads, head_dim] with the pool's head_dim ",
+                s.head_dim);
+    TORCH_CHECK(Q.numel() == 0 || Q.stride(2) == 1, "the last dimension of Q must be contiguous");
+    const int64_t rows = Q.size(0), heads = Q.size(1);
+    c10::cuda::CUDAGuard guard(device);
+    torch::Tensor O;
+    if (out.has_value()) {
+        O = *out;
+        TORCH_CHECK(O.is_cuda() && O.device() == device && O.is_contiguous() && O.sizes() == Q.sizes() &&
+                        O.scalar_type() == out_dtype,
+                    "out must be a contiguous tensor of Q's shape and out_dtype on the pool's device");
+    } else {
+        O = torch::empty(Q.sizes(), Q.options().dtype(out_dtype));
+    }
+    torch::Tensor L;
+    if (want_lse) L = torch::empty({heads, rows}, Q.options().dtype(torch::kFloat32));
+    const int64_t capacity = block_table.size(1) * s.page_size;
+    size_t bytes = 0;
+    raise_status(lca_swa_cached_workspace_size(rows, heads, s.kv_heads, s.head_dim, batch, capacity, window_size,
+                                               (int64_t)global_tokens.size(), &bytes),
+                 "sliding_window_attention_cached");
+    torch::Tensor ws;
+    if (bytes > 0) ws = torch::empty({(int64_t)bytes}, pool.options());
+    raise_status(lca_swa_forward_cached(Q.data_ptr(), type_code(Q.scalar_type(), "Q"), Q.stride(0), Q.stride(1), rows,
+                                        heads, pool.data_ptr(), s.pages, s.kv_heads, s.page_size, s.head_dim,
+                                        block_table.data_ptr<int32_t>(), batch, block_table.size(1),
+                                        kv_lens.data_ptr<int32_t>(), cu_seqlens.data_ptr<int32_t>(), window_size,
+                                        global_tokens.data(), (int64_t)global_tokens.size(), static_cast<float>(scale),
+                                        O.data_ptr(), type_code(out_dtype, "out_dtype"),
+                                        want_lse ? L.data_ptr<float>() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr,
+                                        bytes, current_stream()),
+                 "sliding_window_attention_cached");
+    if (want_lse) return {O, L};
+    return {O};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -231,6 +399,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "Gradients (dQ, dK, dV), fp32, of the forward from its O and LSE and the gradient dO of O",
           py::arg("Q"), py::arg("K"), py::arg("V"), py::arg("O"), py::arg("LSE"), py::arg("dO"),
           py::arg("window_size"), py::arg("global_tokens"), py::arg("scale"));
+    m.def("kv_cache_layout", &kv_cache_layout, "Block tables and slot maps of a step from its requests' lengths",
+          py::arg("block_table"), py::arg("seq_lens"), py::arg("new_lens"), py::arg("free_pages"), py::arg("free_count"),
+          py::arg("page_size"), py::arg("num_tokens"));
+    m.def("kv_cache_release", &kv_cache_release, "Return the pages of the marked requests to the free list",
+          py::arg("block_table"), py::arg("seq_lens"), py::arg("release"), py::arg("free_pages"), py::arg("free_count"),
+          py::arg("page_size"));
+    m.def("kv_cache_append", &kv_cache_append, "Quantise K and V rows into slots of a 4-bit pool", py::arg("pool"),
+          py::arg("k"), py::arg("v"), py::arg("slots"));
+    m.def("kv_cache_read", &kv_cache_read, "The values held in slots of a 4-bit pool", py::arg("pool"),
+          py::arg("slots"), py::arg("out_dtype"));
+    m.def("sliding_window_attention_cached", &sliding_window_attention_cached,
+          "Causal sliding-window + global-token attention of new tokens over a 4-bit pool; returns [O] or [O, LSE]",
+          py::arg("Q"), py::arg("pool"), py::arg("block_table"), py::arg("kv_lens"), py::arg("cu_seqlens"),
+          py::arg("window_size"), py::arg("global_tokens"), py::arg("scale"), py::arg("out_dtype"), py::arg("want_lse"),
+          py::arg("out") = py::none());
     m.def("device_error", &device_error, "Read and clear the device-side error word (synchronises)");
     m.attr("abi_version") = lca_abi_version();
 }

@@ -17,6 +17,7 @@
 #include <string>
 #include <vector>
 
+#include "kv4.h"
 #include "swa_kernels.h"
 #include "swa_backward.h"
 
@@ -397,6 +398,19 @@ unsigned long long wait_timeout_ns() {
     }();
     return v;
 }
+
+}  // namespace
+
+int lca::device_info(int* sms, int** err_word, unsigned long long* wait_ns) {
+    int dev = 0;
+    const int st = check_device(&dev, err_word);
+    if (st != LCA_OK) return st;
+    *sms = g_dev_sms[dev];
+    *wait_ns = wait_timeout_ns();
+    return LCA_OK;
+}
+
+namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -1,0 +1,94 @@
+// kv4.h -- internal interface between the C-ABI layer (kv4_capi.cpp) and the kernels of the
+// paged 4-bit KV cache (kv4_cache.cu, kv4_attention.cu).  Not part of the public ABI.
+//
+// Cache format.  A pool is [pages][kv_heads] pieces of page_size tokens; a piece is
+// page_size / 16 blocks, and a block holds 16 tokens of one head contiguously:
+//
+//   K codes [16][d / 2] | V codes [16][d / 2] | K words [16] | V words [16]   = 16 * (d + 8) bytes
+//
+// so one block (or every block of a page) is one bulk copy.  Bits 4j .. 4j+3 of code word i
+// of a row hold element 8i + j.  A row's word is its fp32 scale with the zero point z in the
+// low four bits; an element is scale * (code - z).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <cstdint>
+
+#include "lca.h"
+
+namespace lca {
+namespace kv4 {
+
+constexpr int kBlock = 16;             // tokens per block
+constexpr int kMaxGlobals = 1024;      // global tokens of one attention call (kernel parameter space)
+constexpr int kMaxRequests = 8192;     // requests of one layout call (shared memory of its scan)
+
+__host__ __device__ constexpr int row_bytes(int d) { return d / 2; }              // code bytes of one row
+__host__ __device__ constexpr int block_bytes(int d) { return kBlock * (d + 8); }
+__host__ __device__ constexpr int v_codes_at(int d) { return kBlock * d / 2; }
+__host__ __device__ constexpr int k_words_at(int d) { return kBlock * d; }
+__host__ __device__ constexpr int v_words_at(int d) { return kBlock * d + 4 * kBlock; }
+
+struct Pool {
+    uint8_t* data;
+    int pages, kv_heads;
+    int page_blocks;  // page_size / 16
+};
+
+struct LayoutParams {
+    int32_t* table;  // [batch][width]
+    int batch, width, page_size, rows;
+    const int32_t *seq_lens, *new_lens, *free_pages, *free_count;
+    int free_cap;
+    int32_t *slots, *positions, *cu, *kv_lens, *placed, *next_seq_lens, *next_free_count;
+};
+
+struct ReleaseParams {
+    const int32_t* table;
+    int batch, width, page_size;
+    const int32_t* seq_lens;
+    const uint8_t* mask;
+    int32_t* free_pages;
+    int free_cap;
+    const int32_t* free_count;
+    int32_t *next_seq_lens, *next_free_count;
+};
+
+struct RowsParams {  // append (k, v read) and read (k, v written)
+    Pool pool;
+    void *k, *v;
+    long long k_token, k_head, v_token, v_head;  // strides in elements
+    const int32_t* slots;
+    int rows;
+};
+
+struct Globals {
+    int32_t at[kMaxGlobals];  // sorted, unique
+};
+
+struct AttnParams {
+    Pool pool;
+    const void* q;
+    long long q_token, q_head;  // strides in elements
+    const int32_t *table, *kv_lens, *cu;
+    int batch, width;
+    int rows, heads, group;  // query rows, query heads, query heads per KV head
+    int window, num_globals;
+    float scale;
+    void* out;   // [rows][heads][d]
+    float* lse;  // [heads][rows] or NULL
+};
+
+cudaError_t launch_layout(const LayoutParams& p, cudaStream_t stream);
+cudaError_t launch_release(const ReleaseParams& p, cudaStream_t stream);
+cudaError_t launch_append(int d, int dtype, bool vector, const RowsParams& p, cudaStream_t stream);
+cudaError_t launch_read(int d, int out_dtype, const RowsParams& p, cudaStream_t stream);
+cudaError_t launch_attention(int d, int dtype, int out_dtype, const AttnParams& p, const Globals& g,
+                             cudaStream_t stream);
+
+}  // namespace kv4
+
+// capi.cpp: checks the current device; its SM count, error word and wait limit.
+int device_info(int* sms, int** err_word, unsigned long long* wait_ns);
+
+}  // namespace lca

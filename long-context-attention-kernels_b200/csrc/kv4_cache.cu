@@ -1,0 +1,405 @@
+// kv4_cache.cu -- block tables and slot maps from request lengths, and the rows of the paged
+// 4-bit KV cache: quantise-and-append, and read back.  The cache format is in kv4.h.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "kv4.h"
+
+namespace lca {
+namespace kv4 {
+namespace {
+
+// ------------------------------------------------------------------ layout
+
+// One block-wide exclusive scan of a value per thread, saturating at `cap` (cap < 2^31, so
+// a sum of two saturated values fits 32 unsigned bits; min(a + b, cap) is associative for
+// non-negative values).  `warp_sums` holds one word per warp.
+template <int THREADS>
+__device__ uint32_t scan_exclusive(uint32_t v, uint32_t cap, uint32_t* warp_sums, uint32_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t inc = min(v, cap);
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc = min(inc + u, cap);
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w == warp) before = all;
+        all = min(all + warp_sums[w], cap);
+    }
+    __syncthreads();
+    *total = all;
+    const uint32_t ex = __shfl_up_sync(0xffffffffu, inc, 1);
+    return lane == 0 ? before : min(before + ex, cap);
+}
+
+constexpr int kLayoutThreads = 512;
+constexpr int kLayoutRows = 4;  // consecutive rows per thread: 16-byte stores of slots and positions
+
+__device__ __forceinline__ int32_t ceil_div(int32_t a, int32_t b) { return a / b + (a % b != 0); }
+
+// Places new_lens[b] tokens behind seq_lens[b] for every request.  A request is placed whole or
+// not at all: it needs its rows inside [0, rows), its pages inside its table row, and its
+// new pages among the free ones, handed out from the end of the list in request order
+// (a request that does not fit keeps its share of the order, so the outcome depends on the
+// lengths alone).
+//
+// Bound by latency: every CTA scans the lengths of all requests for itself (two scans of at most
+// kMaxRequests values, no traffic between CTAs and no second launch), then writes 16 bytes of
+// slots and of positions per thread.  New table entries are written by the row that opens the
+// page; entries that the scan reads and entries that it writes are never the same.
+__global__ void __launch_bounds__(kLayoutThreads) kv_layout(const LayoutParams p) {
+    extern __shared__ int32_t sm[];
+    __shared__ uint32_t warp_sums[kLayoutThreads / 32];
+    int32_t* s_end = sm;              // end of request b's rows
+    int32_t* s_take = sm + p.batch;   // free pages handed out before b; -1: not placed
+    const int per = (p.batch + kLayoutThreads - 1) / kLayoutThreads;
+    const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
+    const int count = min(max(p.free_count[0], 0), p.free_cap);
+    const uint32_t row_cap = (uint32_t)p.rows + 1, page_cap = (uint32_t)count + 1;
+
+    uint32_t sum = 0;
+    for (int b = b0; b < b1; ++b) sum = min(sum + min((uint32_t)max(p.new_lens[b], 0), row_cap), row_cap);
+    uint32_t total;
+    uint32_t end = scan_exclusive<kLayoutThreads>(sum, row_cap, warp_sums, &total);
+    uint32_t pages = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int have = max(p.seq_lens[b], 0), want = max(p.new_lens[b], 0);
+        end = min(end + min((uint32_t)want, row_cap), row_cap);
+        const bool fits = end <= (uint32_t)p.rows && (long long)have + want <= (long long)p.width * p.page_size;
+        const int need = fits ? ceil_div(have + want, p.page_size) - ceil_div(have, p.page_size) : -1;
+        s_end[b] = (int32_t)min(end, (uint32_t)p.rows);
+        s_take[b] = need;
+        pages = min(pages + (uint32_t)max(need, 0), page_cap);
+    }
+    uint32_t take = scan_exclusive<kLayoutThreads>(pages, page_cap, warp_sums, &total);
+    uint32_t used = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int need = s_take[b];
+        const uint32_t before = take;
+        take = min(take + (uint32_t)max(need, 0), page_cap);
+        const bool ok = need == 0 || (need > 0 && take <= (uint32_t)count);
+        s_take[b] = ok ? (int32_t)before : -1;
+        used += ok ? (uint32_t)need : 0;
+        if (blockIdx.x == 0) {
+            const int have = max(p.seq_lens[b], 0), want = max(p.new_lens[b], 0);
+            p.kv_lens[b] = ok ? have + want : 0;
+            p.placed[b] = ok ? want : 0;
+            p.next_seq_lens[b] = ok ? have + want : have;
+            p.cu[b + 1] = s_end[b];
+            if (b == 0) p.cu[0] = 0;
+        }
+    }
+    if (blockIdx.x == 0) {
+        scan_exclusive<kLayoutThreads>(used, page_cap, warp_sums, &total);
+        if (threadIdx.x == 0) {
+            p.next_free_count[0] = count - (int32_t)total;
+            if (p.batch == 0) p.cu[0] = 0;
+        }
+    } else {
+        __syncthreads();
+    }
+
+    for (long long r0 = ((long long)blockIdx.x * kLayoutThreads + threadIdx.x) * kLayoutRows; r0 < p.rows;
+         r0 += (long long)gridDim.x * kLayoutThreads * kLayoutRows) {
+        int lo = 0, hi = p.batch;  // the first request whose rows end behind r0
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (s_end[mid] > r0) hi = mid; else lo = mid + 1;
+        }
+        int slot[kLayoutRows], pos[kLayoutRows];
+#pragma unroll
+        for (int i = 0; i < kLayoutRows; ++i) {
+            const int r = (int)r0 + i;
+            slot[i] = pos[i] = -1;
+            while (lo < p.batch && s_end[lo] <= r) ++lo;
+            if (lo >= p.batch || s_take[lo] < 0) continue;
+            const int have = max(p.seq_lens[lo], 0);
+            const int at = have + r - (lo == 0 ? 0 : s_end[lo - 1]);
+            const int pi = at / p.page_size, held = ceil_div(have, p.page_size), in = at - pi * p.page_size;
+            int32_t* entry = p.table + (long long)lo * p.width + pi;
+            int page;
+            if (pi < held) {
+                page = *entry;
+            } else {
+                page = p.free_pages[count - 1 - (s_take[lo] + pi - held)];
+                if (in == 0) *entry = page;
+            }
+            const long long s = (long long)page * p.page_size + in;
+            pos[i] = at;
+            slot[i] = page >= 0 && s <= 0x7fffffffll ? (int)s : -1;
+        }
+        if (r0 + kLayoutRows <= p.rows) {
+            *reinterpret_cast<int4*>(p.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            *reinterpret_cast<int4*>(p.positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+            for (int i = 0; r0 + i < p.rows; ++i) {
+                p.slots[r0 + i] = slot[i];
+                p.positions[r0 + i] = pos[i];
+            }
+        }
+    }
+}
+
+// Puts every page of the marked requests at the end of the free list, in request order, and
+// sets their lengths to zero.  Same scan as kv_layout; the warps of the grid copy the rows.
+__global__ void __launch_bounds__(kLayoutThreads) kv_release(const ReleaseParams p) {
+    extern __shared__ int32_t sm[];
+    __shared__ uint32_t warp_sums[kLayoutThreads / 32];
+    const int per = (p.batch + kLayoutThreads - 1) / kLayoutThreads;
+    const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
+    const int count = min(max(p.free_count[0], 0), p.free_cap);
+    const uint32_t cap = (uint32_t)(p.free_cap - count);  // a list that is full drops the rest
+    auto held = [&](int b) {
+        if (!p.mask[b]) return 0;
+        return min(ceil_div(max(p.seq_lens[b], 0), p.page_size), p.width);
+    };
+    uint32_t sum = 0, total;
+    for (int b = b0; b < b1; ++b) sum = min(sum + (uint32_t)held(b), cap);
+    uint32_t at = scan_exclusive<kLayoutThreads>(sum, cap, warp_sums, &total);
+    for (int b = b0; b < b1; ++b) {
+        sm[b] = (int32_t)at;
+        at = min(at + (uint32_t)held(b), cap);
+        if (blockIdx.x == 0) p.next_seq_lens[b] = p.mask[b] ? 0 : max(p.seq_lens[b], 0);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.next_free_count[0] = count + (int32_t)total;
+    __syncthreads();
+    const int warps = kLayoutThreads / 32, lane = threadIdx.x & 31;
+    for (int b = blockIdx.x * warps + (threadIdx.x >> 5); b < p.batch; b += gridDim.x * warps) {
+        const int n = held(b), to = sm[b];
+        for (int i = lane; i < n && to + i < (int)cap; i += 32)
+            p.free_pages[count + to + i] = p.table[(long long)b * p.width + i];
+    }
+}
+
+// ------------------------------------------------------------------ rows
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+__device__ __forceinline__ uint8_t* block_of(const Pool& pool, int d, int slot, int head, int* row) {
+    const int block = slot / kBlock;
+    *row = slot - block * kBlock;
+    const int page = block / pool.page_blocks, in = block - page * pool.page_blocks;
+    return pool.data + (((long long)page * pool.kv_heads + head) * pool.page_blocks + in) * block_bytes(d);
+}
+
+__device__ __forceinline__ bool slot_ok(const Pool& pool, int slot) {
+    return slot >= 0 && slot / (kBlock * pool.page_blocks) < pool.pages;
+}
+
+// Quantises one row held by LANES lanes, 8 elements a lane, and stores it.  With lo = min(row, 0)
+// and hi = max(row, 0): scale = hi/15 - lo/15 (products with fp32 1/15, so that opposite extremes
+// of bf16 do not overflow) with its low four bits cleared, z = rint(-lo / scale), code =
+// clamp(rint(x / scale) + z, 0, 15); quotients are fp32 products with 1 / scale.  Every operation
+// is the IEEE one (no contraction), so the codes are a function of the row alone.  A scale
+// below the smallest normal number stores zeros; a row with an infinity or a NaN stores NaN.
+template <int LANES>
+__device__ __forceinline__ void store_row(const float (&x)[8], int lane, uint8_t* codes, uint8_t* word) {
+    float hi = 0.f, lo = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi = fmaxf(hi, x[i]);
+        lo = fminf(lo, x[i]);
+        finite &= fabsf(x[i]) < INFINITY;
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o /= 2) {
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        finite &= __shfl_xor_sync(0xffffffffu, (int)finite, o) != 0;
+    }
+    constexpr float k15 = 1.0f / 15.0f;
+    float scale = __fsub_rn(__fmul_rn(hi, k15), __fmul_rn(lo, k15));
+    scale = __uint_as_float(__float_as_uint(scale) & ~15u);
+    const bool normal = finite && scale >= 1.17549435e-38f;
+    const float inv = normal ? __frcp_rn(scale) : 0.f;
+    const float z = normal ? rintf(__fmul_rn(-lo, inv)) : 0.f;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float c = fminf(fmaxf(__fadd_rn(rintf(__fmul_rn(x[i], inv)), z), 0.f), 15.f);
+        w |= (normal ? (uint32_t)c : 0u) << (4 * i);
+    }
+    if (lane >= 0) {
+        reinterpret_cast<uint32_t*>(codes)[lane] = w;
+        if (lane == 0)
+            *reinterpret_cast<uint32_t*>(word) =
+                normal ? __float_as_uint(scale) | (uint32_t)z : (finite ? 0u : 0x7fc00000u);
+    }
+}
+
+constexpr int kRowThreads = 256;
+
+// One group of d / 8 lanes per (token, head): the group loads 16 bytes a lane of the K and of the
+// V row, reduces the extremes by shuffles and stores one 32-bit word of codes a lane.  Bound by
+// memory: 4d bytes read and d + 8 written a (token, head).
+template <int D, typename T, bool VECTOR>
+__global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
+    constexpr int LANES = D / 8, GROUPS = kRowThreads / LANES;
+    const long long item = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
+    const long long items = (long long)p.rows * p.pool.kv_heads;
+    const bool inside = item < items;
+    const int token = inside ? (int)(item / p.pool.kv_heads) : 0;
+    const int head = inside ? (int)(item - (long long)token * p.pool.kv_heads) : 0;
+    const int slot = inside ? p.slots[token] : -1;
+    const bool keep = slot_ok(p.pool, slot);
+    float k[8], v[8];
+    const T* kp = static_cast<const T*>(p.k) + token * p.k_token + head * p.k_head + lane * 8;
+    const T* vp = static_cast<const T*>(p.v) + token * p.v_token + head * p.v_head + lane * 8;
+    if (keep) {
+        if (VECTOR) {
+            const uint4 a = *reinterpret_cast<const uint4*>(kp), b = *reinterpret_cast<const uint4*>(vp);
+            const T* at = reinterpret_cast<const T*>(&a);
+            const T* bt = reinterpret_cast<const T*>(&b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                k[i] = to_float<T>(at[i]);
+                v[i] = to_float<T>(bt[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                k[i] = to_float<T>(kp[i]);
+                v[i] = to_float<T>(vp[i]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+    }
+    int row = 0;
+    uint8_t* block = keep ? block_of(p.pool, D, slot, head, &row) : p.pool.data;
+    const int who = keep ? lane : -1;  // every lane takes part in the shuffles
+    store_row<LANES>(k, who, block + row * row_bytes(D), block + k_words_at(D) + 4 * row);
+    store_row<LANES>(v, who, block + v_codes_at(D) + row * row_bytes(D), block + v_words_at(D) + 4 * row);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* to, const float (&x)[8]);
+template <>
+__device__ __forceinline__ void store8<float>(float* to, const float (&x)[8]) {
+    reinterpret_cast<float4*>(to)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(to)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <>
+__device__ __forceinline__ void store8<__half>(__half* to, const float (&x)[8]) {
+    __half2 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
+}
+template <>
+__device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* to, const float (&x)[8]) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
+}
+
+__device__ __forceinline__ void load_row(const uint8_t* codes, const uint8_t* word, int lane, float (&x)[8]) {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[lane];
+    const uint32_t sw = *reinterpret_cast<const uint32_t*>(word);
+    const float scale = __uint_as_float(sw & ~15u);
+    const int z = (int)(sw & 15u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(scale, (float)((int)((w >> (4 * i)) & 15u) - z));
+}
+
+// The rows of `slots` as values, rounded once to the output's type; a slot outside the pool reads
+// as zeros.  The inverse of kv4_append, with the same lanes; bound by the bytes it writes.
+template <int D, typename T>
+__global__ void __launch_bounds__(kRowThreads) kv4_read(const RowsParams p) {
+    constexpr int LANES = D / 8, GROUPS = kRowThreads / LANES;
+    const long long item = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
+    if (item >= (long long)p.rows * p.pool.kv_heads) return;
+    const int token = (int)(item / p.pool.kv_heads), head = (int)(item - (long long)token * p.pool.kv_heads);
+    const int slot = p.slots[token];
+    float k[8], v[8];
+    if (slot_ok(p.pool, slot)) {
+        int row;
+        const uint8_t* block = block_of(p.pool, D, slot, head, &row);
+        load_row(block + row * row_bytes(D), block + k_words_at(D) + 4 * row, lane, k);
+        load_row(block + v_codes_at(D) + row * row_bytes(D), block + v_words_at(D) + 4 * row, lane, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+    }
+    store8<T>(static_cast<T*>(p.k) + token * p.k_token + head * p.k_head + lane * 8, k);
+    store8<T>(static_cast<T*>(p.v) + token * p.v_token + head * p.v_head + lane * 8, v);
+}
+
+unsigned row_blocks(int d, const RowsParams& p) {
+    const long long groups = kRowThreads / (d / 8);
+    return (unsigned)(((long long)p.rows * p.pool.kv_heads + groups - 1) / groups);
+}
+
+template <int D, typename T>
+void append_of(bool vector, const RowsParams& p, cudaStream_t stream) {
+    if (vector)
+        kv4_append<D, T, true><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+    else
+        kv4_append<D, T, false><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+}
+
+template <int D>
+void read_of(int out_dtype, const RowsParams& p, cudaStream_t stream) {
+    if (out_dtype == LCA_DTYPE_F32)
+        kv4_read<D, float><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+    else if (out_dtype == LCA_DTYPE_F16)
+        kv4_read<D, __half><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+    else
+        kv4_read<D, __nv_bfloat16><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+}
+
+}  // namespace
+
+cudaError_t launch_layout(const LayoutParams& p, cudaStream_t stream) {
+    const int blocks = std::max(1, std::min(148, (p.rows + kLayoutThreads * kLayoutRows - 1) /
+                                                     (kLayoutThreads * kLayoutRows)));
+    const size_t smem = 2 * sizeof(int32_t) * (size_t)p.batch;
+    static_assert(2 * sizeof(int32_t) * kMaxRequests <= 64 * 1024, "shared memory of the scan");
+    if (smem > 40 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kv_layout, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
+        if (e != cudaSuccess) return e;
+    }
+    kv_layout<<<blocks, kLayoutThreads, smem, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_release(const ReleaseParams& p, cudaStream_t stream) {
+    const int blocks = std::max(1, std::min(148, (p.batch + kLayoutThreads / 32 - 1) / (kLayoutThreads / 32)));
+    static_assert(sizeof(int32_t) * kMaxRequests <= 40 * 1024, "shared memory of the scan");
+    kv_release<<<blocks, kLayoutThreads, sizeof(int32_t) * (size_t)p.batch, stream>>>(p);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_append(int d, int dtype, bool vector, const RowsParams& p, cudaStream_t stream) {
+    if (d == 64)
+        dtype == LCA_DTYPE_F16 ? append_of<64, __half>(vector, p, stream) : append_of<64, __nv_bfloat16>(vector, p, stream);
+    else
+        dtype == LCA_DTYPE_F16 ? append_of<128, __half>(vector, p, stream)
+                               : append_of<128, __nv_bfloat16>(vector, p, stream);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_read(int d, int out_dtype, const RowsParams& p, cudaStream_t stream) {
+    d == 64 ? read_of<64>(out_dtype, p, stream) : read_of<128>(out_dtype, p, stream);
+    return cudaGetLastError();
+}
+
+}  // namespace kv4
+}  // namespace lca

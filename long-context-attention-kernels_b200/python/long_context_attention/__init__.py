@@ -19,9 +19,12 @@ from typing import Sequence
 import torch
 
 from ._native import extension, native_error
+from .kv_cache import (KVCacheStep, QuantizedKVCache, kv_cache_append, kv_cache_layout, kv_cache_pool, kv_cache_read,
+                       kv_cache_release, sliding_window_attention_cached)
 
 __all__ = ["sliding_window_attention", "sliding_window_attention_with_lse", "sliding_window_attention_varlen",
-           "sliding_window_attention_backward"]
+           "sliding_window_attention_backward", "sliding_window_attention_cached", "QuantizedKVCache", "KVCacheStep",
+           "kv_cache_pool", "kv_cache_layout", "kv_cache_release", "kv_cache_append", "kv_cache_read"]
 
 
 def _reference_sliding_window_attention(

@@ -118,6 +118,18 @@ class CABI:
         lib.lca_swa_backward.restype = ctypes.c_int
         lib.lca_swa_backward.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_int, i64, i64, i64, i64, i64,
                                          ctypes.c_float, ctypes.POINTER(i64), i64, vp, sz, vp]
+        f32, ci = ctypes.c_float, ctypes.c_int
+        for name, args in {
+            "lca_kv_layout": [vp, i64, i64, vp, vp, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp, vp],
+            "lca_kv_release": [vp, i64, i64, vp, vp, vp, i64, vp, i64, vp, vp, vp],
+            "lca_kv4_append": [vp, i64, i64, i64, i64, vp, vp, ci, i64, i64, i64, i64, vp, i64, vp],
+            "lca_kv4_read": [vp, i64, i64, i64, i64, vp, i64, vp, vp, ci, vp],
+            "lca_swa_cached_workspace_size": [i64] * 8 + [ctypes.POINTER(sz)],
+            "lca_swa_forward_cached": [vp, ci, i64, i64, i64, i64, vp, i64, i64, i64, i64, vp, i64, i64, vp, vp, i64,
+                                       ctypes.POINTER(i64), i64, f32, vp, ci, vp, vp, sz, vp],
+        }.items():
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = args
         dp, lp = ctypes.POINTER(ShardDesc), ctypes.POINTER(ShardLayout)
         lib.lca_swa_shard_layout.restype = ctypes.c_int
         lib.lca_swa_shard_layout.argtypes = [dp, i64, lp]

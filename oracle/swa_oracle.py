@@ -210,3 +210,111 @@ def sliding_window_attention_backward_banded(Q, K, V, dO, window_size: int, glob
             if g.size:
                 rows_pass(b, h, g, np.arange(n, dtype=np.int64), np.ones((g.size, n), dtype=bool))
     return dQ, dK, dV
+
+
+# ---------------------------------------------------------------- paged 4-bit KV cache
+
+
+def kv4_quantize(x: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
+    """Rows [..., d] -> (codes uint8 [..., d], scale fp32 [...], zero point uint8 [...]) of the 4-bit
+    cache (include/lca.h): fp32 arithmetic step by step, as the format is defined."""
+    x = np.asarray(x, dtype=np.float32)
+    f = np.float32
+    with np.errstate(all="ignore"):
+        finite = np.isfinite(x).all(-1)
+        hi = np.maximum(np.nanmax(x, axis=-1, initial=0), f(0))
+        lo = np.minimum(np.nanmin(x, axis=-1, initial=0), f(0))
+        fifteenth = f(1) / f(15)
+        scale = (hi * fifteenth - lo * fifteenth).astype(np.float32)
+        scale = (scale.view(np.uint32) & np.uint32(0xFFFFFFF0)).view(np.float32)
+        normal = finite & (scale >= np.finfo(np.float32).tiny)
+        inv = np.where(normal, f(1) / scale, f(0)).astype(np.float32)
+        zero = np.where(normal, np.rint(-lo * inv), f(0)).astype(np.float32)
+        codes = np.clip(np.rint(x * inv[..., None]) + zero[..., None], 0, 15)
+        codes = np.where(normal[..., None], codes, 0).astype(np.uint8)
+    scale = np.where(normal, scale, np.where(finite, f(0), f(np.nan))).astype(np.float32)
+    return codes, scale, zero.astype(np.uint8)
+
+
+def kv4_values(x: np.ndarray) -> np.ndarray:
+    """What rows [..., d] read back as, fp64."""
+    codes, scale, zero = kv4_quantize(x)
+    return scale[..., None].astype(np.float64) * (codes.astype(np.int64) - zero[..., None])
+
+
+def kv4_block(k: np.ndarray, v: np.ndarray) -> np.ndarray:
+    """The bytes of one block: 16 tokens of one head, k and v [16, d]."""
+    parts, words = [], []
+    for x in (k, v):
+        codes, scale, zero = kv4_quantize(x)
+        c = codes.reshape(16, -1, 2)
+        parts.append((c[..., 0] | (c[..., 1] << 4)).astype(np.uint8).reshape(-1))
+        w = np.where(np.isnan(scale), np.uint32(0x7FC00000), scale.view(np.uint32) | zero)
+        words.append(w.astype("<u4").view(np.uint8))
+    return np.concatenate(parts + words)
+
+
+def kv_layout(block_table, seq_lens, new_lens, free_pages, free_count, page_size, num_tokens) -> dict:
+    """Block table, slots and lengths of one step, request by request (lca_kv_layout)."""
+    table = np.array(block_table, dtype=np.int64)
+    batch, width = table.shape
+    count = min(max(int(free_count), 0), len(free_pages))
+    slots, positions = np.full(num_tokens, -1, np.int64), np.full(num_tokens, -1, np.int64)
+    cu, kv_lens, placed, after = [0], [], [], []
+    end = asked = given = 0
+    for b in range(batch):
+        have, want = max(int(seq_lens[b]), 0), max(int(new_lens[b]), 0)
+        start = min(end, num_tokens)
+        end += want
+        held = -(-have // page_size)
+        ok = end <= num_tokens and have + want <= width * page_size
+        need = -(-(have + want) // page_size) - held if ok else 0
+        first = asked
+        asked += need
+        ok = ok and (need == 0 or asked <= count)
+        cu.append(min(end, num_tokens))
+        if ok:
+            given += need
+            for i in range(need):
+                table[b, held + i] = free_pages[count - 1 - first - i]
+            for i in range(want):
+                p = have + i
+                page = int(table[b, p // page_size])
+                positions[start + i] = p
+                s = page * page_size + p % page_size
+                slots[start + i] = s if page >= 0 and s < 2 ** 31 else -1
+        kv_lens.append(have + want if ok else 0)
+        placed.append(want if ok else 0)
+        after.append(have + want if ok else have)
+    return dict(block_table=table, slots=slots, positions=positions, cu_seqlens=np.array(cu), kv_lens=np.array(kv_lens),
+                placed=np.array(placed), seq_lens=np.array(after), free_count=np.array([count - given]))
+
+
+def cached_attention(q, k, v, window, global_tokens, scale):
+    """One request's new rows over its cached keys, fp64: q [n, heads, d] are the last n of the len
+    tokens k, v [len, kv_heads, d] (values, as read back).  Returns (O [n, heads, d], LSE [heads, n],
+    A, S): A is the same average of |v|, S [heads, n] the largest scale * sum |q_d k_jd| over the row's
+    visible keys, the quantities error bounds are made of."""
+    q, k, v = (np.asarray(t, dtype=np.float64) for t in (q, k, v))
+    n, heads, d = q.shape
+    length, kv_heads = k.shape[:2]
+    pos = length - n + np.arange(n)
+    key = np.arange(length)
+    glob = np.isin(key, list(global_tokens))
+    row_glob = np.isin(pos, list(global_tokens))
+    seen = (key[None, :] <= pos[:, None]) & ((pos[:, None] - key[None, :] <= window) | glob[None, :] | row_glob[:, None])
+    out, mean = np.zeros((n, heads, d)), np.zeros((n, heads, d))
+    lse, size = np.full((heads, n), -np.inf), np.zeros((heads, n))
+    for h in range(heads):
+        kh, vh = k[:, h // (heads // kv_heads)], v[:, h // (heads // kv_heads)]
+        x = np.where(seen, scale * (q[:, h] @ kh.T), -np.inf) if length else np.full((n, 0), -np.inf)
+        for i in range(n):
+            at = np.flatnonzero(seen[i]) if length else []
+            if len(at) == 0:
+                continue
+            m = x[i, at].max()
+            e = np.exp(x[i, at] - m)
+            out[i, h], mean[i, h] = e @ vh[at] / e.sum(), e @ np.abs(vh[at]) / e.sum()
+            lse[h, i] = m + np.log(e.sum())
+            size[h, i] = abs(scale) * (np.abs(kh[at]) @ np.abs(q[i, h])).max()
+    return out, lse, mean, size
