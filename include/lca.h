@@ -53,7 +53,8 @@ enum {
     LCA_DEVERR_TIMEOUT_SOFTMAX = 3,  /* main kernel: a softmax warp waited for S or O */
     LCA_DEVERR_TIMEOUT_DRAIN = 4,    /* main kernel: waiting for its own copies at exit */
     LCA_DEVERR_TIMEOUT_PEER = 5,     /* peer exchange: another rank's data did not arrive */
-    LCA_DEVERR_TIMEOUT_BACKWARD = 6  /* backward kernel: waited for a tile or an MMA */
+    LCA_DEVERR_TIMEOUT_BACKWARD = 6, /* backward kernel: waited for a tile or an MMA */
+    LCA_DEVERR_TIMEOUT_CACHE = 7     /* cached attention: a copy out of the pool did not arrive */
 };
 
 /* Element types: Q, K, V share LCA_DTYPE_F16 or LCA_DTYPE_BF16; the output is fp32

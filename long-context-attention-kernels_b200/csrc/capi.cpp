@@ -401,11 +401,10 @@ unsigned long long wait_timeout_ns() {
 
 }  // namespace
 
-int lca::device_info(int* sms, int** err_word, unsigned long long* wait_ns) {
+int lca::device_info(int** err_word, unsigned long long* wait_ns) {
     int dev = 0;
     const int st = check_device(&dev, err_word);
     if (st != LCA_OK) return st;
-    *sms = g_dev_sms[dev];
     *wait_ns = wait_timeout_ns();
     return LCA_OK;
 }

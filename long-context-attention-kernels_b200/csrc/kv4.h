@@ -75,20 +75,36 @@ struct AttnParams {
     int rows, heads, group;  // query rows, query heads, query heads per KV head
     int window, num_globals;
     float scale;
+    int bf16, out_dtype;
     void* out;   // [rows][heads][d]
     float* lse;  // [heads][rows] or NULL
+    int ctas, split;  // CTAs that share the line of tiles; whether items may be cut between them
+    long long items;  // at most this many items
+    float* part_o;    // [ctas][2][tile rows][d]: the parts of cut items, and
+    float2* part_ml;  // [ctas][2][tile rows]: their maxima and sums
+    int* err_word;
+    unsigned long long wait_ns;
+};
+
+struct AttnPlan {
+    int q_tiles;  // groups of 8 query rows a tile
+    int ctas;
+    bool split;
+    int64_t items;
+    size_t part_o, part_ml;  // bytes
 };
 
 cudaError_t launch_layout(const LayoutParams& p, cudaStream_t stream);
 cudaError_t launch_release(const ReleaseParams& p, cudaStream_t stream);
 cudaError_t launch_append(int d, int dtype, bool vector, const RowsParams& p, cudaStream_t stream);
 cudaError_t launch_read(int d, int out_dtype, const RowsParams& p, cudaStream_t stream);
-cudaError_t launch_attention(int d, int dtype, int out_dtype, const AttnParams& p, const Globals& g,
-                             cudaStream_t stream);
+AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t batch, int64_t capacity,
+                        int64_t window, int64_t num_globals);
+cudaError_t launch_attention(int d, int q_tiles, const AttnParams& p, const Globals& g, cudaStream_t stream);
 
 }  // namespace kv4
 
-// capi.cpp: checks the current device; its SM count, error word and wait limit.
-int device_info(int* sms, int** err_word, unsigned long long* wait_ns);
+// capi.cpp: checks the current device; its error word and wait limit.
+int device_info(int** err_word, unsigned long long* wait_ns);
 
 }  // namespace lca

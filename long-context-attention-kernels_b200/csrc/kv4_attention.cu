@@ -6,8 +6,14 @@
 // p = len - n + i and computes, over the keys j <= p with p - j <= window, or j or p global,
 //
 //   x_j = scale * sk_j * sum_d q_d (ck_jd - zk_j),   O_d = sum_j e^(x_j - m) sv_j (cv_jd - zv_j) / l.
+//
+// The integers c - z are exact in fp16, so both products run on the tensor cores over them
+// (mma.sync m16n8k16, keys by queries and elements by queries, fp32 sums) and the scales stay in
+// fp32, outside the products: sk multiplies a finished score, sv the weight of its key.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "kv4.h"
 #include "sm100_ptx.cuh"
@@ -16,11 +22,16 @@ namespace lca {
 namespace kv4 {
 namespace {
 
-__device__ __forceinline__ float load_f(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ float load_f(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void store_f(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_f(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void store_f(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = 32;    // keys per tile: two blocks, one warp's step
+constexpr int kStages = 3;   // tiles in flight per warp
+constexpr int kMinTiles = 8; // least tiles of a CTA where items are split
+constexpr int kWholeTiles = 48;  // items of up to this many tiles are not split
+constexpr int kSms = 148;
+
+constexpr uint32_t kAll = 0xffffffffu;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int lower_bound(const int32_t* a, int n, int v) {
     int lo = 0;
@@ -31,113 +42,847 @@ __device__ __forceinline__ int lower_bound(const int32_t* a, int n, int v) {
     return lo;
 }
 
-// One warp per (query row, head): a lane per key for the scores, then d / 32 elements a lane
-// for the product with V.
-template <int D, typename T, typename O>
-__global__ void __launch_bounds__(128) kv4_attention_rows(const AttnParams p, const __grid_constant__ Globals g) {
-    __shared__ float s_q[4][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + warp;
-    if (item >= (long long)p.rows * p.heads) return;
-    const int r = (int)(item / p.heads), head = (int)(item - (long long)r * p.heads), kv_head = head / p.group;
-    if (r >= p.cu[p.batch] || r < p.cu[0]) return;  // rows outside the requests stay as they were
-    int b = 0, hi = p.batch;
-    while (b < hi) {
-        const int mid = (b + hi) >> 1;
-        if (p.cu[mid + 1] > r) hi = mid; else b = mid + 1;
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     ptx::smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
+// Two codes minus their zero points as a pair of fp16, from the nibbles at bits 0 and 16 (LOW) or 4
+// and 20 of w.  0x6400 | c is 1024 + c; 0x6400 | 16 c is 1024 + 16 c, a sixteenth of which is 64 + c.
+// z holds the fp16 pairs 1024 + zp and -(64 + zp); every step is exact.
+struct Zero {
+    uint32_t low, high;
+};
+
+__device__ __forceinline__ Zero zero_pair(uint32_t word0, uint32_t word1) {
+    const uint32_t z = (word0 & 15u) | ((word1 & 15u) << 16);
+    return {0x64006400u + z, 0xd400d400u + (z << 4)};
+}
+
+__device__ __forceinline__ uint32_t codes_low(uint32_t w, const Zero& z) {
+    return hsub2((w & 0x000f000fu) | 0x64006400u, z.low);
+}
+
+__device__ __forceinline__ uint32_t codes_high(uint32_t w, const Zero& z) {
+    return hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.high);
+}
+
+__device__ __forceinline__ uint32_t codes_pair(uint32_t w, int nibble, const Zero& z) {  // nibble: 0 .. 3, a constant
+    const uint32_t v = nibble >= 2 ? w >> 8 : w;
+    return (nibble & 1) ? codes_high(v, z) : codes_low(v, z);
+}
+
+// ------------------------------------------------------------------ the work of a call
+
+// An item is one (request, KV head, tile of 8 * NT query rows); rows of a request are ordered
+// token by token, and within a token by the query heads of the group.  Its keys are whole
+// tiles of 32 positions that cover the band of its rows, then tiles of 32 gathered
+// global tokens in front of the band.  Request b has `items` items of at most `tiles` tiles
+// each (exactly `tiles` when it has one query tile per head); all its tiles, item after item and
+// request after request, form one line of tiles that the CTAs share out evenly.
+struct Request {
+    int q0, len, rows;      // first row of q, cached tokens, rows (tokens * group)
+    int q_tiles, tiles;
+};
+
+struct Span {
+    int first, band, globals, gathered;  // first band tile, band tiles, gathered keys and their tiles
+    int lo, hi;                          // positions of the first and the last row
+};
+
+template <int ROWS>
+__device__ __forceinline__ Span span_of(const AttnParams& p, const Globals& g, const Request& r, int q_tile) {
+    Span s;
+    const int n = r.rows / p.group;
+    const int from = q_tile * ROWS, to = min(from + ROWS, r.rows) - 1;
+    s.lo = r.len - n + from / p.group;
+    s.hi = r.len - n + to / p.group;
+    if (s.hi < 0) return {0, 0, 0, 0, s.lo, s.hi};
+    int lo = max(0, s.lo - p.window);
+    s.globals = 0;
+    if (p.num_globals > 0) {
+        if (lo > 0) {
+            const int at = lower_bound(g.at, p.num_globals, s.lo);
+            if (at < p.num_globals && g.at[at] <= s.hi) lo = 0;  // a global row sees every key up to itself
+        }
+        lo &= ~(kTile - 1);
+        s.globals = lower_bound(g.at, p.num_globals, lo);
     }
-    const long long cap = min((long long)p.width * p.pool.page_blocks * kBlock, 0x7fffffffll);
-    const int len = (int)min((long long)max(p.kv_lens[b], 0), cap);
-    const int pos = len - (p.cu[b + 1] - r);
-    for (int i = lane; i < D; i += 32) s_q[warp][i] = load_f(static_cast<const T*>(p.q) + r * p.q_token + head * p.q_head + i);
-    __syncwarp();
-    int lo = max(0, pos - p.window);
-    const int at = lower_bound(g.at, p.num_globals, pos);
-    if (at < p.num_globals && g.at[at] == pos) lo = 0;
-    const int before = lower_bound(g.at, p.num_globals, lo);
-    const int keys = pos < 0 ? 0 : before + pos + 1 - lo;
-    float m = -INFINITY, l = 0.f, acc[D / 32] = {};
-    for (int k0 = 0; k0 < keys; k0 += 32) {
-        const int k = k0 + lane;
-        float x = -INFINITY, sv = 0.f;
-        const uint8_t* vrow = nullptr;
-        int zv = 0;
-        if (k < keys) {
-            const int j = k < before ? g.at[k] : lo + k - before;
-            const int blk = j / kBlock, row = j % kBlock;
-            const int page = p.table[(long long)b * p.width + blk / p.pool.page_blocks];
-            if (page >= 0 && page < p.pool.pages) {
-                const uint8_t* block = p.pool.data + (((long long)page * p.pool.kv_heads + kv_head) * p.pool.page_blocks +
-                                                      blk % p.pool.page_blocks) * block_bytes(D);
-                const uint32_t wk = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row);
-                const uint32_t wv = *reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row);
-                const uint32_t* codes = reinterpret_cast<const uint32_t*>(block + row * row_bytes(D));
-                const int zk = wk & 15u;
-                float dot = 0.f;
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t c = codes[i];
-                    for (int e = 0; e < 8; ++e) dot += s_q[warp][8 * i + e] * (float)((int)((c >> (4 * e)) & 15u) - zk);
+    s.first = lo / kTile;
+    s.band = s.hi / kTile - s.first + 1;
+    s.gathered = (s.globals + kTile - 1) / kTile;
+    return s;
+}
+
+template <int ROWS>
+__device__ __forceinline__ Request request_of(const AttnParams& p, const Globals& g, int b) {
+    Request r = {0, 0, 0, 0, 0};
+    if (b >= p.batch) return r;
+    const int q0 = min(max(p.cu[b], 0), p.rows), q1 = min(max(p.cu[b + 1], 0), p.rows);
+    if (q1 <= q0) return r;
+    const int cap = p.width * p.pool.page_blocks * kBlock;
+    r.q0 = q0;
+    r.len = min(max(p.kv_lens[b], 0), cap);
+    r.rows = (q1 - q0) * p.group;
+    r.q_tiles = (r.rows + ROWS - 1) / ROWS;
+    Span s = span_of<ROWS>(p, g, r, r.q_tiles - 1);
+    r.tiles = s.band + s.gathered;
+    if (r.q_tiles > 1) {
+        // any tile: its rows lie within so many tokens, so its band within so many tiles; whole
+        // when one of the new tokens is global
+        const int tokens = (ROWS - 2) / p.group + 2;
+        int band = (int)min((long long)(p.window + tokens - 1) / kTile + 2, (long long)r.len / kTile + 1);
+        const int first = r.len - (q1 - q0);
+        const int at = lower_bound(g.at, p.num_globals, first);
+        if (at < p.num_globals && g.at[at] < r.len) band = r.len / kTile + 1;
+        r.tiles = band + (lower_bound(g.at, p.num_globals, max(0, r.len - p.window)) + kTile - 1) / kTile;
+    }
+    r.tiles = max(r.tiles, 1);
+    return r;
+}
+
+__device__ __forceinline__ long long line_of(const AttnParams& p, const Request& r) {
+    return (long long)r.q_tiles * p.pool.kv_heads * r.tiles;
+}
+
+// Block-wide: the sum of a value over the threads, and each thread's exclusive prefix.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long v, long long* scratch, long long* before) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const long long u = __shfl_up_sync(kAll, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    long long all = 0, mine = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w == warp) mine = all;
+        all += scratch[w];
+    }
+    __syncthreads();
+    *before = mine + inc - v;
+    return all;
+}
+
+struct Place {
+    int b;             // request
+    long long start;   // its first tile on the line
+};
+
+// The request that holds position `at` of the line, searched from `from` on, whose own part of the
+// line begins at `start`.  `at` lies on the line.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ Place locate(const AttnParams& p, const Globals& g, int from, long long start, long long at,
+                                        long long* scratch, Place* found) {
+    for (int b0 = from; b0 < p.batch; b0 += THREADS) {
+        const long long mine = line_of(p, request_of<ROWS>(p, g, b0 + (int)threadIdx.x));
+        long long before;
+        const long long all = block_scan<THREADS>(mine, scratch, &before);
+        if (at < start + all) {
+            if (start + before <= at && at < start + before + mine) *found = {b0 + (int)threadIdx.x, start + before};
+            __syncthreads();
+            const Place r = *found;
+            __syncthreads();
+            return r;
+        }
+        start += all;
+    }
+    return {p.batch, start};
+}
+
+template <int ROWS, int THREADS>
+__device__ __forceinline__ long long whole_line(const AttnParams& p, const Globals& g, long long* scratch) {
+    long long sum = 0, before;
+    for (int b = threadIdx.x; b < p.batch; b += THREADS) sum += line_of(p, request_of<ROWS>(p, g, b));
+    return block_scan<THREADS>(sum, scratch, &before);
+}
+
+__device__ __forceinline__ void store_out(const AttnParams& p, int out_dtype, long long at, const float (&v)[4]) {
+    if (out_dtype == LCA_DTYPE_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else if (out_dtype == LCA_DTYPE_F16) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
+template <int D, int NT>
+struct Cfg {
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int STAGE = 2 * block_bytes(D);
+    static constexpr int RING = kWarps * kStages * STAGE;
+    static constexpr int PITCH = D + 4;  // floats of one row in the merge buffer
+    static constexpr int MERGE = kWarps * ROWS * (PITCH + 2) * 4;
+    static constexpr int MAIN = RING > MERGE ? RING : MERGE;
+    static constexpr int SMEM = MAIN + kWarps * kStages * 12 + 128;
+};
+
+// Position of slot s of a block in the products: the codes of slots 2t and 2t + 1 (V) and of slots
+// g (K) are then read from shared memory with the fewest conflicts that a plain layout allows.
+__device__ __forceinline__ int slot_row(int s) { return s ^ ((s >> 1) & 1); }
+
+// One warp streams tiles of 32 keys through its own ring of bulk copies and keeps the running
+// softmax of 8 * NT query rows; the four warps of a CTA take the tiles of a segment in turn and
+// merge at its end.  Per tile: scores S^T = K Q^T (keys are the 16 rows of the product, queries
+// its 8 columns), weights, then O^T += V^T P^T.  The score fragment of a thread holds two
+// queries of a key; transposed 8 x 8 it is the second product's operand.
+//
+// M is the running maximum of x_j log2(e) + log2(sv_j), so that the weights w = p sv that enter the second
+// product as fp16 are at most 1 (2^8 between rescalings) whatever the sizes of V; p itself, which the
+// sum l takes, stays within 2^100 of it because log2(sv) is cut at -100.  Rounding: w to fp16
+// (2^-11); with an fp32 output the remainder w - fp16(w) goes through a second product (2^-22).
+template <int D, int NT, bool SPLIT_W>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
+    kv4_attention(const AttnParams p, const __grid_constant__ Globals g) {
+    using C = Cfg<D, NT>;
+    constexpr int STEPS = D / 16;  // products over d of a score, and 16-element tiles of O
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::MAIN);
+    uint32_t* masks = reinterpret_cast<uint32_t*>(bars + kWarps * kStages);
+    __shared__ long long scratch[kWarps];
+    __shared__ Place found;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
+    uint8_t* ring = smem + warp * kStages * C::STAGE;
+    uint64_t* bar = bars + warp * kStages;
+    volatile uint32_t* mask = masks + warp * kStages;
+    if (threadIdx.x < kWarps * kStages) ptx::mbar_init(&bars[threadIdx.x], 1);
+    if (threadIdx.x == 0) ptx::fence_mbar_init();
+    ptx::griddep_launch();
+
+    const long long line = whole_line<C::ROWS, kThreads>(p, g, scratch);
+    long long per = (line + gridDim.x - 1) / gridDim.x;
+    if (p.split) per = max(per, (long long)kMinTiles);
+    long long at = per * blockIdx.x;
+    const long long end = min(at + per, line);
+    if (at >= end) return;
+    Place here = locate<C::ROWS, kThreads>(p, g, 0, 0, at, scratch, &found);
+    Request r = request_of<C::ROWS>(p, g, here.b);
+    uint32_t done = 0;  // tiles this warp has taken from its ring since the start
+    bool ok = true;
+
+    while (here.b < p.batch) {
+        const long long in = at - here.start;
+        int item = (int)(in / r.tiles);
+        int t0 = (int)(in - (long long)item * r.tiles), t1 = r.tiles;
+        if (p.split) {
+            t1 = (int)min((long long)r.tiles, t0 + (end - at));
+        } else if (t0 > 0) {  // whole items only: this one belongs to the CTA before
+            ++item;
+            t0 = 0;
+            at = here.start + (long long)item * r.tiles;
+        }
+        if (at >= end) break;
+        const bool in_request = item < r.q_tiles * p.pool.kv_heads;
+        if (in_request) {
+            const int head = item / r.q_tiles, q_tile = item - head * r.q_tiles;
+            const Span span = span_of<C::ROWS>(p, g, r, q_tile);
+            const int tiles = min(t1, span.band + span.gathered);
+            const int mine = max(0, (tiles - t0 - warp + kWarps - 1) / kWarps);
+            const int32_t* table = p.table + (long long)here.b * p.width;
+
+            // ---- loads: tile t0 + warp + 4 i of the item into the ring
+            int pages = -1, pages_next = -1;  // page ids of 16 tiles of this warp, two blocks each
+            auto fetch_pages = [&](int i0) {
+                const int tile = t0 + warp + kWarps * (i0 + (lane >> 1));
+                const int block = 2 * (span.first + tile) + (lane & 1);
+                return i0 + (lane >> 1) < mine && tile < span.band && block <= span.hi / kBlock
+                           ? table[block / p.pool.page_blocks]
+                           : -1;
+            };
+            auto issue = [&](int i) {
+                if ((i & 15) == 0) {
+                    pages = i == 0 ? fetch_pages(0) : pages_next;
+                } else if ((i & 15) == 8) {
+                    pages_next = fetch_pages((i & ~15) + 16);
                 }
-                x = dot * __uint_as_float(wk & ~15u) * p.scale;
-                sv = __uint_as_float(wv & ~15u);
-                zv = wv & 15u;
-                vrow = block + v_codes_at(D) + row * row_bytes(D);
+                const int slot = (done + i) % kStages;
+                uint8_t* dst = ring + slot * C::STAGE;
+                const int tile = t0 + warp + kWarps * i;
+                if (tile < span.band) {
+                    const int page0 = __shfl_sync(kAll, pages, 2 * (i & 15)), page1 = __shfl_sync(kAll, pages, 2 * (i & 15) + 1);
+                    if (lane == 0) {
+                        const int block = 2 * (span.first + tile);
+                        const int in0 = block % p.pool.page_blocks, in1 = in0 + 1 == p.pool.page_blocks ? 0 : in0 + 1;
+                        const bool have0 = (unsigned)page0 < (unsigned)p.pool.pages,
+                                   have1 = (unsigned)page1 < (unsigned)p.pool.pages;
+                        const uint8_t* src0 =
+                            p.pool.data + (((long long)page0 * p.pool.kv_heads + head) * p.pool.page_blocks + in0) * block_bytes(D);
+                        const uint8_t* src1 =
+                            p.pool.data + (((long long)page1 * p.pool.kv_heads + head) * p.pool.page_blocks + in1) * block_bytes(D);
+                        mask[slot] = (have0 ? 0xffffu : 0u) | (have1 ? 0xffff0000u : 0u);
+                        ptx::mbar_arrive_expect_tx(&bar[slot], (have0 + have1) * block_bytes(D));
+                        if (have0 && have1 && src1 == src0 + block_bytes(D)) {
+                            bulk_load(dst, src0, 2 * block_bytes(D), &bar[slot]);
+                        } else {
+                            if (have0) bulk_load(dst, src0, block_bytes(D), &bar[slot]);
+                            if (have1) bulk_load(dst + block_bytes(D), src1, block_bytes(D), &bar[slot]);
+                        }
+                    }
+                } else {  // a lane per global token
+                    const int k = (tile - span.band) * kTile + lane;
+                    const uint8_t* src = nullptr;
+                    int row = 0;
+                    if (k < span.globals) {
+                        const int pos = g.at[k], block = pos / kBlock;
+                        row = pos % kBlock;
+                        const int page = table[block / p.pool.page_blocks];
+                        if ((unsigned)page < (unsigned)p.pool.pages)
+                            src = p.pool.data + (((long long)page * p.pool.kv_heads + head) * p.pool.page_blocks +
+                                                 block % p.pool.page_blocks) * block_bytes(D);
+                    }
+                    const uint32_t have = __ballot_sync(kAll, src != nullptr);
+                    uint8_t* to = dst + (lane >> 4) * block_bytes(D);
+                    const int to_row = lane & 15;
+                    if (src != nullptr) {
+                        *reinterpret_cast<uint32_t*>(to + k_words_at(D) + 4 * to_row) =
+                            *reinterpret_cast<const uint32_t*>(src + k_words_at(D) + 4 * row);
+                        *reinterpret_cast<uint32_t*>(to + v_words_at(D) + 4 * to_row) =
+                            *reinterpret_cast<const uint32_t*>(src + v_words_at(D) + 4 * row);
+                        ptx::fence_proxy_async_smem();  // a later copy may land on these words
+                    }
+                    if (lane == 0) {
+                        mask[slot] = have;
+                        ptx::mbar_arrive_expect_tx(&bar[slot], __popc(have) * D);
+                    }
+                    __syncwarp();
+                    if (src != nullptr) {
+                        bulk_load(to + to_row * row_bytes(D), src + row * row_bytes(D), row_bytes(D), &bar[slot]);
+                        bulk_load(to + v_codes_at(D) + to_row * row_bytes(D), src + v_codes_at(D) + row * row_bytes(D),
+                                  row_bytes(D), &bar[slot]);
+                    }
+                }
+                __syncwarp();
+            };
+            int issued = 0;
+            if (ok)
+                for (; issued < min(mine, kStages); ++issued) issue(issued);
+
+            // ---- queries: rows of the tile as the second operand, in the order of the K codes
+            uint32_t q[NT][STEPS][2];
+            float q_scale[NT][2];             // of this thread's two columns
+            int row_hi[NT][2], row_lo[NT][2];  // their positions and band starts
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int row = q_tile * C::ROWS + 8 * nt + gq;
+                uint32_t raw[D / 8];
+                if (row < r.rows) {
+                    const int token = row / p.group, of = row - token * p.group;
+                    const uint4* src = reinterpret_cast<const uint4*>(
+                        static_cast<const uint16_t*>(p.q) + (r.q0 + token) * p.q_token +
+                        (long long)(head * p.group + of) * p.q_head + t * (D / 4));
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint4 v = src[i];
+                        raw[4 * i] = v.x, raw[4 * i + 1] = v.y, raw[4 * i + 2] = v.z, raw[4 * i + 3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) raw[i] = 0;
+                }
+                // fp16 as it is; bf16 moved by a power of two that takes the row's largest element to
+                // [2^14, 2^15), where fp16 holds 8 bits of every element down to 2^-31 of it
+                float mult = p.scale * kLog2e;
+                uint32_t top = 0;
+                if (p.bf16) {
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+                    top = max(top, __shfl_xor_sync(kAll, top, 1));
+                    top = max(top, __shfl_xor_sync(kAll, top, 2));
+                    const int e = max((int)(top >> 7) - 127, -100);  // above 2^-100; smaller rows score 0
+                    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                    mult *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                        raw[i] = ptx::pack_f16x2(__uint_as_float(raw[i] << 16) * up,
+                                                 __uint_as_float(raw[i] & 0xffff0000u) * up);
+                    if (top >= 0x7f80u) mult = NAN;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+                    top = max(top, __shfl_xor_sync(kAll, top, 1));
+                    top = max(top, __shfl_xor_sync(kAll, top, 2));
+                    if (top >= 0x7c00u) mult = NAN;
+                }
+#pragma unroll
+                for (int w = 0; w < D / 32; ++w) {  // elements 8w .. 8w + 7 of this thread's chunk
+                    q[nt][2 * w][0] = __byte_perm(raw[4 * w], raw[4 * w + 2], 0x5410);
+                    q[nt][2 * w][1] = __byte_perm(raw[4 * w], raw[4 * w + 2], 0x7632);
+                    q[nt][2 * w + 1][0] = __byte_perm(raw[4 * w + 1], raw[4 * w + 3], 0x5410);
+                    q[nt][2 * w + 1][1] = __byte_perm(raw[4 * w + 1], raw[4 * w + 3], 0x7632);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    q_scale[nt][e] = __shfl_sync(kAll, mult, 4 * (2 * t + e));
+                    const int col = q_tile * C::ROWS + 8 * nt + 2 * t + e;
+                    const int pos = col < r.rows ? r.len - r.rows / p.group + col / p.group : -1;
+                    row_hi[nt][e] = pos;
+                    row_lo[nt][e] = max(0, pos - p.window);
+                    if (p.num_globals > 0 && span.first == 0) {
+                        const int k = lower_bound(g.at, p.num_globals, pos);
+                        if (k < p.num_globals && g.at[k] == pos) row_lo[nt][e] = 0;
+                    }
+                }
             }
+
+            float o[NT][STEPS][4], top[NT][2], sum[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                top[nt][0] = top[nt][1] = -INFINITY;
+                sum[nt][0] = sum[nt][1] = 0.f;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+            }
+
+#pragma unroll 1
+            for (int i = 0; i < issued; ++i) {
+                const int slot = (done + i) % kStages;
+                ok &= ptx::mbar_wait(&bar[slot], ((done + i) / kStages) & 1, nullptr, p.err_word,
+                                     LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
+                ok = __all_sync(kAll, ok);
+                if (!ok) continue;  // results are invalid; the copies still in flight are waited for
+                const uint8_t* stage = ring + slot * C::STAGE;
+                const int tile = t0 + warp + kWarps * i;
+                const int key0 = (span.first + tile) * kTile;
+                const uint32_t have = mask[slot];
+                const int row0 = slot_row(gq);
+
+                // ---- scores
+                float s[2][NT][4];
+                float sk[4], sv[4];
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const uint8_t* block = stage + m * block_bytes(D);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s[m][nt][0] = s[m][nt][1] = s[m][nt][2] = s[m][nt][3] = 0.f;
+                    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row0);
+                    const uint32_t w1 = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row0 + 32);
+                    sk[2 * m] = __uint_as_float(w0 & ~15u);
+                    sk[2 * m + 1] = __uint_as_float(w1 & ~15u);
+                    sv[2 * m] = __uint_as_float(*reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0) & ~15u);
+                    sv[2 * m + 1] =
+                        __uint_as_float(*reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0 + 32) & ~15u);
+                    const Zero z0 = zero_pair(w0, w0), z1 = zero_pair(w1, w1);
+                    uint32_t c0[D / 32], c1[D / 32];
+                    const uint8_t* at0 = block + row0 * row_bytes(D) + t * (D / 8);
+                    const uint8_t* at1 = at0 + 8 * row_bytes(D);
+                    if (D == 128) {
+                        *reinterpret_cast<uint4*>(c0) = *reinterpret_cast<const uint4*>(at0);
+                        *reinterpret_cast<uint4*>(c1) = *reinterpret_cast<const uint4*>(at1);
+                    } else {
+                        *reinterpret_cast<uint2*>(c0) = *reinterpret_cast<const uint2*>(at0);
+                        *reinterpret_cast<uint2*>(c1) = *reinterpret_cast<const uint2*>(at1);
+                    }
+#pragma unroll
+                    for (int w = 0; w < D / 32; ++w) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t a0 = codes_pair(c0[w], 2 * h, z0), a1 = codes_pair(c1[w], 2 * h, z1);
+                            const uint32_t a2 = codes_pair(c0[w], 2 * h + 1, z0), a3 = codes_pair(c1[w], 2 * h + 1, z1);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                mma(s[m][nt], a0, a1, a2, a3, q[nt][2 * w + h][0], q[nt][2 * w + h][1]);
+                        }
+                    }
+                }
+
+                // ---- visibility: nothing to do where the whole tile is visible to every row
+                const bool band = tile < span.band;
+                uint32_t seen[NT];  // bit 4 m + c of column pair nt
+                const bool full = have == kAll && (!band || (key0 + kTile - 1 <= span.lo && key0 >= span.hi - p.window));
+                if (full) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) seen[nt] = 0xffu;
+                } else {
+                    uint32_t glob = 0;  // global keys of the tile, which rows outside whose band they lie see
+                    if (band && p.num_globals > 0) {
+                        const int k = lower_bound(g.at, p.num_globals, key0 + lane);
+                        glob = __ballot_sync(kAll, k < p.num_globals && g.at[k] == key0 + lane);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        seen[nt] = 0;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {  // c = 4 m + 2 (second row) + column
+                            const int k = 16 * (c >> 2) + 8 * ((c >> 1) & 1) + row0, e = c & 1;
+                            const bool there = (have >> k) & 1;
+                            const int j = key0 + k;
+                            const bool vis = there && (band ? j <= row_hi[nt][e] && (j >= row_lo[nt][e] || ((glob >> k) & 1))
+                                                            : row_hi[nt][e] >= 0);
+                            seen[nt] |= (uint32_t)vis << c;
+                        }
+                    }
+                }
+
+                // ---- softmax
+                float lam[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) lam[c] = fmaxf(lg2(fabsf(sv[c])), -100.f);
+                float peak[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    peak[nt][0] = peak[nt][1] = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        float& x = s[c >> 2][nt][c & 3];
+                        x *= sk[c >> 1] * q_scale[nt][c & 1];
+                        if (!((seen[nt] >> c) & 1)) x = -INFINITY;
+                        peak[nt][c & 1] = fmaxf(peak[nt][c & 1], x + lam[c >> 1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (int m = 4; m < 32; m *= 2)
+                            peak[nt][e] = fmaxf(peak[nt][e], __shfl_xor_sync(kAll, peak[nt][e], m));
+                    }
+                }
+                bool raise = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) raise |= peak[nt][0] > top[nt][0] + 8.f || peak[nt][1] > top[nt][1] + 8.f;
+                if (__any_sync(kAll, raise)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float f[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float to = fmaxf(top[nt][e], peak[nt][e]);
+                            f[e] = to == -INFINITY ? 1.f : ptx::ex2(top[nt][e] - to);
+                            top[nt][e] = to;
+                            sum[nt][e] *= f[e];
+                        }
+#pragma unroll
+                        for (int k = 0; k < STEPS; ++k) {
+                            o[nt][k][0] *= f[0], o[nt][k][1] *= f[1];
+                            o[nt][k][2] *= f[0], o[nt][k][3] *= f[1];
+                        }
+                    }
+                }
+                uint32_t w_hi[NT][4], w_lo[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float ref0 = top[nt][0] == -INFINITY ? 0.f : top[nt][0];
+                    const float ref1 = top[nt][1] == -INFINITY ? 0.f : top[nt][1];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {  // key row c of this thread, both columns
+                        float* x = &s[c >> 1][nt][2 * (c & 1)];
+                        const float p0 = ptx::ex2(x[0] - ref0), p1 = ptx::ex2(x[1] - ref1);
+                        sum[nt][0] += p0;
+                        sum[nt][1] += p1;
+                        const float v0 = (seen[nt] >> (2 * c)) & 1 ? p0 * sv[c] : 0.f;
+                        const float v1 = (seen[nt] >> (2 * c + 1)) & 1 ? p1 * sv[c] : 0.f;
+                        const uint32_t hi = ptx::pack_f16x2(v0, v1);
+                        w_hi[nt][c] = transpose8(hi);
+                        if (SPLIT_W) {
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                            w_lo[nt][c] = transpose8(ptx::pack_f16x2(v0 - back.x, v1 - back.y));
+                        }
+                    }
+                }
+
+                // ---- product with V
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const uint8_t* block = stage + m * block_bytes(D);
+                    const int r0 = slot_row(2 * t), r1 = slot_row(2 * t + 1);
+                    const uint32_t* words = reinterpret_cast<const uint32_t*>(block + v_words_at(D));
+                    const Zero z01 = zero_pair(words[r0], words[r1]), z23 = zero_pair(words[r0 + 8], words[r1 + 8]);
+                    const uint8_t* codes = block + v_codes_at(D) + gq * (D / 16);
+                    // [half of the m-tile's rows][low or high 16 bits of a word]
+                    uint32_t a01[2][2], a23[2][2];
+                    if (D == 128) {
+                        const uint2 x0 = *reinterpret_cast<const uint2*>(codes + r0 * row_bytes(D));
+                        const uint2 x1 = *reinterpret_cast<const uint2*>(codes + r1 * row_bytes(D));
+                        const uint2 x2 = *reinterpret_cast<const uint2*>(codes + (r0 + 8) * row_bytes(D));
+                        const uint2 x3 = *reinterpret_cast<const uint2*>(codes + (r1 + 8) * row_bytes(D));
+                        a01[0][0] = __byte_perm(x0.x, x1.x, 0x5410), a01[0][1] = __byte_perm(x0.x, x1.x, 0x7632);
+                        a01[1][0] = __byte_perm(x0.y, x1.y, 0x5410), a01[1][1] = __byte_perm(x0.y, x1.y, 0x7632);
+                        a23[0][0] = __byte_perm(x2.x, x3.x, 0x5410), a23[0][1] = __byte_perm(x2.x, x3.x, 0x7632);
+                        a23[1][0] = __byte_perm(x2.y, x3.y, 0x5410), a23[1][1] = __byte_perm(x2.y, x3.y, 0x7632);
+                    } else {
+                        const uint32_t x0 = *reinterpret_cast<const uint32_t*>(codes + r0 * row_bytes(D));
+                        const uint32_t x1 = *reinterpret_cast<const uint32_t*>(codes + r1 * row_bytes(D));
+                        const uint32_t x2 = *reinterpret_cast<const uint32_t*>(codes + (r0 + 8) * row_bytes(D));
+                        const uint32_t x3 = *reinterpret_cast<const uint32_t*>(codes + (r1 + 8) * row_bytes(D));
+                        a01[0][0] = __byte_perm(x0, x1, 0x5410), a01[1][0] = __byte_perm(x0, x1, 0x7632);
+                        a23[0][0] = __byte_perm(x2, x3, 0x5410), a23[1][0] = __byte_perm(x2, x3, 0x7632);
+                        a01[0][1] = a01[1][1] = a23[0][1] = a23[1][1] = 0;
+                    }
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        const int part = k >> 2, nib = k & 3;
+                        const uint32_t b0 = codes_pair(a01[0][part], nib, z01), b1 = codes_pair(a01[1][part], nib, z01);
+                        const uint32_t b2 = codes_pair(a23[0][part], nib, z23), b3 = codes_pair(a23[1][part], nib, z23);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma(o[nt][k], b0, b1, b2, b3, w_hi[nt][2 * m], w_hi[nt][2 * m + 1]);
+                            if (SPLIT_W) mma(o[nt][k], b0, b1, b2, b3, w_lo[nt][2 * m], w_lo[nt][2 * m + 1]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (issued < mine) {
+                    issue(issued);
+                    ++issued;
+                }
+            }
+            done += issued;
+
+            // ---- the four warps' parts of the segment
+            __syncthreads();
+            float* buf = reinterpret_cast<float*>(smem);
+            float2* stats = reinterpret_cast<float2*>(buf + kWarps * C::ROWS * C::PITCH);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int m = 4; m < 32; m *= 2) sum[nt][e] += __shfl_xor_sync(kAll, sum[nt][e], m);
+                    const int row = warp * C::ROWS + 8 * nt + 2 * t + e;
+                    if (gq == 0) stats[row] = make_float2(top[nt][e], sum[nt][e]);
+                    float* to = buf + row * C::PITCH + gq * (D / 8);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k = 0; k < STEPS; k += 4)
+                            *reinterpret_cast<float4*>(to + h * STEPS + k) =
+                                make_float4(o[nt][k][2 * h + e], o[nt][k + 1][2 * h + e], o[nt][k + 2][2 * h + e],
+                                            o[nt][k + 3][2 * h + e]);
+                }
+            }
+            __syncthreads();
+            const bool whole = t0 == 0 && t1 == r.tiles;
+            const int part = (int)(2 * blockIdx.x) + (at != per * blockIdx.x);
+            for (int x = threadIdx.x; x < C::ROWS * (D / 4); x += kThreads) {
+                const int row = x / (D / 4), d = 4 * (x - row * (D / 4));
+                const int of = q_tile * C::ROWS + row;
+                if (of >= r.rows) continue;
+                float m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, stats[w * C::ROWS + row].x);
+                const float ref = m == -INFINITY ? 0.f : m;
+                float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 st = stats[w * C::ROWS + row];
+                    const float f = ptx::ex2(st.x - ref);
+                    l += f * st.y;
+                    const float4 a = *reinterpret_cast<const float4*>(buf + (w * C::ROWS + row) * C::PITCH + d);
+                    v[0] += f * a.x, v[1] += f * a.y, v[2] += f * a.z, v[3] += f * a.w;
+                }
+                if (whole) {
+                    const int token = of / p.group, h = head * p.group + of - token * p.group;
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    if (l == 0.f) v[0] = v[1] = v[2] = v[3] = 0.f;
+                    v[0] *= inv, v[1] *= inv, v[2] *= inv, v[3] *= inv;
+                    store_out(p, p.out_dtype, ((long long)(r.q0 + token) * p.heads + h) * D + d, v);
+                    if (p.lse != nullptr && d == 0)
+                        p.lse[(long long)h * p.rows + r.q0 + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+                } else {
+                    const long long to = (long long)part * C::ROWS + row;
+                    *reinterpret_cast<float4*>(p.part_o + to * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (d == 0) p.part_ml[to] = make_float2(m, l);
+                }
+            }
+            ptx::fence_proxy_async_smem();  // the next copies land where these values were
+            __syncthreads();
         }
-        float top = x;
-        for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float m1 = fmaxf(m, top);
-        const float ref = m1 == -INFINITY ? 0.f : m1;
-        const float f = expf(m - ref);
-        m = m1;
-        const float e = vrow != nullptr ? expf(x - ref) : 0.f;
-        l = l * f + e;
-        for (int i = 0; i < D / 32; ++i) acc[i] *= f;
-        for (int t = 0; t < 32; ++t) {
-            const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)vrow, t));
-            if (v == nullptr) continue;
-            const float w = __shfl_sync(0xffffffffu, e * sv, t);
-            const int z = __shfl_sync(0xffffffffu, zv, t);
-            for (int i = 0; i < D / 32; ++i) {
-                const int el = lane + 32 * i;
-                const uint32_t c = (v[el / 2] >> (4 * (el & 1))) & 15u;
-                acc[i] += w * (float)((int)c - z);
-            }
+        at = p.split ? at + (t1 - t0) : at + r.tiles;
+        if (!in_request) at = here.start + line_of(p, r);
+        if (at >= end) break;
+        if (at >= here.start + line_of(p, r)) {
+            here = locate<C::ROWS, kThreads>(p, g, here.b + 1, here.start + line_of(p, r), at, scratch, &found);
+            r = request_of<C::ROWS>(p, g, here.b);
         }
     }
-    for (int o = 16; o > 0; o /= 2) l += __shfl_xor_sync(0xffffffffu, l, o);
-    O* out = static_cast<O*>(p.out) + ((long long)r * p.heads + head) * D;
-    for (int i = 0; i < D / 32; ++i) store_f(out + lane + 32 * i, l == 0.f ? 0.f : acc[i] / l);
-    if (p.lse != nullptr && lane == 0) p.lse[(long long)head * p.rows + r] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
-template <int D, typename T, typename O>
-void attention_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const long long items = (long long)p.rows * p.heads;
-    kv4_attention_rows<D, T, O><<<(unsigned)((items + 3) / 4), 128, 0, stream>>>(p, g);
+// The parts of the items that several CTAs shared: one CTA per (item, row), a warp per eighth of the
+// parts.  Parts are summed in the order of the line, so a call's result does not depend on timing.
+// Starts while the attention drains (programmatic launch) and finds its item meanwhile.
+constexpr int kMergeWarps = 8;
+
+template <int D, int NT>
+__global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const AttnParams p, const __grid_constant__ Globals g) {
+    constexpr int ROWS = Cfg<D, NT>::ROWS, THREADS = 32 * kMergeWarps, PER = D / 32;
+    __shared__ long long scratch[kMergeWarps];
+    __shared__ Place found;
+    __shared__ int found_item;
+    __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
+    const int id = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) found.b = -1;
+    long long line = 0, items = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
+        const Request r = request_of<ROWS>(p, g, b0 + (int)threadIdx.x);
+        const long long mine = line_of(p, r), count = (long long)r.q_tiles * p.pool.kv_heads;
+        long long before, items_before;
+        const long long all = block_scan<THREADS>(mine, scratch, &before);
+        const long long all_items = block_scan<THREADS>(count, scratch, &items_before);
+        if (items + items_before <= id && id < items + items_before + count) {
+            found = {b0 + (int)threadIdx.x, line + before};
+            found_item = (int)(id - items - items_before);
+        }
+        line += all;
+        items += all_items;
+    }
+    __syncthreads();
+    if (found.b < 0) return;
+    const Request r = request_of<ROWS>(p, g, found.b);
+    const int head = found_item / r.q_tiles, q_tile = found_item - head * r.q_tiles, of = q_tile * ROWS + row;
+    if (of >= r.rows) return;
+    const long long per = max((line + p.ctas - 1) / p.ctas, (long long)kMinTiles);
+    const long long s = found.start + (long long)found_item * r.tiles, e = s + r.tiles;
+    const int c0 = (int)(s / per), c1 = (int)((e - 1) / per);
+    if (c0 == c1) return;  // one CTA had it all and wrote the output
+    ptx::griddep_wait();
+
+    auto part_of = [&](int c) { return ((long long)2 * c + (s > c * per)) * ROWS + row; };
+    float m = -INFINITY, l = 0.f, o[PER] = {};
+    for (int c = c0 + warp; c <= c1; c += kMergeWarps) m = fmaxf(m, p.part_ml[part_of(c)].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
+        const long long at = part_of(c);
+        const float2 ml = p.part_ml[at];
+        const float f = ptx::ex2(ml.x - ref);
+        l += f * ml.y;
+        const float* src = p.part_o + at * D + lane * PER;
+        if (PER == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            o[0] += f * v.x, o[1] += f * v.y, o[PER - 2] += f * v.z, o[PER - 1] += f * v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            o[0] += f * v.x, o[1] += f * v.y;
+        }
+    }
+    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s_o[warp][lane * PER + i] = o[i];
+    __syncthreads();
+    if (threadIdx.x >= D / 4) return;
+    float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, s_m[w]);
+    const float ref_top = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+        const float f = ptx::ex2(s_m[w] - ref_top);
+        sum += f * s_l[w];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += f * s_o[w][4 * threadIdx.x + i];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] * inv;
+    const int token = of / p.group, h = head * p.group + of - token * p.group;
+    store_out(p, p.out_dtype, ((long long)(r.q0 + token) * p.heads + h) * D + 4 * threadIdx.x, v);
+    if (p.lse != nullptr && threadIdx.x == 0)
+        p.lse[(long long)h * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-template <int D, typename T>
-void attention_out(int out_dtype, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    if (out_dtype == LCA_DTYPE_F32)
-        attention_of<D, T, float>(p, g, stream);
-    else if (out_dtype == LCA_DTYPE_F16)
-        attention_of<D, T, __half>(p, g, stream);
-    else
-        attention_of<D, T, __nv_bfloat16>(p, g, stream);
+template <int D, int NT, bool SPLIT_W>
+cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    const int smem = Cfg<D, NT>::SMEM;
+    cudaError_t e = cudaFuncSetAttribute(kv4_attention<D, NT, SPLIT_W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    kv4_attention<D, NT, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !p.split) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.items, 8 * NT);
+    cfg.blockDim = dim3(32 * kMergeWarps);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv4_attention_merge<D, NT>, p, g);
+}
+
+template <int D>
+cudaError_t attention_tiles(int tiles, bool split_w, const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    if (tiles == 1)
+        return split_w ? attention_of<D, 1, true>(p, g, stream) : attention_of<D, 1, false>(p, g, stream);
+    if (tiles == 2)
+        return split_w ? attention_of<D, 2, true>(p, g, stream) : attention_of<D, 2, false>(p, g, stream);
+    return split_w ? attention_of<D, 4, true>(p, g, stream) : attention_of<D, 4, false>(p, g, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_attention(int d, int dtype, int out_dtype, const AttnParams& p, const Globals& g,
-                             cudaStream_t stream) {
-    if (d == 64)
-        dtype == LCA_DTYPE_F16 ? attention_out<64, __half>(out_dtype, p, g, stream)
-                               : attention_out<64, __nv_bfloat16>(out_dtype, p, g, stream);
-    else
-        dtype == LCA_DTYPE_F16 ? attention_out<128, __half>(out_dtype, p, g, stream)
-                               : attention_out<128, __nv_bfloat16>(out_dtype, p, g, stream);
-    return cudaGetLastError();
+// Query tiles: as many groups of 8 rows as an average request has, so that a tile of keys is
+// unpacked once for all of them, up to the 32 rows whose sums fit the registers.
+AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t batch, int64_t capacity,
+                        int64_t window, int64_t num_globals) {
+    AttnPlan a = {};
+    if (rows <= 0 || batch <= 0) return a;
+    const int64_t group = heads / kv_heads;
+    const int64_t mean = (rows + batch - 1) / batch * group;
+    a.q_tiles = mean <= 8 ? 1 : (mean <= 16 ? 2 : 4);
+    const int64_t tile_rows = 8 * a.q_tiles;
+    // at most one partial query tile a request, and one at least a row's heads need
+    const int64_t items = kv_heads * std::min(rows * ((group + tile_rows - 1) / tile_rows), batch + rows * group / tile_rows);
+    const int64_t tokens = (tile_rows - 2) / group + 2;
+    const int64_t band = std::min((std::min(window, capacity) + tokens - 1) / kTile + 2, capacity / kTile + 1);
+    const int64_t longest = band + (num_globals + kTile - 1) / kTile;
+    // Long items are cut wherever a CTA's share of the line ends, and merged by a second kernel;
+    // short ones (a band) stay whole, which saves that launch.
+    a.split = longest > kWholeTiles;
+    const int per_sm = a.q_tiles == 1 ? 4 : (a.q_tiles == 2 ? 3 : 2);
+    a.items = std::min<int64_t>(items, 0x7fffffff);
+    a.ctas = (int)(a.split ? kSms * per_sm : std::min<int64_t>(items, (int64_t)kSms * per_sm * 16));
+    if (a.split) {
+        a.part_o = (size_t)a.ctas * 2 * tile_rows * head_dim * sizeof(float);
+        a.part_ml = (size_t)a.ctas * 2 * tile_rows * sizeof(float2);
+    }
+    return a;
+}
+
+cudaError_t launch_attention(int d, int tiles, const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    const bool split_w = p.out_dtype == LCA_DTYPE_F32;
+    return d == 64 ? attention_tiles<64>(tiles, split_w, p, g, stream) : attention_tiles<128>(tiles, split_w, p, g, stream);
 }
 
 }  // namespace kv4

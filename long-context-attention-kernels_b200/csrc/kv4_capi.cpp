@@ -22,11 +22,24 @@ int after_launch(cudaError_t e, const char* what) {
     return report_error(LCA_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
 }
 
-int check_device() {
-    int sms = 0;
+int check_device(int** err_word = nullptr, unsigned long long* wait_ns = nullptr) {
     int* err = nullptr;
     unsigned long long ns = 0;
-    return lca::device_info(&sms, &err, &ns);
+    const int st = lca::device_info(&err, &ns);
+    if (err_word != nullptr) *err_word = err;
+    if (wait_ns != nullptr) *wait_ns = ns;
+    return st;
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+int check_heads(int64_t rows, int64_t heads, int64_t kv_heads) {
+    if (kv_heads < 1 || heads < 1 || heads % kv_heads != 0 || heads > 65535)
+        return report_error(LCA_ERR_INVALID_ARGUMENT, "heads (%lld) must be a multiple of kv_heads (%lld), at most 65535",
+                            (long long)heads, (long long)kv_heads);
+    if (rows > INT_MAX / heads)
+        return report_error(LCA_ERR_UNSUPPORTED, "%lld rows of %lld heads are too many", (long long)rows, (long long)heads);
+    return LCA_OK;
 }
 
 int check_page_size(int64_t page_size) {
@@ -41,8 +54,8 @@ int check_table(int64_t batch, int64_t width, int64_t page_size) {
     if (batch > lca::kv4::kMaxRequests)
         return report_error(LCA_ERR_UNSUPPORTED, "%lld requests are more than %d", (long long)batch,
                             lca::kv4::kMaxRequests);
-    if (width > INT_MAX / page_size)
-        return report_error(LCA_ERR_UNSUPPORTED, "block_table holds %lld pages of %lld tokens a request (at most 2^31 - 1 tokens)",
+    if (width > ((int64_t)1 << 30) / page_size)
+        return report_error(LCA_ERR_UNSUPPORTED, "block_table holds %lld pages of %lld tokens a request (at most 2^30 tokens)",
                             (long long)width, (long long)page_size);
     return LCA_OK;
 }
@@ -214,6 +227,14 @@ int lca_swa_cached_workspace_size(int64_t num_rows, int64_t heads, int64_t kv_he
                                   int64_t capacity, int64_t window_size, int64_t num_unique_global, size_t* out_bytes) {
     if (out_bytes == nullptr) return report_error(LCA_ERR_INVALID_ARGUMENT, "out_bytes is NULL");
     *out_bytes = 0;
+    if (window_size < 0)
+        return report_error(LCA_ERR_INVALID_ARGUMENT, "window_size must be >= 0 (got %lld)", (long long)window_size);
+    if (num_rows < 0 || batch < 0 || capacity < 0 || num_unique_global < 0)
+        return report_error(LCA_ERR_INVALID_ARGUMENT, "negative shape");
+    if (int st = check_heads(num_rows, heads, kv_heads)) return st;
+    const lca::kv4::AttnPlan a =
+        lca::kv4::plan_attention(num_rows, heads, kv_heads, head_dim, batch, capacity, window_size, num_unique_global);
+    *out_bytes = round256(a.part_o) + a.part_ml;
     return LCA_OK;
 }
 
@@ -228,10 +249,8 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     if (int st = check_out_type(out_dtype)) return st;
     if (int st = check_pool(&p.pool, pool, num_pages, kv_heads, page_size, head_dim)) return st;
     if (int st = check_table(batch, table_width, page_size)) return st;
-    if (heads < 1 || heads % kv_heads != 0 || heads > 65535)
-        return report_error(LCA_ERR_INVALID_ARGUMENT, "heads (%lld) must be a multiple of kv_heads (%lld), at most 65535",
-                            (long long)heads, (long long)kv_heads);
     if (int st = check_rows(num_rows, heads)) return st;
+    if (int st = check_heads(num_rows, heads, kv_heads)) return st;
     if (window_size < 0)
         return report_error(LCA_ERR_INVALID_ARGUMENT, "window_size must be >= 0 (got %lld)", (long long)window_size);
     if (num_global_tokens < 0 || (num_global_tokens > 0 && global_tokens == nullptr))
@@ -260,7 +279,20 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
         return report_error(LCA_ERR_INVALID_ARGUMENT, "q must be 16-byte aligned with strides of a multiple of 8 elements");
     if (!aligned(out, 16)) return report_error(LCA_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned");
     if (!aligned(lse, 4)) return report_error(LCA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
-    if (int st = check_device()) return st;
+    const lca::kv4::AttnPlan a =
+        lca::kv4::plan_attention(num_rows, heads, kv_heads, head_dim, batch, capacity, window_size, n);
+    const size_t need = round256(a.part_o) + a.part_ml;
+    if (need > 0 && (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need))
+        return report_error(LCA_ERR_WORKSPACE, "workspace needs %zu bytes, non-NULL and 256-byte aligned (got %zu)", need,
+                            workspace_bytes);
+    if (int st = check_device(&p.err_word, &p.wait_ns)) return st;
+    p.ctas = a.ctas;
+    p.split = a.split;
+    p.items = a.items;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + round256(a.part_o));
+    p.bf16 = dtype == LCA_DTYPE_BF16;
+    p.out_dtype = out_dtype;
     p.q = q;
     p.q_token = q_row_stride;
     p.q_head = q_head_stride;
@@ -277,8 +309,7 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     p.scale = scale;
     p.out = out;
     p.lse = lse;
-    return after_launch(lca::kv4::launch_attention((int)head_dim, dtype, out_dtype, p, g,
-                                                   static_cast<cudaStream_t>(stream)),
+    return after_launch(lca::kv4::launch_attention((int)head_dim, a.q_tiles, p, g, static_cast<cudaStream_t>(stream)),
                         "cached attention launch");
 }
 

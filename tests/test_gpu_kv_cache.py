@@ -346,7 +346,9 @@ def test_rows_that_see_nothing():
     # a length past the table's capacity is the capacity
     a = lca.sliding_window_attention_cached(q[:1], pool, table[:1], ints([10 ** 9]), ints([0, 1]), 5)
     b = lca.sliding_window_attention_cached(q[:1], pool, table[:1], ints([48]), ints([0, 1]), 5)
-    assert torch.equal(a, b)
+    # tokens 40 to 47 were never written: their random words may be scales of 2^127, whose products
+    # with codes overflow to infinities and then NaN, the same in both calls
+    torch.testing.assert_close(a, b, rtol=0, atol=0, equal_nan=True)
 
 
 def test_strided_queries_streams_and_graphs():
