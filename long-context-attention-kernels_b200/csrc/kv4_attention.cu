@@ -31,6 +31,11 @@ constexpr int kWholeTiles = 48;  // items of up to this many tiles are not split
 constexpr int kSms = 148;
 
 constexpr uint32_t kAll = 0xffffffffu;
+
+// A value that every lane holds alike, in a form from which the compiler can tell (branches on
+// it need no reconvergence, addresses go to uniform registers).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(kAll, v, 0); }
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int lower_bound(const int32_t* a, int n, int v) {
@@ -87,17 +92,21 @@ struct Zero {
     uint32_t low, high;
 };
 
-__device__ __forceinline__ Zero zero_pair(uint32_t word0, uint32_t word1) {
-    const uint32_t z = (word0 & 15u) | ((word1 & 15u) << 16);
-    return {0x64006400u + z, 0xd400d400u + (z << 4)};
+// z: a zero point in bits 0 .. 3 and one in bits 16 .. 19.
+__device__ __forceinline__ Zero zero_pair(uint32_t z) { return {0x64006400u + z, 0xd400d400u + 16u * z}; }
+
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {  // (a & b) | c, one instruction
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
 }
 
 __device__ __forceinline__ uint32_t codes_low(uint32_t w, const Zero& z) {
-    return hsub2((w & 0x000f000fu) | 0x64006400u, z.low);
+    return hsub2(and_or(w, 0x000f000fu, 0x64006400u), z.low);
 }
 
 __device__ __forceinline__ uint32_t codes_high(uint32_t w, const Zero& z) {
-    return hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, z.high);
+    return hfma2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, z.high);
 }
 
 __device__ __forceinline__ uint32_t codes_pair(uint32_t w, int nibble, const Zero& z) {  // nibble: 0 .. 3, a constant
@@ -284,7 +293,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
     __shared__ long long scratch[kWarps];
     __shared__ Place found;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
+    const uint32_t pair_order = (t & 1) ? 0x1054u : 0x5410u;
     uint8_t* ring = smem + warp * kStages * C::STAGE;
     uint64_t* bar = bars + warp * kStages;
     volatile uint32_t* mask = masks + warp * kStages;
@@ -300,7 +310,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
     if (at >= end) return;
     Place here = locate<C::ROWS, kThreads>(p, g, 0, 0, at, scratch, &found);
     Request r = request_of<C::ROWS>(p, g, here.b);
-    uint32_t done = 0;  // tiles this warp has taken from its ring since the start
+    // the next slot of the ring to fill, and the next to empty with its phase
+    int fill = 0, drain = 0, phase = 0;
     bool ok = true;
 
     while (here.b < p.batch) {
@@ -318,47 +329,49 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         const bool in_request = item < r.q_tiles * p.pool.kv_heads;
         if (in_request) {
             const int head = item / r.q_tiles, q_tile = item - head * r.q_tiles;
-            const Span span = span_of<C::ROWS>(p, g, r, q_tile);
+            Span span = span_of<C::ROWS>(p, g, r, q_tile);
+            span.first = uniform(span.first), span.band = uniform(span.band);
+            span.lo = uniform(span.lo), span.hi = uniform(span.hi);
             const int tiles = min(t1, span.band + span.gathered);
-            const int mine = max(0, (tiles - t0 - warp + kWarps - 1) / kWarps);
+            const int mine = uniform(max(0, (tiles - t0 - warp + kWarps - 1) / kWarps)), first_tile = uniform(t0) + warp;
             const int32_t* table = p.table + (long long)here.b * p.width;
 
             // ---- loads: tile t0 + warp + 4 i of the item into the ring
-            int pages = -1, pages_next = -1;  // page ids of 16 tiles of this warp, two blocks each
-            auto fetch_pages = [&](int i0) {
-                const int tile = t0 + warp + kWarps * (i0 + (lane >> 1));
+            // Where 16 tiles of this warp lie, two blocks each, a lane per block: index of the block in
+            // the pool (a pool of 2^31 blocks would be 2 TB), -1 where there is none.  Fetched 8 tiles
+            // ahead, so that neither the table's latency nor the divisions are paid per tile.
+            int where = -1, where_next = -1;
+            auto fetch = [&](int i0) {
+                const int tile = first_tile + kWarps * (i0 + (lane >> 1));
                 const int block = 2 * (span.first + tile) + (lane & 1);
-                return i0 + (lane >> 1) < mine && tile < span.band && block <= span.hi / kBlock
-                           ? table[block / p.pool.page_blocks]
-                           : -1;
+                if (i0 + (lane >> 1) >= mine || tile >= span.band || block > span.hi / kBlock) return -1;
+                const int page_at = block / p.pool.page_blocks, page = table[page_at];
+                if ((unsigned)page >= (unsigned)p.pool.pages) return -1;
+                return (page * p.pool.kv_heads + head) * p.pool.page_blocks + block - page_at * p.pool.page_blocks;
             };
             auto issue = [&](int i) {
                 if ((i & 15) == 0) {
-                    pages = i == 0 ? fetch_pages(0) : pages_next;
+                    where = i == 0 ? fetch(0) : where_next;
                 } else if ((i & 15) == 8) {
-                    pages_next = fetch_pages((i & ~15) + 16);
+                    where_next = fetch((i & ~15) + 16);
                 }
-                const int slot = (done + i) % kStages;
+                const int slot = fill;
+                fill = fill + 1 == kStages ? 0 : fill + 1;
                 uint8_t* dst = ring + slot * C::STAGE;
-                const int tile = t0 + warp + kWarps * i;
+                const int tile = first_tile + kWarps * i;
                 if (tile < span.band) {
-                    const int page0 = __shfl_sync(kAll, pages, 2 * (i & 15)), page1 = __shfl_sync(kAll, pages, 2 * (i & 15) + 1);
+                    const int at0 = __shfl_sync(kAll, where, 2 * (i & 15)), at1 = __shfl_sync(kAll, where, 2 * (i & 15) + 1);
                     if (lane == 0) {
-                        const int block = 2 * (span.first + tile);
-                        const int in0 = block % p.pool.page_blocks, in1 = in0 + 1 == p.pool.page_blocks ? 0 : in0 + 1;
-                        const bool have0 = (unsigned)page0 < (unsigned)p.pool.pages,
-                                   have1 = (unsigned)page1 < (unsigned)p.pool.pages;
-                        const uint8_t* src0 =
-                            p.pool.data + (((long long)page0 * p.pool.kv_heads + head) * p.pool.page_blocks + in0) * block_bytes(D);
-                        const uint8_t* src1 =
-                            p.pool.data + (((long long)page1 * p.pool.kv_heads + head) * p.pool.page_blocks + in1) * block_bytes(D);
-                        mask[slot] = (have0 ? 0xffffu : 0u) | (have1 ? 0xffff0000u : 0u);
-                        ptx::mbar_arrive_expect_tx(&bar[slot], (have0 + have1) * block_bytes(D));
-                        if (have0 && have1 && src1 == src0 + block_bytes(D)) {
-                            bulk_load(dst, src0, 2 * block_bytes(D), &bar[slot]);
+                        const uint8_t* src = p.pool.data + (long long)at0 * block_bytes(D);
+                        mask[slot] = (at0 >= 0 ? 0xffffu : 0u) | (at1 >= 0 ? 0xffff0000u : 0u);
+                        ptx::mbar_arrive_expect_tx(&bar[slot], ((at0 >= 0) + (at1 >= 0)) * block_bytes(D));
+                        if (at0 >= 0 && at1 == at0 + 1) {
+                            bulk_load(dst, src, 2 * block_bytes(D), &bar[slot]);
                         } else {
-                            if (have0) bulk_load(dst, src0, block_bytes(D), &bar[slot]);
-                            if (have1) bulk_load(dst + block_bytes(D), src1, block_bytes(D), &bar[slot]);
+                            if (at0 >= 0) bulk_load(dst, src, block_bytes(D), &bar[slot]);
+                            if (at1 >= 0)
+                                bulk_load(dst + block_bytes(D), p.pool.data + (long long)at1 * block_bytes(D), block_bytes(D),
+                                          &bar[slot]);
                         }
                     }
                 } else {  // a lane per global token
@@ -424,13 +437,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 }
                 // fp16 as it is; bf16 moved by a power of two that takes the row's largest element to
                 // [2^14, 2^15), where fp16 holds 8 bits of every element down to 2^-31 of it
-                float mult = p.scale * kLog2e;
+                float mult = fabsf(p.scale) * kLog2e;
                 uint32_t top = 0;
-                if (p.bf16) {
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
-                    top = max(top, __shfl_xor_sync(kAll, top, 1));
-                    top = max(top, __shfl_xor_sync(kAll, top, 2));
+                for (int i = 0; i < D / 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+                top = max(top, __shfl_xor_sync(kAll, top, 1));
+                top = max(top, __shfl_xor_sync(kAll, top, 2));
+                if (p.bf16) {
                     const int e = max((int)(top >> 7) - 127, -100);  // above 2^-100; smaller rows score 0
                     const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
                     mult *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
@@ -438,13 +451,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     for (int i = 0; i < D / 8; ++i)
                         raw[i] = ptx::pack_f16x2(__uint_as_float(raw[i] << 16) * up,
                                                  __uint_as_float(raw[i] & 0xffff0000u) * up);
-                    if (top >= 0x7f80u) mult = NAN;
-                } else {
+                }
+                // The factor of a score is positive and finite, so that it leaves the -inf of a masked
+                // one alone: the scale's sign goes to the row, a factor of 0 makes it a row of zeros,
+                // and a row that is not finite, or a scale that is not, a row of NaN.
+                const bool finite = top < (p.bf16 ? 0x7f80u : 0x7c00u) && mult < INFINITY;
+                const bool zero = mult < 1.17549435e-38f;
+                if (!finite || zero) mult = 1.f;
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
-                    top = max(top, __shfl_xor_sync(kAll, top, 1));
-                    top = max(top, __shfl_xor_sync(kAll, top, 2));
-                    if (top >= 0x7c00u) mult = NAN;
+                for (int i = 0; i < D / 8; ++i) {
+                    if (p.scale < 0.f) raw[i] ^= 0x80008000u;
+                    if (zero) raw[i] = 0;
+                    if (!finite) raw[i] = 0x7e007e00u;
                 }
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w) {  // elements 8w .. 8w + 7 of this thread's chunk
@@ -478,15 +496,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
 
 #pragma unroll 1
             for (int i = 0; i < issued; ++i) {
-                const int slot = (done + i) % kStages;
-                ok &= ptx::mbar_wait(&bar[slot], ((done + i) / kStages) & 1, nullptr, p.err_word,
-                                     LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
+                const int slot = drain;
+                if (!ptx::mbar_wait(&bar[slot], phase, nullptr, p.err_word, LCA_DEVERR_TIMEOUT_CACHE,
+                                    p.wait_ns))
+                    ok = false;
+                drain = drain + 1 == kStages ? 0 : drain + 1;
+                phase ^= drain == 0;
                 ok = __all_sync(kAll, ok);
                 if (!ok) continue;  // results are invalid; the copies still in flight are waited for
                 const uint8_t* stage = ring + slot * C::STAGE;
-                const int tile = t0 + warp + kWarps * i;
+                const int tile = first_tile + kWarps * i;
                 const int key0 = (span.first + tile) * kTile;
-                const uint32_t have = mask[slot];
+                const uint32_t have = uniform(mask[slot]);
                 const int row0 = slot_row(gq);
 
                 // ---- scores
@@ -504,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     sv[2 * m] = __uint_as_float(*reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0) & ~15u);
                     sv[2 * m + 1] =
                         __uint_as_float(*reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0 + 32) & ~15u);
-                    const Zero z0 = zero_pair(w0, w0), z1 = zero_pair(w1, w1);
+                    const Zero z0 = zero_pair((w0 & 15u) * 0x10001u), z1 = zero_pair((w1 & 15u) * 0x10001u);
                     uint32_t c0[D / 32], c1[D / 32];
                     const uint8_t* at0 = block + row0 * row_bytes(D) + t * (D / 8);
                     const uint8_t* at1 = at0 + 8 * row_bytes(D);
@@ -530,12 +551,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
 
                 // ---- visibility: nothing to do where the whole tile is visible to every row
                 const bool band = tile < span.band;
-                uint32_t seen[NT];  // bit 4 m + c of column pair nt
                 const bool full = have == kAll && (!band || (key0 + kTile - 1 <= span.lo && key0 >= span.hi - p.window));
-                if (full) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) seen[nt] = 0xffu;
-                } else {
+                uint32_t seen[NT];  // bit c = 4 m + 2 (second row) + column
+                if (!full) {
                     uint32_t glob = 0;  // global keys of the tile, which rows outside whose band they lie see
                     if (band && p.num_globals > 0) {
                         const int k = lower_bound(g.at, p.num_globals, key0 + lane);
@@ -545,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     for (int nt = 0; nt < NT; ++nt) {
                         seen[nt] = 0;
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {  // c = 4 m + 2 (second row) + column
+                        for (int c = 0; c < 8; ++c) {
                             const int k = 16 * (c >> 2) + 8 * ((c >> 1) & 1) + row0, e = c & 1;
                             const bool there = (have >> k) & 1;
                             const int j = key0 + k;
@@ -560,34 +578,35 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 float lam[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) lam[c] = fmaxf(lg2(fabsf(sv[c])), -100.f);
-                float peak[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    peak[nt][0] = peak[nt][1] = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        float& x = s[c >> 2][nt][c & 3];
-                        x *= sk[c >> 1] * q_scale[nt][c & 1];
-                        if (!((seen[nt] >> c) & 1)) x = -INFINITY;
-                        peak[nt][c & 1] = fmaxf(peak[nt][c & 1], x + lam[c >> 1]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                        for (int m = 4; m < 32; m *= 2)
-                            peak[nt][e] = fmaxf(peak[nt][e], __shfl_xor_sync(kAll, peak[nt][e], m));
-                    }
-                }
                 bool raise = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) raise |= peak[nt][0] > top[nt][0] + 8.f || peak[nt][1] > top[nt][1] + 8.f;
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) s[c >> 2][nt][c & 3] *= sk[c >> 1];
+                    if (!full) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            if (!((seen[nt] >> c) & 1)) s[c >> 2][nt][c & 3] = -INFINITY;
+                    }
+                }
+                auto peaks = [&](int nt, int e) {  // of this thread's keys
+                    float m = s[0][nt][e] * q_scale[nt][e] + lam[0];
+                    m = fmaxf(m, s[0][nt][2 + e] * q_scale[nt][e] + lam[1]);
+                    m = fmaxf(m, s[1][nt][e] * q_scale[nt][e] + lam[2]);
+                    return fmaxf(m, s[1][nt][2 + e] * q_scale[nt][e] + lam[3]);
+                };
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) raise |= peaks(nt, 0) > top[nt][0] + 8.f || peaks(nt, 1) > top[nt][1] + 8.f;
                 if (__any_sync(kAll, raise)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float f[2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float to = fmaxf(top[nt][e], peak[nt][e]);
+                            float to = peaks(nt, e);
+#pragma unroll
+                            for (int m = 4; m < 32; m *= 2) to = fmaxf(to, __shfl_xor_sync(kAll, to, m));
+                            to = fmaxf(to, top[nt][e]);
                             f[e] = to == -INFINITY ? 1.f : ptx::ex2(top[nt][e] - to);
                             top[nt][e] = to;
                             sum[nt][e] *= f[e];
@@ -604,19 +623,28 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 for (int nt = 0; nt < NT; ++nt) {
                     const float ref0 = top[nt][0] == -INFINITY ? 0.f : top[nt][0];
                     const float ref1 = top[nt][1] == -INFINITY ? 0.f : top[nt][1];
+                    float w[8];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {  // key row c of this thread, both columns
-                        float* x = &s[c >> 1][nt][2 * (c & 1)];
-                        const float p0 = ptx::ex2(x[0] - ref0), p1 = ptx::ex2(x[1] - ref1);
+                        const float* x = &s[c >> 1][nt][2 * (c & 1)];
+                        const float p0 = ptx::ex2(x[0] * q_scale[nt][0] - ref0), p1 = ptx::ex2(x[1] * q_scale[nt][1] - ref1);
                         sum[nt][0] += p0;
                         sum[nt][1] += p1;
-                        const float v0 = (seen[nt] >> (2 * c)) & 1 ? p0 * sv[c] : 0.f;
-                        const float v1 = (seen[nt] >> (2 * c + 1)) & 1 ? p1 * sv[c] : 0.f;
-                        const uint32_t hi = ptx::pack_f16x2(v0, v1);
+                        w[2 * c] = p0 * sv[c];
+                        w[2 * c + 1] = p1 * sv[c];
+                    }
+                    if (!full) {  // 0 also where the scale of a key that is not there is not finite
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            if (!((seen[nt] >> c) & 1)) w[c] = 0.f;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t hi = ptx::pack_f16x2(w[2 * c], w[2 * c + 1]);
                         w_hi[nt][c] = transpose8(hi);
                         if (SPLIT_W) {
                             const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                            w_lo[nt][c] = transpose8(ptx::pack_f16x2(v0 - back.x, v1 - back.y));
+                            w_lo[nt][c] = transpose8(ptx::pack_f16x2(w[2 * c] - back.x, w[2 * c + 1] - back.y));
                         }
                     }
                 }
@@ -626,8 +654,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 for (int m = 0; m < 2; ++m) {
                     const uint8_t* block = stage + m * block_bytes(D);
                     const int r0 = slot_row(2 * t), r1 = slot_row(2 * t + 1);
-                    const uint32_t* words = reinterpret_cast<const uint32_t*>(block + v_words_at(D));
-                    const Zero z01 = zero_pair(words[r0], words[r1]), z23 = zero_pair(words[r0 + 8], words[r1 + 8]);
+                    // r0 and r1 are 2t and 2t + 1, in that order for an even t
+                    const uint2 w01 = *reinterpret_cast<const uint2*>(block + v_words_at(D) + 8 * t);
+                    const uint2 w23 = *reinterpret_cast<const uint2*>(block + v_words_at(D) + 8 * t + 32);
+                    const Zero z01 = zero_pair(__byte_perm(w01.x, w01.y, pair_order) & 0x000f000fu);
+                    const Zero z23 = zero_pair(__byte_perm(w23.x, w23.y, pair_order) & 0x000f000fu);
                     const uint8_t* codes = block + v_codes_at(D) + gq * (D / 16);
                     // [half of the m-tile's rows][low or high 16 bits of a word]
                     uint32_t a01[2][2], a23[2][2];
@@ -667,8 +698,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     ++issued;
                 }
             }
-            done += issued;
-
             // ---- the four warps' parts of the segment
             __syncthreads();
             float* buf = reinterpret_cast<float*>(smem);
@@ -881,7 +910,7 @@ AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t h
 }
 
 cudaError_t launch_attention(int d, int tiles, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const bool split_w = p.out_dtype == LCA_DTYPE_F32;
+    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;
     return d == 64 ? attention_tiles<64>(tiles, split_w, p, g, stream) : attention_tiles<128>(tiles, split_w, p, g, stream);
 }
 
