@@ -30,9 +30,9 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_HOME = os.path.dirname(os.path.dirname(NVCC))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-CABI_SOURCES = ["swa_kernels.cu", "swa_backward.cu", "kv4_cache.cu", "kv4_attention.cu", "capi.cpp", "kv4_capi.cpp",
+CABI_SOURCES = ["swa_kernels.cu", "swa_backward.cu", "kv4_cache.cu", "kv4_attention.cu", "kv4_chunk.cu", "capi.cpp", "kv4_capi.cpp",
                 "noalloc.cu"]
-CABI_HEADERS = ["sm100_ptx.cuh", "swa_kernels.h", "swa_backward.h", "kv4.h", "trace.cuh"]
+CABI_HEADERS = ["sm100_ptx.cuh", "swa_kernels.h", "swa_backward.h", "kv4.h", "kv4_attention.cuh", "trace.cuh"]
 LIB_NAME = "liblca_b200.so"
 TRACE_LIB_NAME = "liblca_b200_trace.so"  # -DLCA_TRACE: in-kernel event trace (trace.cuh)
 EXT_NAME = "long_context_attention_kernels"

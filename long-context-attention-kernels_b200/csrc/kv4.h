@@ -21,6 +21,8 @@ namespace kv4 {
 
 constexpr int kBlock = 16;             // tokens per block
 constexpr int kMaxGlobals = 1024;      // global tokens of one attention call (kernel parameter space)
+constexpr int kChunkRows = 256;        // query rows and keys of a tile of the tcgen05 kernel
+constexpr int kChunkKeys = 64;
 constexpr int kMaxRequests = 8192;     // requests of one layout call (shared memory of its scan)
 
 __host__ __device__ constexpr int row_bytes(int d) { return d / 2; }              // code bytes of one row
@@ -79,6 +81,7 @@ struct AttnParams {
     void* out;   // [rows][heads][d]
     float* lse;  // [heads][rows] or NULL
     int ctas, split;  // CTAs that share the line of tiles; whether items may be cut between them
+    int min_tiles;    // and then the least tiles of a CTA
     long long items;  // at most this many items
     float* part_o;    // [ctas][2][tile rows][d]: the parts of cut items, and
     float2* part_ml;  // [ctas][2][tile rows]: their maxima and sums
@@ -87,8 +90,8 @@ struct AttnParams {
 };
 
 struct AttnPlan {
-    int q_tiles;  // groups of 8 query rows a tile
-    int ctas;
+    int tile_rows;  // query rows of an item: 8, 16 or 32 (kv4_attention.cu) or kChunkRows (kv4_chunk.cu)
+    int ctas, min_tiles;
     bool split;
     int64_t items;
     size_t part_o, part_ml;  // bytes
@@ -100,7 +103,8 @@ cudaError_t launch_append(int d, int dtype, bool vector, const RowsParams& p, cu
 cudaError_t launch_read(int d, int out_dtype, const RowsParams& p, cudaStream_t stream);
 AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t batch, int64_t capacity,
                         int64_t window, int64_t num_globals);
-cudaError_t launch_attention(int d, int q_tiles, const AttnParams& p, const Globals& g, cudaStream_t stream);
+cudaError_t launch_chunk(int d, const AttnParams& p, const Globals& g, cudaStream_t stream);
+cudaError_t launch_attention(int d, int tile_rows, const AttnParams& p, const Globals& g, cudaStream_t stream);
 
 }  // namespace kv4
 

@@ -10,13 +10,9 @@
 // The integers c - z are exact in fp16, so both products run on the tensor cores over them
 // (mma.sync m16n8k16, keys by queries and elements by queries, fp32 sums) and the scales stay in
 // fp32, outside the products: sk multiplies a finished score, sv the weight of its key.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
-#include "kv4.h"
-#include "sm100_ptx.cuh"
+#include "kv4_attention.cuh"
 
 namespace lca {
 namespace kv4 {
@@ -28,24 +24,8 @@ constexpr int kTile = 32;    // keys per tile: two blocks, one warp's step
 constexpr int kStages = 3;   // tiles in flight per warp
 constexpr int kMinTiles = 8; // least tiles of a CTA where items are split
 constexpr int kWholeTiles = 48;  // items of up to this many tiles are not split
+constexpr int kChunkFrom = 64;   // mean rows a request from which the tcgen05 kernel takes the call
 constexpr int kSms = 148;
-
-constexpr uint32_t kAll = 0xffffffffu;
-
-// A value that every lane holds alike, in a form from which the compiler can tell (branches on
-// it need no reconvergence, addresses go to uniform registers).
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(kAll, v, 0); }
-
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ int lower_bound(const int32_t* a, int n, int v) {
-    int lo = 0;
-    while (lo < n) {
-        const int mid = (lo + n) >> 1;
-        if (a[mid] < v) lo = mid + 1; else n = mid;
-    }
-    return lo;
-}
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -65,196 +45,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
-}
-
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t d;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-// Two codes minus their zero points as a pair of fp16, from the nibbles at bits 0 and 16 (LOW) or 4
-// and 20 of w.  0x6400 | c is 1024 + c; 0x6400 | 16 c is 1024 + 16 c, a sixteenth of which is 64 + c.
-// z holds the fp16 pairs 1024 + zp and -(64 + zp); every step is exact.
-struct Zero {
-    uint32_t low, high;
-};
-
-// z: a zero point in bits 0 .. 3 and one in bits 16 .. 19.
-__device__ __forceinline__ Zero zero_pair(uint32_t z) { return {0x64006400u + z, 0xd400d400u + 16u * z}; }
-
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {  // (a & b) | c, one instruction
-    uint32_t d;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint32_t codes_low(uint32_t w, const Zero& z) {
-    return hsub2(and_or(w, 0x000f000fu, 0x64006400u), z.low);
-}
-
-__device__ __forceinline__ uint32_t codes_high(uint32_t w, const Zero& z) {
-    return hfma2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, z.high);
-}
-
-__device__ __forceinline__ uint32_t codes_pair(uint32_t w, int nibble, const Zero& z) {  // nibble: 0 .. 3, a constant
-    const uint32_t v = nibble >= 2 ? w >> 8 : w;
-    return (nibble & 1) ? codes_high(v, z) : codes_low(v, z);
-}
-
-// ------------------------------------------------------------------ the work of a call
-
-// An item is one (request, KV head, tile of 8 * NT query rows); rows of a request are ordered
-// token by token, and within a token by the query heads of the group.  Its keys are whole
-// tiles of 32 positions that cover the band of its rows, then tiles of 32 gathered
-// global tokens in front of the band.  Request b has `items` items of at most `tiles` tiles
-// each (exactly `tiles` when it has one query tile per head); all its tiles, item after item and
-// request after request, form one line of tiles that the CTAs share out evenly.
-struct Request {
-    int q0, len, rows;      // first row of q, cached tokens, rows (tokens * group)
-    int q_tiles, tiles;
-};
-
-struct Span {
-    int first, band, globals, gathered;  // first band tile, band tiles, gathered keys and their tiles
-    int lo, hi;                          // positions of the first and the last row
-};
-
-template <int ROWS>
-__device__ __forceinline__ Span span_of(const AttnParams& p, const Globals& g, const Request& r, int q_tile) {
-    Span s;
-    const int n = r.rows / p.group;
-    const int from = q_tile * ROWS, to = min(from + ROWS, r.rows) - 1;
-    s.lo = r.len - n + from / p.group;
-    s.hi = r.len - n + to / p.group;
-    if (s.hi < 0) return {0, 0, 0, 0, s.lo, s.hi};
-    int lo = max(0, s.lo - p.window);
-    s.globals = 0;
-    if (p.num_globals > 0) {
-        if (lo > 0) {
-            const int at = lower_bound(g.at, p.num_globals, s.lo);
-            if (at < p.num_globals && g.at[at] <= s.hi) lo = 0;  // a global row sees every key up to itself
-        }
-        lo &= ~(kTile - 1);
-        s.globals = lower_bound(g.at, p.num_globals, lo);
-    }
-    s.first = lo / kTile;
-    s.band = s.hi / kTile - s.first + 1;
-    s.gathered = (s.globals + kTile - 1) / kTile;
-    return s;
-}
-
-template <int ROWS>
-__device__ __forceinline__ Request request_of(const AttnParams& p, const Globals& g, int b) {
-    Request r = {0, 0, 0, 0, 0};
-    if (b >= p.batch) return r;
-    const int q0 = min(max(p.cu[b], 0), p.rows), q1 = min(max(p.cu[b + 1], 0), p.rows);
-    if (q1 <= q0) return r;
-    const int cap = p.width * p.pool.page_blocks * kBlock;
-    r.q0 = q0;
-    r.len = min(max(p.kv_lens[b], 0), cap);
-    r.rows = (q1 - q0) * p.group;
-    r.q_tiles = (r.rows + ROWS - 1) / ROWS;
-    Span s = span_of<ROWS>(p, g, r, r.q_tiles - 1);
-    r.tiles = s.band + s.gathered;
-    if (r.q_tiles > 1) {
-        // any tile: its rows lie within so many tokens, so its band within so many tiles; whole
-        // when one of the new tokens is global
-        const int tokens = (ROWS - 2) / p.group + 2;
-        int band = (int)min((long long)(p.window + tokens - 1) / kTile + 2, (long long)r.len / kTile + 1);
-        const int first = r.len - (q1 - q0);
-        const int at = lower_bound(g.at, p.num_globals, first);
-        if (at < p.num_globals && g.at[at] < r.len) band = r.len / kTile + 1;
-        r.tiles = band + (lower_bound(g.at, p.num_globals, max(0, r.len - p.window)) + kTile - 1) / kTile;
-    }
-    r.tiles = max(r.tiles, 1);
-    return r;
-}
-
-__device__ __forceinline__ long long line_of(const AttnParams& p, const Request& r) {
-    return (long long)r.q_tiles * p.pool.kv_heads * r.tiles;
-}
-
-// Block-wide: the sum of a value over the threads, and each thread's exclusive prefix.
-template <int THREADS>
-__device__ __forceinline__ long long block_scan(long long v, long long* scratch, long long* before) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const long long u = __shfl_up_sync(kAll, inc, o);
-        if (lane >= o) inc += u;
-    }
-    if (lane == 31) scratch[warp] = inc;
-    __syncthreads();
-    long long all = 0, mine = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w == warp) mine = all;
-        all += scratch[w];
-    }
-    __syncthreads();
-    *before = mine + inc - v;
-    return all;
-}
-
-struct Place {
-    int b;             // request
-    long long start;   // its first tile on the line
-};
-
-// The request that holds position `at` of the line, searched from `from` on, whose own part of the
-// line begins at `start`.  `at` lies on the line.
-template <int ROWS, int THREADS>
-__device__ __forceinline__ Place locate(const AttnParams& p, const Globals& g, int from, long long start, long long at,
-                                        long long* scratch, Place* found) {
-    for (int b0 = from; b0 < p.batch; b0 += THREADS) {
-        const long long mine = line_of(p, request_of<ROWS>(p, g, b0 + (int)threadIdx.x));
-        long long before;
-        const long long all = block_scan<THREADS>(mine, scratch, &before);
-        if (at < start + all) {
-            if (start + before <= at && at < start + before + mine) *found = {b0 + (int)threadIdx.x, start + before};
-            __syncthreads();
-            const Place r = *found;
-            __syncthreads();
-            return r;
-        }
-        start += all;
-    }
-    return {p.batch, start};
-}
-
-template <int ROWS, int THREADS>
-__device__ __forceinline__ long long whole_line(const AttnParams& p, const Globals& g, long long* scratch) {
-    long long sum = 0, before;
-    for (int b = threadIdx.x; b < p.batch; b += THREADS) sum += line_of(p, request_of<ROWS>(p, g, b));
-    return block_scan<THREADS>(sum, scratch, &before);
-}
-
-__device__ __forceinline__ void store_out(const AttnParams& p, int out_dtype, long long at, const float (&v)[4]) {
-    if (out_dtype == LCA_DTYPE_F32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-    } else if (out_dtype == LCA_DTYPE_F16) {
-        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-        *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    } else {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    }
 }
 
 template <int D, int NT>
@@ -302,21 +92,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
     if (threadIdx.x == 0) ptx::fence_mbar_init();
     ptx::griddep_launch();
 
-    const long long line = whole_line<C::ROWS, kThreads>(p, g, scratch);
-    long long per = (line + gridDim.x - 1) / gridDim.x;
-    if (p.split) per = max(per, (long long)kMinTiles);
+    const long long line = whole_line<C::ROWS, kTile, kThreads>(p, g, scratch);
+    long long per = divide(line + gridDim.x - 1, gridDim.x);
+    if (p.split) per = max(per, (long long)p.min_tiles);
     long long at = per * blockIdx.x;
     const long long end = min(at + per, line);
     if (at >= end) return;
-    Place here = locate<C::ROWS, kThreads>(p, g, 0, 0, at, scratch, &found);
-    Request r = request_of<C::ROWS>(p, g, here.b);
+    Place here = locate<C::ROWS, kTile, kThreads>(p, g, 0, 0, at, scratch, &found);
+    Request r = request_of<C::ROWS, kTile>(p, g, here.b);
     // the next slot of the ring to fill, and the next to empty with its phase
     int fill = 0, drain = 0, phase = 0;
     bool ok = true;
 
     while (here.b < p.batch) {
         const long long in = at - here.start;
-        int item = (int)(in / r.tiles);
+        int item = (int)divide(in, r.tiles);
         int t0 = (int)(in - (long long)item * r.tiles), t1 = r.tiles;
         if (p.split) {
             t1 = (int)min((long long)r.tiles, t0 + (end - at));
@@ -329,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         const bool in_request = item < r.q_tiles * p.pool.kv_heads;
         if (in_request) {
             const int head = item / r.q_tiles, q_tile = item - head * r.q_tiles;
-            Span span = span_of<C::ROWS>(p, g, r, q_tile);
+            Span span = span_of<C::ROWS, kTile>(p, g, r, q_tile);
             span.first = uniform(span.first), span.band = uniform(span.band);
             span.lo = uniform(span.lo), span.hi = uniform(span.hi);
             const int tiles = min(t1, span.band + span.gathered);
@@ -761,8 +551,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         if (!in_request) at = here.start + line_of(p, r);
         if (at >= end) break;
         if (at >= here.start + line_of(p, r)) {
-            here = locate<C::ROWS, kThreads>(p, g, here.b + 1, here.start + line_of(p, r), at, scratch, &found);
-            r = request_of<C::ROWS>(p, g, here.b);
+            here = locate<C::ROWS, kTile, kThreads>(p, g, here.b + 1, here.start + line_of(p, r), at, scratch, &found);
+            r = request_of<C::ROWS, kTile>(p, g, here.b);
         }
     }
 }
@@ -772,9 +562,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
 // Starts while the attention drains (programmatic launch) and finds its item meanwhile.
 constexpr int kMergeWarps = 8;
 
-template <int D, int NT>
+template <int D, int ROWS, int TILE>
 __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const AttnParams p, const __grid_constant__ Globals g) {
-    constexpr int ROWS = Cfg<D, NT>::ROWS, THREADS = 32 * kMergeWarps, PER = D / 32;
+    constexpr int THREADS = 32 * kMergeWarps, PER = D / 32;
     __shared__ long long scratch[kMergeWarps];
     __shared__ Place found;
     __shared__ int found_item;
@@ -783,7 +573,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     if (threadIdx.x == 0) found.b = -1;
     long long line = 0, items = 0;
     for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
-        const Request r = request_of<ROWS>(p, g, b0 + (int)threadIdx.x);
+        const Request r = request_of<ROWS, TILE>(p, g, b0 + (int)threadIdx.x);
         const long long mine = line_of(p, r), count = (long long)r.q_tiles * p.pool.kv_heads;
         long long before, items_before;
         const long long all = block_scan<THREADS>(mine, scratch, &before);
@@ -797,10 +587,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     }
     __syncthreads();
     if (found.b < 0) return;
-    const Request r = request_of<ROWS>(p, g, found.b);
+    const Request r = request_of<ROWS, TILE>(p, g, found.b);
     const int head = found_item / r.q_tiles, q_tile = found_item - head * r.q_tiles, of = q_tile * ROWS + row;
     if (of >= r.rows) return;
-    const long long per = max((line + p.ctas - 1) / p.ctas, (long long)kMinTiles);
+    const long long per = max(divide(line + p.ctas - 1, p.ctas), (long long)p.min_tiles);
     const long long s = found.start + (long long)found_item * r.tiles, e = s + r.tiles;
     const int c0 = (int)(s / per), c1 = (int)((e - 1) / per);
     if (c0 == c1) return;  // one CTA had it all and wrote the output
@@ -850,16 +640,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
         p.lse[(long long)h * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
-template <int D, int NT, bool SPLIT_W>
-cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const int smem = Cfg<D, NT>::SMEM;
-    cudaError_t e = cudaFuncSetAttribute(kv4_attention<D, NT, SPLIT_W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    kv4_attention<D, NT, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
-    e = cudaGetLastError();
-    if (e != cudaSuccess || !p.split) return e;
+template <int D, int ROWS, int TILE>
+cudaError_t merge_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.items, 8 * NT);
+    cfg.gridDim = dim3((unsigned)p.items, ROWS);
     cfg.blockDim = dim3(32 * kMergeWarps);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -867,51 +651,67 @@ cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t str
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_attention_merge<D, NT>, p, g);
+    return cudaLaunchKernelEx(&cfg, kv4_attention_merge<D, ROWS, TILE>, p, g);
+}
+
+template <int D, int NT, bool SPLIT_W>
+cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    const int smem = Cfg<D, NT>::SMEM;
+    cudaError_t e = cudaFuncSetAttribute(kv4_attention<D, NT, SPLIT_W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    kv4_attention<D, NT, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
+    e = cudaGetLastError();
+    return e != cudaSuccess || !p.split ? e : merge_of<D, 8 * NT, kTile>(p, g, stream);
 }
 
 template <int D>
-cudaError_t attention_tiles(int tiles, bool split_w, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    if (tiles == 1)
+cudaError_t attention_rows(int tile_rows, const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;  // bf16 is rounded more coarsely than the weights
+    if (tile_rows == 8)
         return split_w ? attention_of<D, 1, true>(p, g, stream) : attention_of<D, 1, false>(p, g, stream);
-    if (tiles == 2)
+    if (tile_rows == 16)
         return split_w ? attention_of<D, 2, true>(p, g, stream) : attention_of<D, 2, false>(p, g, stream);
-    return split_w ? attention_of<D, 4, true>(p, g, stream) : attention_of<D, 4, false>(p, g, stream);
+    if (tile_rows == 32)
+        return split_w ? attention_of<D, 4, true>(p, g, stream) : attention_of<D, 4, false>(p, g, stream);
+    const cudaError_t e = launch_chunk(D, p, g, stream);
+    return e != cudaSuccess || !p.split ? e : merge_of<D, kChunkRows, kChunkKeys>(p, g, stream);
 }
 
 }  // namespace
 
-// Query tiles: as many groups of 8 rows as an average request has, so that a tile of keys is
-// unpacked once for all of them, up to the 32 rows whose sums fit the registers.
+// Rows of an item: as many groups of 8 as an average request has, so that a tile of keys is
+// unpacked once for all of them, up to the 32 whose sums fit the registers of one warp; from
+// kChunkFrom rows on, 256 rows on tcgen05.
 AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t batch, int64_t capacity,
                         int64_t window, int64_t num_globals) {
     AttnPlan a = {};
     if (rows <= 0 || batch <= 0) return a;
     const int64_t group = heads / kv_heads;
     const int64_t mean = (rows + batch - 1) / batch * group;
-    a.q_tiles = mean <= 8 ? 1 : (mean <= 16 ? 2 : 4);
-    const int64_t tile_rows = 8 * a.q_tiles;
-    // at most one partial query tile a request, and one at least a row's heads need
-    const int64_t items = kv_heads * std::min(rows * ((group + tile_rows - 1) / tile_rows), batch + rows * group / tile_rows);
-    const int64_t tokens = (tile_rows - 2) / group + 2;
-    const int64_t band = std::min((std::min(window, capacity) + tokens - 1) / kTile + 2, capacity / kTile + 1);
-    const int64_t longest = band + (num_globals + kTile - 1) / kTile;
+    const bool chunk = mean >= kChunkFrom;
+    a.tile_rows = chunk ? kChunkRows : (mean <= 8 ? 8 : (mean <= 16 ? 16 : 32));
+    const int64_t tile = chunk ? kChunkKeys : kTile;
+    // at most one partial item a request and head, and a row's heads need so many at least
+    const int64_t items = kv_heads * std::min(rows * ((group + a.tile_rows - 1) / a.tile_rows), batch + rows * group / a.tile_rows);
+    const int64_t tokens = (a.tile_rows - 2) / group + 2;
+    const int64_t band = std::min((std::min(window, capacity) + tokens - 1) / tile + 2, capacity / tile + 1);
+    const int64_t longest = band + (num_globals + tile - 1) / tile;
     // Long items are cut wherever a CTA's share of the line ends, and merged by a second kernel;
     // short ones (a band) stay whole, which saves that launch.
     a.split = longest > kWholeTiles;
-    const int per_sm = a.q_tiles == 1 ? 4 : (a.q_tiles == 2 ? 3 : 2);
+    a.min_tiles = chunk ? 4 : kMinTiles;
+    const int per_sm = chunk ? 1 : (a.tile_rows == 8 ? 4 : (a.tile_rows == 16 ? 3 : 2));
     a.items = std::min<int64_t>(items, 0x7fffffff);
-    a.ctas = (int)(a.split ? kSms * per_sm : std::min<int64_t>(items, (int64_t)kSms * per_sm * 16));
+    a.ctas = (int)(a.split || chunk ? kSms * per_sm : std::min<int64_t>(items, (int64_t)kSms * per_sm * 16));
     if (a.split) {
-        a.part_o = (size_t)a.ctas * 2 * tile_rows * head_dim * sizeof(float);
-        a.part_ml = (size_t)a.ctas * 2 * tile_rows * sizeof(float2);
+        a.part_o = (size_t)a.ctas * 2 * a.tile_rows * head_dim * sizeof(float);
+        a.part_ml = (size_t)a.ctas * 2 * a.tile_rows * sizeof(float2);
     }
     return a;
 }
 
-cudaError_t launch_attention(int d, int tiles, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;
-    return d == 64 ? attention_tiles<64>(tiles, split_w, p, g, stream) : attention_tiles<128>(tiles, split_w, p, g, stream);
+cudaError_t launch_attention(int d, int tile_rows, const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    return d == 64 ? attention_rows<64>(tile_rows, p, g, stream) : attention_rows<128>(tile_rows, p, g, stream);
 }
 
 }  // namespace kv4

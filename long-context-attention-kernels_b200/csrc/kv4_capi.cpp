@@ -287,6 +287,7 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
                             workspace_bytes);
     if (int st = check_device(&p.err_word, &p.wait_ns)) return st;
     p.ctas = a.ctas;
+    p.min_tiles = a.min_tiles;
     p.split = a.split;
     p.items = a.items;
     p.part_o = static_cast<float*>(workspace);
@@ -309,7 +310,7 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     p.scale = scale;
     p.out = out;
     p.lse = lse;
-    return after_launch(lca::kv4::launch_attention((int)head_dim, a.q_tiles, p, g, static_cast<cudaStream_t>(stream)),
+    return after_launch(lca::kv4::launch_attention((int)head_dim, a.tile_rows, p, g, static_cast<cudaStream_t>(stream)),
                         "cached attention launch");
 }
 

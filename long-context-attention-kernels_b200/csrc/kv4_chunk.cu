@@ -1,0 +1,603 @@
+// kv4_chunk.cu -- attention of many new tokens a request (a prompt's chunk) over the paged 4-bit KV
+// cache, on tcgen05.  Mathematics as in kv4_attention.cu: products over the exact integers c - z,
+// scales outside them in fp32.
+//
+// A CTA takes 256 query rows (tokens x the heads of a group) of one KV head at a time, as two
+// tiles A and B of 128 rows, over tiles of 64 keys:
+//   unpack warps (4)   a block of 16 keys each: codes from global memory two tiles ahead, as fp16
+//                      c - z into a ring of swizzled K and V tiles; scales into a small table
+//   MMA warp (1 lane)  S = Q K^T into one of two buffers in TMEM, then O += W V of the tile before, W
+//                      read from TMEM where it lies over its S
+//   softmax warps (8)  a thread per row: scores times scales, the running maximum, weights to fp16
+// Barriers with one phase per tile of one parity (n & 1), so that a wait for tile n - 1 cannot be
+// answered by a phase before or after it.
+// A tile of codes is unpacked once for 256 rows, and the products of one tile run under
+// the softmax of the other.  K, V and Q are held with the elements of each group of 8 in the order
+// 0 4 1 5 2 6 3 7, in which the codes come out of a word; Q is stored so too, and the output put
+// back in order as it is read.
+#include <algorithm>
+
+#include "kv4_attention.cuh"
+
+namespace lca {
+namespace kv4 {
+namespace {
+
+constexpr int kHalfRows = 128;            // rows of a tile A or B
+constexpr int kKeys = kChunkKeys;         // keys of a tile
+constexpr int kRing = 3;                  // unpacked tiles
+constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4, kMmaWarp = kSoftmaxWarps + kUnpackWarps;
+constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, products
+// registers a thread of each: 2 * 176 + 96 + 64 = 4 * 128, what the block is launched with
+constexpr int kSoftmaxRegs = 176, kUnpackRegs = 96, kMmaRegs = 64;
+constexpr uint32_t kTmemCols = 512;
+
+template <int D>
+struct Cfg {
+    static constexpr int Q_PANEL = kHalfRows * 128, KV_PANEL = kKeys * 128;  // 64 elements of every row
+    static constexpr int Q_BYTES = D / 64 * Q_PANEL, KV_BYTES = D / 64 * KV_PANEL;
+    static constexpr int OFF_KV = 2 * Q_BYTES;
+    static constexpr int OFF_TABLE = OFF_KV + kRing * 2 * KV_BYTES;  // [kRing][3][kKeys] sk, log2 sv, sv
+    static constexpr int OFF_HAVE = OFF_TABLE + kRing * 3 * kKeys * 4;  // [kRing][4] keys that are there
+    static constexpr int OFF_BAR = OFF_HAVE + kRing * 16;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;  // and the alignment of the panels
+};
+
+// The items of this CTA, in order; every warp walks them for itself.
+struct Walk {
+    Place here;
+    Request r;
+    long long at, end;
+    int head, q_tile, t0, t1;
+};
+
+template <int ROWS, int TILE>
+__device__ __forceinline__ Place locate_warp(const AttnParams& p, const Globals& g, int from, long long start, long long at) {
+    const int lane = threadIdx.x & 31;
+    for (int b0 = from; b0 < p.batch; b0 += 32) {
+        const long long mine = line_of(p, request_of<ROWS, TILE>(p, g, b0 + lane));
+        long long inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const long long u = __shfl_up_sync(kAll, inc, o);
+            if (lane >= o) inc += u;
+        }
+        const uint32_t hit = __ballot_sync(kAll, at < start + inc);
+        if (hit) {
+            const int who = __ffs(hit) - 1;
+            return {b0 + who, __shfl_sync(kAll, start + inc - mine, who)};
+        }
+        start += __shfl_sync(kAll, inc, 31);
+    }
+    return {p.batch, start};
+}
+
+// The next item (or part of one) of the walk, or false.
+__device__ __forceinline__ bool next_item(const AttnParams& p, const Globals& g, Walk& w) {
+    while (w.at < w.end && w.here.b < p.batch) {
+        const long long stop = w.here.start + line_of(p, w.r);
+        if (w.at >= stop) {
+            w.here = locate_warp<kChunkRows, kKeys>(p, g, w.here.b + 1, stop, w.at);
+            w.r = request_of<kChunkRows, kKeys>(p, g, w.here.b);
+            continue;
+        }
+        const long long in = w.at - w.here.start;
+        const int item = (int)divide(in, w.r.tiles);
+        w.t0 = (int)(in - (long long)item * w.r.tiles);
+        if (!p.split && w.t0 > 0) {  // whole items only: this one belongs to the CTA before
+            w.at = w.here.start + (long long)(item + 1) * w.r.tiles;
+            continue;
+        }
+        w.t1 = p.split ? (int)min((long long)w.r.tiles, w.t0 + (w.end - w.at)) : w.r.tiles;
+        w.head = item / w.r.q_tiles;
+        w.q_tile = item - w.head * w.r.q_tiles;
+        return true;
+    }
+    return false;
+}
+
+// One row of 64 keys' bits below key index n.
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1); }
+
+template <int D, bool SPLIT_W>
+__global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, const __grid_constant__ Globals g) {
+    using C = Cfg<D>;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+    float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
+    volatile uint32_t* have_at = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_HAVE);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+    uint64_t *q_full = bars, *kv_full = bars + 2, *kv_free = kv_full + kRing, *s_full = kv_free + kRing, *p_full = s_full + 4,
+             *pv_done = p_full + 4, *drain = pv_done + 4;
+    __shared__ long long scratch[kThreads / 32];
+    __shared__ Place found;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) ptx::mbar_init(&q_full[i], 4);
+        for (int i = 0; i < kRing; ++i) {
+            ptx::mbar_init(&kv_full[i], kUnpackWarps);
+            ptx::mbar_init(&kv_free[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            ptx::mbar_init(&s_full[i], 1);
+            ptx::mbar_init(&p_full[i], 4);
+            ptx::mbar_init(&pv_done[i], 1);
+        }
+        ptx::mbar_init(drain, 1);
+        s_abort = 0;
+        ptx::fence_mbar_init();
+    }
+    ptx::griddep_launch();
+    Walk walk;
+    {
+        const long long line = whole_line<kChunkRows, kKeys, kThreads>(p, g, scratch);
+        long long per = divide(line + gridDim.x - 1, gridDim.x);
+        if (p.split) per = max(per, (long long)p.min_tiles);
+        walk.at = per * blockIdx.x;
+        walk.end = min(walk.at + per, line);
+        if (walk.at >= walk.end) return;
+        walk.here = locate<kChunkRows, kKeys, kThreads>(p, g, 0, 0, walk.at, scratch, &found);
+        walk.r = request_of<kChunkRows, kKeys>(p, g, walk.here.b);
+    }
+    const long long line_at = walk.at;
+    if (warp == kMmaWarp) {
+        ptx::tmem_alloc(&s_tmem, kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int parity) {
+        if (ok) ok = ptx::mbar_wait(bar, (uint32_t)parity & 1u, &s_abort, p.err_word, LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
+    };
+    auto wait_all = [&](uint64_t* bar, int parity) {  // for a whole warp: every lane learns the same
+        wait(bar, parity);
+        ok = __all_sync(kAll, ok);
+    };
+    auto tiles_of = [&](Span& s) {  // whole or partial item: its tiles [t0, t0 + n)
+        s = span_of<kChunkRows, kKeys>(p, g, walk.r, walk.q_tile);
+        return max(0, min(walk.t1, s.band + s.gathered) - walk.t0);
+    };
+    int n = 0;  // tiles since the start, the same count in every role
+
+    if (warp >= kMmaWarp) {
+        ptx::setmaxnreg_dec<kMmaRegs>();
+    } else if (warp >= kSoftmaxWarps) {
+        ptx::setmaxnreg_dec<kUnpackRegs>();
+    } else {
+        ptx::setmaxnreg_inc<kSoftmaxRegs>();
+    }
+    if (warp > kMmaWarp) {
+        // the rest of the products' warpgroup has nothing to do
+    } else if (warp == kMmaWarp) {
+        // ============================================================ products
+        const uint32_t hi = ptx::smem_desc_sw128_hi(1024);
+        const uint32_t idesc_s = ptx::idesc_f16(false, kHalfRows, kKeys, false);
+        const uint32_t idesc_o = ptx::idesc_f16(false, kHalfRows, D, true);
+        int items = 0;
+        auto accumulate = [&](int m, bool first) {  // O += W V of tile m
+            const uint32_t v = ptx::smem_u32(smem + C::OFF_KV + (m % kRing) * 2 * C::KV_BYTES + C::KV_BYTES);
+            const uint32_t v_lo = ptx::smem_desc_sw128_lo(v, C::KV_PANEL);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                wait(&p_full[2 * h + (m & 1)], m >> 1);
+                if (!ok) return;
+                ptx::tc_fence_after();
+                const uint32_t o = tmem + 256 * h, w = tmem + 256 * h + 128 + 64 * (m & 1);
+#pragma unroll
+                for (int part = 0; part < (SPLIT_W ? 2 : 1); ++part)
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        ptx::mma_f16_ts(o, w + 32 * part + 8 * k, ptx::desc_join(v_lo + ((16 * k * 128) >> 4), hi), idesc_o,
+                                        !first || part > 0 || k > 0);
+                ptx::mma_commit(&pv_done[2 * h + (m & 1)]);
+            }
+            ptx::mma_commit(&kv_free[m % kRing]);
+        };
+        while (ok && next_item(p, g, walk)) {
+            Span span;
+            const int tiles = tiles_of(span);
+            walk.at += walk.t1 - walk.t0;
+            if (tiles == 0) continue;
+            if (lane == 0) {
+                wait(&q_full[0], items);
+                wait(&q_full[1], items);
+                for (int i = 0; i < tiles && ok; ++i, ++n) {
+                    wait(&kv_full[n % kRing], n / kRing);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    const uint32_t k_lo =
+                        ptx::smem_desc_sw128_lo(ptx::smem_u32(smem + C::OFF_KV + (n % kRing) * 2 * C::KV_BYTES), 0);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t q_lo = ptx::smem_desc_sw128_lo(ptx::smem_u32(smem + h * C::Q_BYTES), 0);
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+                            ptx::mma_f16_ss(tmem + 256 * h + 128 + 64 * (n & 1),
+                                            ptx::desc_join(q_lo + (((k >> 2) * C::Q_PANEL + (k & 3) * 32) >> 4), hi),
+                                            ptx::desc_join(k_lo + (((k >> 2) * C::KV_PANEL + (k & 3) * 32) >> 4), hi), idesc_s,
+                                            k > 0);
+                        ptx::mma_commit(&s_full[2 * h + (n & 1)]);
+                    }
+                    if (i > 0) accumulate(n - 1, i == 1);
+                }
+                if (ok) accumulate(n - 1, tiles == 1);
+            }
+            ++items;
+            ok = __shfl_sync(kAll, (int)ok, 0) != 0;
+        }
+        if (lane == 0) {  // whatever was issued has finished before the tiles and TMEM go
+            ptx::mma_commit(drain);
+            ptx::mbar_wait(drain, 0, nullptr, p.err_word, LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
+        }
+        __syncwarp();
+    } else if (warp >= kSoftmaxWarps) {
+        // ============================================================ unpacking
+        const int w = warp - kSoftmaxWarps, row = lane & 15, side = lane >> 4;
+        constexpr int CHUNKS = D / 64;  // 16-byte pieces of a code row per lane
+        struct Raw {
+            uint4 k[CHUNKS], v[CHUNKS];
+            uint32_t word, have;
+        };
+        while (ok && next_item(p, g, walk)) {
+            Span span;
+            const int tiles = uniform(tiles_of(span)), t0 = uniform(walk.t0), band = uniform(span.band);
+            const int32_t* pages = p.table + (long long)walk.here.b * p.width;
+            walk.at += walk.t1 - walk.t0;
+            // the pool's block of a position, or -1
+            auto block_at = [&](int block) {
+                const int page_at = block / p.pool.page_blocks, page = pages[page_at];
+                if ((unsigned)page >= (unsigned)p.pool.pages) return -1;
+                return (page * p.pool.kv_heads + walk.head) * p.pool.page_blocks + block - page_at * p.pool.page_blocks;
+            };
+            int where = -1;  // blocks of this warp in 32 tiles, a lane per tile
+            auto load = [&](int i, Raw& x) {
+                if (i >= tiles) return;
+                if ((i & 31) == 0) {
+                    const int block = 4 * (span.first + t0 + i + lane) + w;
+                    where = i + lane < tiles && t0 + i + lane < band && block <= span.hi / kBlock ? block_at(block) : -1;
+                }
+                int at, of = row;
+                if (t0 + i < band) {
+                    at = __shfl_sync(kAll, where, i & 31);
+                } else {
+                    const int k = (t0 + i - band) * kKeys + kBlock * w + row;
+                    at = -1;
+                    if (k < span.globals) {
+                        at = block_at(g.at[k] / kBlock);
+                        of = g.at[k] % kBlock;
+                    }
+                }
+                x.have = __ballot_sync(kAll, at >= 0) & 0xffffu;
+                const uint8_t* src = p.pool.data + (long long)at * block_bytes(D);
+                if (at >= 0) {
+                    x.word = *reinterpret_cast<const uint32_t*>(src + (side ? v_words_at(D) : k_words_at(D)) + 4 * of);
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        x.k[c] = *reinterpret_cast<const uint4*>(src + of * row_bytes(D) + 16 * (side + 2 * c));
+                        x.v[c] = *reinterpret_cast<const uint4*>(src + v_codes_at(D) + of * row_bytes(D) + 16 * (side + 2 * c));
+                    }
+                } else {
+                    x.word = 0;
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c) x.k[c] = x.v[c] = make_uint4(0, 0, 0, 0);
+                }
+            };
+            auto store = [&](int i, const Raw& x) {
+                if (i >= tiles) return;
+                const int slot = n % kRing;
+                if (n >= kRing) wait_all(&kv_free[slot], n / kRing - 1);
+                if (!ok) return;
+                float* sk = table + slot * 3 * kKeys;
+                const float scale = __uint_as_float(x.word & ~15u);
+                if (side == 0) {
+                    sk[kBlock * w + row] = scale;
+                } else {
+                    sk[kKeys + kBlock * w + row] = fmaxf(lg2(fabsf(scale)), -100.f);
+                    sk[2 * kKeys + kBlock * w + row] = scale;
+                }
+                if (lane == 0) have_at[slot * 4 + w] = x.have;
+                const uint32_t word_k = __shfl_sync(kAll, x.word, row), word_v = __shfl_sync(kAll, x.word, row + 16);
+                const Zero zk = zero_pair((word_k & 15u) * 0x10001u), zv = zero_pair((word_v & 15u) * 0x10001u);
+                uint8_t* k_tile = smem + C::OFF_KV + slot * 2 * C::KV_BYTES;
+                const int r = kBlock * w + row;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c) {
+                    const uint32_t kw[4] = {x.k[c].x, x.k[c].y, x.k[c].z, x.k[c].w};
+                    const uint32_t vw[4] = {x.v[c].x, x.v[c].y, x.v[c].z, x.v[c].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        // word 4 (side + 2c) + j of the row: 8 elements, 16 bytes of a panel's row
+                        const int word = 4 * (side + 2 * c) + j;
+                        uint8_t* to = k_tile + (word >> 3) * C::KV_PANEL + r * 128 + (((word & 7) ^ (r & 7)) << 4);
+                        *reinterpret_cast<uint4*>(to) = make_uint4(codes_pair(kw[j], 0, zk), codes_pair(kw[j], 1, zk),
+                                                                   codes_pair(kw[j], 2, zk), codes_pair(kw[j], 3, zk));
+                        *reinterpret_cast<uint4*>(to + C::KV_BYTES) =
+                            make_uint4(codes_pair(vw[j], 0, zv), codes_pair(vw[j], 1, zv), codes_pair(vw[j], 2, zv),
+                                       codes_pair(vw[j], 3, zv));
+                    }
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&kv_full[slot]);
+                ++n;
+            };
+            Raw a, b;
+            load(0, a);
+            load(1, b);
+#pragma unroll 1
+            for (int i = 0; i < tiles && ok; i += 2) {
+                store(i, a);
+                load(i + 2, a);
+                store(i + 1, b);
+                load(i + 3, b);
+            }
+        }
+    } else {
+        // ============================================================ softmax
+        const int h = warp >> 2, in_half = 32 * (warp & 3) + lane;
+        const uint32_t mine = tmem + 256 * h + ((uint32_t)(32 * (warp & 3)) << 16);
+        while (ok && next_item(p, g, walk)) {
+            Span span;
+            const int tiles = uniform(tiles_of(span));
+            const Request& r = walk.r;
+            const int of = walk.q_tile * kChunkRows + h * kHalfRows + in_half;
+            const bool valid = of < r.rows;
+            const int token = of / p.group, head = walk.head * p.group + of - token * p.group;
+            const int pos = valid ? r.len - r.rows / p.group + token : -1;
+            int row_lo = max(0, pos - p.window);
+            float factor = 1.f, top = -INFINITY;
+            uint64_t sum2 = ptx::f2_pack(0.f, 0.f);
+            if (tiles > 0) {
+                if (p.num_globals > 0 && span.first == 0 && valid) {
+                    const int k = lower_bound(g.at, p.num_globals, pos);
+                    if (k < p.num_globals && g.at[k] == pos) row_lo = 0;
+                }
+                // ---- this thread's query row, as in kv4_attention.cu: fp16 as it is, bf16 moved by a
+                // power of two, the scale's sign in the row, a factor that is positive and finite
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
+                                                                  (long long)(r.q0 + token) * p.q_token + head * p.q_head);
+                uint32_t raw[D / 2];
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint4 v = valid ? src[i] : make_uint4(0, 0, 0, 0);
+                    raw[4 * i] = v.x, raw[4 * i + 1] = v.y, raw[4 * i + 2] = v.z, raw[4 * i + 3] = v.w;
+                }
+#pragma unroll
+                for (int i = 0; i < D / 2; ++i) most = max(most, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
+                factor = fabsf(p.scale) * kLog2e;
+                float up = 1.f;
+                if (p.bf16) {
+                    const int e = max((int)(most >> 7) - 127, -100);
+                    up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                    factor *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
+                }
+                const bool finite = most < (p.bf16 ? 0x7f80u : 0x7c00u) && factor < INFINITY;
+                const bool zero = factor < 1.17549435e-38f;
+                if (!finite || zero) factor = 1.f;
+                uint8_t* q_row = smem + h * C::Q_BYTES + in_half * 128;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    uint32_t x[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t v = raw[4 * i + j];
+                        if (p.bf16) v = ptx::pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up);
+                        if (p.scale < 0.f) v ^= 0x80008000u;
+                        if (zero) v = 0;
+                        if (!finite) v = 0x7e007e00u;
+                        x[j] = v;
+                    }
+                    *reinterpret_cast<uint4*>(q_row + (i >> 3) * C::Q_PANEL + (((i & 7) ^ (in_half & 7)) << 4)) =
+                        make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632),
+                                   __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632));
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&q_full[h]);
+            }
+            const uint64_t factor2 = ptx::f2_pack(factor, factor);
+
+#pragma unroll 1
+            for (int i = 0; i < tiles; ++i, ++n) {
+                const int slot = n % kRing, buf = n & 1, tile = walk.t0 + i;
+                wait_all(&kv_full[slot], n / kRing);  // complete since its scores are: makes the table visible here
+                wait_all(&s_full[2 * h + buf], n >> 1);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                uint64_t s[kKeys / 2];  // pairs of keys
+                const uint32_t s_at = mine + 128 + 64 * buf;
+                {
+                    float x[32];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        ptx::tmem_ld32(s_at + 32 * half, x);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[16 * half + j] = ptx::f2_pack(x[2 * j], x[2 * j + 1]);
+                    }
+                }
+                const ulonglong2* sk = reinterpret_cast<const ulonglong2*>(table + slot * 3 * kKeys);
+                const ulonglong2 *lam = sk + kKeys / 4, *sv = lam + kKeys / 4;
+#pragma unroll
+                for (int j = 0; j < kKeys / 4; ++j) {
+                    const ulonglong2 a = sk[j];
+                    s[2 * j] = ptx::f2_mul(s[2 * j], a.x);
+                    s[2 * j + 1] = ptx::f2_mul(s[2 * j + 1], a.y);
+                }
+
+                // ---- visibility
+                const bool in_band = tile < span.band;
+                const int key0 = (span.first + tile) * kKeys;
+                const uint64_t have = (uint64_t)(have_at[slot * 4] | (have_at[slot * 4 + 1] << 16)) |
+                                      ((uint64_t)(have_at[slot * 4 + 2] | (have_at[slot * 4 + 3] << 16)) << 32);
+                const bool full = __all_sync(kAll, have == ~0ull && (!valid || !in_band || (row_lo <= key0 && pos >= key0 + kKeys - 1)));
+                uint64_t seen = ~0ull;
+                if (!full) {
+                    uint64_t glob = 0;
+                    if (in_band && p.num_globals > 0) {
+                        uint32_t part[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = key0 + 32 * e + lane, k = lower_bound(g.at, p.num_globals, key);
+                            part[e] = __ballot_sync(kAll, k < p.num_globals && g.at[k] == key);
+                        }
+                        glob = part[0] | (uint64_t)part[1] << 32;
+                    }
+                    if (in_band)
+                        seen = bits_below(pos - key0 + 1) & (~bits_below(row_lo - key0) | glob);
+                    else
+                        seen = pos >= 0 ? ~0ull : 0ull;
+                    seen &= have;
+#pragma unroll
+                    for (int j = 0; j < kKeys / 2; ++j) {
+                        const float x = (seen >> (2 * j)) & 1 ? ptx::f2_lo(s[j]) : -INFINITY;
+                        const float y = (seen >> (2 * j + 1)) & 1 ? ptx::f2_hi(s[j]) : -INFINITY;
+                        s[j] = ptx::f2_pack(x, y);
+                    }
+                }
+
+                // ---- running maximum of x log2(e) + log2(sv)
+                float peak = -INFINITY, peak1 = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < kKeys / 4; ++j) {
+                    const ulonglong2 a = lam[j];
+                    const uint64_t u = ptx::f2_fma(s[2 * j], factor2, a.x), v = ptx::f2_fma(s[2 * j + 1], factor2, a.y);
+                    peak = ptx::fmax3(peak, ptx::f2_lo(u), ptx::f2_hi(u));
+                    peak1 = ptx::fmax3(peak1, ptx::f2_lo(v), ptx::f2_hi(v));
+                }
+                peak = fmaxf(peak, peak1);
+                if (__any_sync(kAll, peak > top + 8.f)) {
+                    const float to = fmaxf(peak, top);
+                    const float f = to == -INFINITY ? 1.f : ptx::ex2(top - to);
+                    top = to;
+                    sum2 = ptx::f2_mul(sum2, ptx::f2_pack(f, f));
+                    if (i > 0) {
+                        wait_all(&pv_done[2 * h + ((n - 1) & 1)], (n - 1) >> 1);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            float x[32];
+                            ptx::tmem_ld32(mine + c, x);
+                            ptx::tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) x[j] *= f;
+                            ptx::tmem_st32(mine + c, x);
+                        }
+                        ptx::tmem_wait_st();
+                    }
+                }
+
+                // ---- weights
+                const float ref = top == -INFINITY ? 0.f : -top;
+                const uint64_t ref2 = ptx::f2_pack(ref, ref);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t hi[kKeys / 4], lo[kKeys / 4];
+#pragma unroll
+                    for (int k = 0; k < kKeys / 4; ++k) {
+                        const int j = half * (kKeys / 4) + k;
+                        const uint64_t x = ptx::f2_fma(s[j], factor2, ref2);
+                        const uint64_t e = ptx::f2_pack(ptx::ex2(ptx::f2_lo(x)), ptx::ex2(ptx::f2_hi(x)));
+                        sum2 = ptx::f2_add(sum2, e);
+                        const ulonglong2 v4 = sv[j >> 1];
+                        const uint64_t w = ptx::f2_mul(e, (j & 1) ? v4.y : v4.x);
+                        float w0 = ptx::f2_lo(w), w1 = ptx::f2_hi(w);
+                        if (!full) {  // 0 also where the scale of a key out of sight is not finite
+                            if (!((seen >> (2 * j)) & 1)) w0 = 0.f;
+                            if (!((seen >> (2 * j + 1)) & 1)) w1 = 0.f;
+                        }
+                        hi[k] = ptx::pack_f16x2(w0, w1);
+                        if (SPLIT_W) {
+                            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+                            lo[k] = ptx::pack_f16x2(w0 - back.x, w1 - back.y);
+                        }
+                    }
+                    ptx::tmem_st16u(s_at + kKeys / 4 * half, hi);
+                    if constexpr (SPLIT_W) ptx::tmem_st16u(s_at + kKeys / 2 + kKeys / 4 * half, lo);
+                }
+                ptx::tmem_wait_st();
+                ptx::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&p_full[2 * h + buf]);
+            }
+
+            // ---- the row's output, or its part
+            if (ok && tiles > 0) {
+                wait_all(&pv_done[2 * h + ((n - 1) & 1)], (n - 1) >> 1);
+                ptx::tc_fence_after();
+            }
+            if (!ok) break;
+            const float sum = ptx::f2_lo(sum2) + ptx::f2_hi(sum2);
+            const bool whole = walk.t0 == 0 && walk.t1 == r.tiles;
+            const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+            const long long part = (long long)(2 * blockIdx.x + (walk.at != line_at)) * kChunkRows + h * kHalfRows + in_half;
+            const long long out_at = ((long long)(r.q0 + token) * p.heads + head) * D;
+            if (valid) {
+                if (!whole) {
+                    p.part_ml[part] = make_float2(top, sum);
+                } else if (p.lse != nullptr) {
+                    p.lse[(long long)head * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+                }
+            }
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float x[32];
+                if (tiles > 0) {
+                    ptx::tmem_ld32(mine + c, x);
+                    ptx::tmem_wait_ld();
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = tiles == 0 || (whole && sum == 0.f) ? 0.f : x[j] * inv;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {  // back from the order 0 4 1 5 2 6 3 7
+                    if (!valid) break;
+                    const float a[4] = {x[j], x[j + 2], x[j + 4], x[j + 6]}, b[4] = {x[j + 1], x[j + 3], x[j + 5], x[j + 7]};
+                    if (whole) {
+                        store_out(p, p.out_dtype, out_at + c + j, a);
+                        store_out(p, p.out_dtype, out_at + c + j + 4, b);
+                    } else {
+                        *reinterpret_cast<float4*>(p.part_o + part * D + c + j) = make_float4(a[0], a[1], a[2], a[3]);
+                        *reinterpret_cast<float4*>(p.part_o + part * D + c + j + 4) = make_float4(b[0], b[1], b[2], b[3]);
+                    }
+                }
+                __syncwarp();
+            }
+            ptx::tc_fence_before();  // the next item's products overwrite what was read here
+            walk.at += walk.t1 - walk.t0;
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <int D, bool SPLIT_W>
+cudaError_t chunk_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(kv4_chunk<D, SPLIT_W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+    if (e != cudaSuccess) return e;
+    kv4_chunk<D, SPLIT_W><<<p.ctas, kThreads, Cfg<D>::SMEM, stream>>>(p, g);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_chunk(int d, const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;
+    if (d == 64) return split_w ? chunk_of<64, true>(p, g, stream) : chunk_of<64, false>(p, g, stream);
+    return split_w ? chunk_of<128, true>(p, g, stream) : chunk_of<128, false>(p, g, stream);
+}
+
+}  // namespace kv4
+}  // namespace lca
