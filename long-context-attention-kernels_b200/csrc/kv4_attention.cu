@@ -698,7 +698,8 @@ AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t h
     const int64_t longest = band + (num_globals + tile - 1) / tile;
     // Long items are cut wherever a CTA's share of the line ends, and merged by a second kernel;
     // short ones (a band) stay whole, which saves that launch.
-    a.split = longest > kWholeTiles;
+    // Many long items of many rows balance by themselves, and their parts are large.
+    a.split = longest > kWholeTiles && (!chunk || items < 4 * kSms);
     a.min_tiles = chunk ? 4 : kMinTiles;
     const int per_sm = chunk ? 1 : (a.tile_rows == 8 ? 4 : (a.tile_rows == 16 ? 3 : 2));
     a.items = std::min<int64_t>(items, 0x7fffffff);

@@ -99,6 +99,19 @@ __device__ __forceinline__ bool next_item(const AttnParams& p, const Globals& g,
 // One row of 64 keys' bits below key index n.
 __device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1); }
 
+// Where element e of a group of 8 lies in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ constexpr int place(int e) { return e < 4 ? 2 * e : 2 * e - 7; }
+
+// 32 columns of this thread's row of O, times `inv`; zeros where there is nothing to read.
+__device__ __forceinline__ void read_out(float (&x)[32], uint32_t taddr, bool some, bool any, float inv) {
+    if (any) {  // the same in the whole warp
+        ptx::tmem_ld32(taddr, x);
+        ptx::tmem_wait_ld();
+    }
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = some ? x[j] * inv : 0.f;
+}
+
 template <int D, bool SPLIT_W>
 __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, const __grid_constant__ Globals g) {
     using C = Cfg<D>;
@@ -359,45 +372,53 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     const int k = lower_bound(g.at, p.num_globals, pos);
                     if (k < p.num_globals && g.at[k] == pos) row_lo = 0;
                 }
-                // ---- this thread's query row, as in kv4_attention.cu: fp16 as it is, bf16 moved by a
-                // power of two, the scale's sign in the row, a factor that is positive and finite
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
-                                                                  (long long)(r.q0 + token) * p.q_token + head * p.q_head);
-                uint32_t raw[D / 2];
-                uint32_t most = 0;
+                // ---- the warp's 32 query rows, D / 8 lanes a row (a thread per row would touch 32 lines an
+                // instruction).  As in kv4_attention.cu: fp16 as it is, bf16 moved by a power of two, the
+                // scale's sign in the row, a factor that is positive and finite.
+                constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+                const int piece = lane % LANES, sub = lane / LANES;
+                const int first_of = walk.q_tile * kChunkRows + h * kHalfRows + 32 * (warp & 3);
+                uint4 raw[LANES];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint4 v = valid ? src[i] : make_uint4(0, 0, 0, 0);
-                    raw[4 * i] = v.x, raw[4 * i + 1] = v.y, raw[4 * i + 2] = v.z, raw[4 * i + 3] = v.w;
+                for (int i = 0; i < LANES; ++i) {
+                    const int x = first_of + AT_ONCE * i + sub, tok = x / p.group;
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (x < r.rows)
+                        raw[i] = *reinterpret_cast<const uint4*>(
+                            static_cast<const uint16_t*>(p.q) + (long long)(r.q0 + tok) * p.q_token +
+                            (long long)(walk.head * p.group + x - tok * p.group) * p.q_head + 8 * piece);
                 }
 #pragma unroll
-                for (int i = 0; i < D / 2; ++i) most = max(most, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
-                factor = fabsf(p.scale) * kLog2e;
-                float up = 1.f;
-                if (p.bf16) {
-                    const int e = max((int)(most >> 7) - 127, -100);
-                    up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-                    factor *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
-                }
-                const bool finite = most < (p.bf16 ? 0x7f80u : 0x7c00u) && factor < INFINITY;
-                const bool zero = factor < 1.17549435e-38f;
-                if (!finite || zero) factor = 1.f;
-                uint8_t* q_row = smem + h * C::Q_BYTES + in_half * 128;
+                for (int i = 0; i < LANES; ++i) {
+                    uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w}, most = 0;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    uint32_t x[4];
+                    for (int j = 0; j < 4; ++j) most = max(most, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
+#pragma unroll
+                    for (int o = 1; o < LANES; o *= 2) most = max(most, __shfl_xor_sync(kAll, most, o));
+                    float mult = fabsf(p.scale) * kLog2e, up = 1.f;
+                    if (p.bf16) {
+                        const int e = max((int)(most >> 7) - 127, -100);
+                        up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+                        mult *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
+                    }
+                    const bool finite = most < (p.bf16 ? 0x7f80u : 0x7c00u) && mult < INFINITY;
+                    const bool zero = mult < 1.17549435e-38f;
+                    if (!finite || zero) mult = 1.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        uint32_t v = raw[4 * i + j];
-                        if (p.bf16) v = ptx::pack_f16x2(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up);
-                        if (p.scale < 0.f) v ^= 0x80008000u;
-                        if (zero) v = 0;
-                        if (!finite) v = 0x7e007e00u;
-                        x[j] = v;
+                        if (p.bf16)
+                            x[j] = ptx::pack_f16x2(__uint_as_float(x[j] << 16) * up, __uint_as_float(x[j] & 0xffff0000u) * up);
+                        if (p.scale < 0.f) x[j] ^= 0x80008000u;
+                        if (zero) x[j] = 0;
+                        if (!finite) x[j] = 0x7e007e00u;
                     }
-                    *reinterpret_cast<uint4*>(q_row + (i >> 3) * C::Q_PANEL + (((i & 7) ^ (in_half & 7)) << 4)) =
+                    const int to_row = 32 * (warp & 3) + AT_ONCE * i + sub;
+                    *reinterpret_cast<uint4*>(smem + h * C::Q_BYTES + (piece >> 3) * C::Q_PANEL + to_row * 128 +
+                                              (((piece & 7) ^ (to_row & 7)) << 4)) =
                         make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632),
                                    __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632));
+                    const float of_row = __shfl_sync(kAll, mult, (lane % AT_ONCE) * LANES);
+                    if (lane / AT_ONCE == i) factor = of_row;
                 }
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
@@ -548,28 +569,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     p.lse[(long long)head * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
                 }
             }
+            if (whole && p.out_dtype != LCA_DTYPE_F32) {
+                // 16-bit rows go through the warp's own rows of the query tile, which nothing reads any more,
+                // and leave as whole rows, D / 8 lanes each
+                auto stage = [&](int row, int piece) {
+                    return reinterpret_cast<uint4*>(smem + h * C::Q_BYTES + (piece >> 3) * C::Q_PANEL +
+                                                    (32 * (warp & 3) + row) * 128 + (((piece & 7) ^ (row & 7)) << 4));
+                };
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                float x[32];
-                if (tiles > 0) {
-                    ptx::tmem_ld32(mine + c, x);
-                    ptx::tmem_wait_ld();
-                }
+                for (int c = 0; c < D; c += 32) {
+                    float x[32];
+                    read_out(x, mine + c, tiles > 0 && sum != 0.f, tiles > 0, inv);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = tiles == 0 || (whole && sum == 0.f) ? 0.f : x[j] * inv;
+                    for (int j = 0; j < 32; j += 8) {
+                        uint32_t v[4];
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {  // back from the order 0 4 1 5 2 6 3 7
-                    if (!valid) break;
-                    const float a[4] = {x[j], x[j + 2], x[j + 4], x[j + 6]}, b[4] = {x[j + 1], x[j + 3], x[j + 5], x[j + 7]};
-                    if (whole) {
-                        store_out(p, p.out_dtype, out_at + c + j, a);
-                        store_out(p, p.out_dtype, out_at + c + j + 4, b);
-                    } else {
-                        *reinterpret_cast<float4*>(p.part_o + part * D + c + j) = make_float4(a[0], a[1], a[2], a[3]);
-                        *reinterpret_cast<float4*>(p.part_o + part * D + c + j + 4) = make_float4(b[0], b[1], b[2], b[3]);
+                        for (int k = 0; k < 4; ++k)  // back from the order 0 4 1 5 2 6 3 7
+                            v[k] = p.out_dtype == LCA_DTYPE_F16
+                                       ? ptx::pack_f16x2(x[j + place(2 * k)], x[j + place(2 * k + 1)])
+                                                                : ptx::pack_bf16x2(x[j + place(2 * k)], x[j + place(2 * k + 1)]);
+                        *stage(lane, (c + j) / 8) = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 }
                 __syncwarp();
+                constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+#pragma unroll 4
+                for (int i = 0; i < LANES; ++i) {
+                    const int row = AT_ONCE * i + lane / LANES, piece = lane % LANES;
+                    const int x = walk.q_tile * kChunkRows + h * kHalfRows + 32 * (warp & 3) + row, tok = x / p.group;
+                    if (x < r.rows)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
+                                                  ((long long)(r.q0 + tok) * p.heads + walk.head * p.group + x - tok * p.group) * D +
+                                                  8 * piece) = *stage(row, piece);
+                }
+                __syncwarp();
+            } else {
+                float* to = whole ? static_cast<float*>(p.out) + out_at : p.part_o + part * D;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float x[32];
+                    read_out(x, mine + c, tiles > 0 && !(whole && sum == 0.f), tiles > 0, inv);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float* v = x + (j & ~7);
+                        const int k = j & 4;
+                        if (valid)
+                            *reinterpret_cast<float4*>(to + c + j) =
+                                make_float4(v[place(k)], v[place(k + 1)], v[place(k + 2)], v[place(k + 3)]);
+                    }
+                    __syncwarp();
+                }
             }
             ptx::tc_fence_before();  // the next item's products overwrite what was read here
             walk.at += walk.t1 - walk.t0;
