@@ -233,10 +233,20 @@ int type_code(c10::ScalarType t, const char* name) {
     return t == torch::kFloat32 ? LCA_DTYPE_F32 : (t == torch::kBFloat16 ? LCA_DTYPE_BF16 : LCA_DTYPE_F16);
 }
 
+// Elements [from, from + n) of a contiguous 1-D tensor, sharing its storage.  Made directly: eight of
+// these through the dispatcher cost more host time than the call they return from.
+torch::Tensor part_of(const torch::Tensor& all, int64_t from, int64_t n) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(all.storage_offset() + from);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(c10::IntArrayRef(&n, 1));
+    return t;
+}
+
 void* current_stream() { return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream()); }
 
-std::vector<torch::Tensor> kv_cache_layout(torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor new_lens,
-                                           torch::Tensor free_pages, torch::Tensor free_count, int64_t page_size,
+std::vector<torch::Tensor> kv_cache_layout(const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                                           const torch::Tensor& new_lens, const torch::Tensor& free_pages,
+                                           const torch::Tensor& free_count, int64_t page_size,
                                            int64_t num_tokens) {
     const auto device = block_table.device();
     check_ints(block_table, "block_table", 2, device);
@@ -260,13 +270,14 @@ std::vector<torch::Tensor> kv_cache_layout(torch::Tensor block_table, torch::Ten
                                free_count.data_ptr<int32_t>(), page_size, num_tokens, slots, positions, cu, kv_lens,
                                placed, next, count, current_stream()),
                  "kv_cache_layout");
-    auto part = [&](int32_t* from, int64_t n) { return all.narrow(0, from - at, n); };
+    auto part = [&](int32_t* from, int64_t n) { return part_of(all, from - at, n); };
     return {part(slots, num_tokens), part(positions, num_tokens), part(cu, batch + 1), part(kv_lens, batch),
             part(placed, batch),     part(next, batch),           part(count, 1),      part(next, batch + 1)};
 }
 
-std::vector<torch::Tensor> kv_cache_release(torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor release,
-                                            torch::Tensor free_pages, torch::Tensor free_count, int64_t page_size) {
+std::vector<torch::Tensor> kv_cache_release(const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                                            const torch::Tensor& release, const torch::Tensor& free_pages,
+                                            const torch::Tensor& free_count, int64_t page_size) {
     const auto device = block_table.device();
     check_ints(block_table, "block_table", 2, device);
     check_ints(seq_lens, "seq_lens", 1, device);
@@ -287,10 +298,10 @@ std::vector<torch::Tensor> kv_cache_release(torch::Tensor block_table, torch::Te
                                 free_pages.data_ptr<int32_t>(), free_pages.size(0), free_count.data_ptr<int32_t>(),
                                 page_size, at, at + batch, current_stream()),
                  "kv_cache_release");
-    return {next.narrow(0, 0, batch), next.narrow(0, batch, 1), next};
+    return {part_of(next, 0, batch), part_of(next, batch, 1), next};
 }
 
-void kv_cache_append(torch::Tensor pool, torch::Tensor k, torch::Tensor v, torch::Tensor slots) {
+void kv_cache_append(const torch::Tensor& pool, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& slots) {
     const PoolShape s = check_pool(pool);
     check_ints(slots, "slots", 1, pool.device());
     for (const torch::Tensor* t : {&k, &v}) {
@@ -310,7 +321,7 @@ void kv_cache_append(torch::Tensor pool, torch::Tensor k, torch::Tensor v, torch
                  "kv_cache_append");
 }
 
-std::vector<torch::Tensor> kv_cache_read(torch::Tensor pool, torch::Tensor slots, c10::ScalarType out_dtype) {
+std::vector<torch::Tensor> kv_cache_read(const torch::Tensor& pool, const torch::Tensor& slots, c10::ScalarType out_dtype) {
     const PoolShape s = check_pool(pool);
     check_ints(slots, "slots", 1, pool.device());
     const int code = type_code(out_dtype, "out_dtype");
@@ -323,12 +334,12 @@ std::vector<torch::Tensor> kv_cache_read(torch::Tensor pool, torch::Tensor slots
     return {k, v};
 }
 
-std::vector<torch::Tensor> sliding_window_attention_cached(torch::Tensor Q, torch::Tensor pool,
-                                                           torch::Tensor block_table, torch::Tensor kv_lens,
-                                                           torch::Tensor cu_seqlens, int64_t window_size,
-                                                           std::vector<int64_t> global_tokens, double scale,
+std::vector<torch::Tensor> sliding_window_attention_cached(const torch::Tensor& Q, const torch::Tensor& pool,
+                                                           const torch::Tensor& block_table, const torch::Tensor& kv_lens,
+                                                           const torch::Tensor& cu_seqlens, int64_t window_size,
+                                                           const std::vector<int64_t>& global_tokens, double scale,
                                                            c10::ScalarType out_dtype, bool want_lse,
-                                                           c10::optional<torch::Tensor> out) {
+                                                           const c10::optional<torch::Tensor>& out) {
     const PoolShape s = check_pool(pool);
     const auto device = pool.device();
     check_ints(block_table, "block_table", 2, device);

@@ -657,7 +657,8 @@ cudaError_t merge_of(const AttnParams& p, const Globals& g, cudaStream_t stream)
 template <int D, int NT, bool SPLIT_W>
 cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
     const int smem = Cfg<D, NT>::SMEM;
-    cudaError_t e = cudaFuncSetAttribute(kv4_attention<D, NT, SPLIT_W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = allow_smem(kv4_attention<D, NT, SPLIT_W>, smem, done);
     if (e != cudaSuccess) return e;
     kv4_attention<D, NT, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
     e = cudaGetLastError();

@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kv4.h"
 #include "sm100_ptx.cuh"
 
@@ -208,6 +210,19 @@ __device__ __forceinline__ long long whole_line(const AttnParams& p, const Globa
     long long sum = 0, before;
     for (int b = threadIdx.x; b < p.batch; b += THREADS) sum += line_of(p, request_of<ROWS, TILE>(p, g, b));
     return block_scan<THREADS>(sum, scratch, &before);
+}
+
+// Dynamic shared memory beyond 48 KB for a kernel, asked for once per device.
+template <typename F>
+inline cudaError_t allow_smem(F* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 __device__ __forceinline__ void store_out(const AttnParams& p, int out_dtype, long long at, const float (&v)[4]) {

@@ -181,11 +181,29 @@ __global__ void __launch_bounds__(kLayoutThreads) kv_release(const ReleaseParams
 // ------------------------------------------------------------------ rows
 
 template <typename T>
-__device__ __forceinline__ float to_float(T x);
+struct Half;  // the two 16-bit inputs: a pair of elements is a 32-bit word
 template <>
-__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
+struct Half<__half> {
+    static constexpr uint32_t kSign = 0x80008000u;
+    static __device__ __forceinline__ float low(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)w)); }
+    static __device__ __forceinline__ float high(uint32_t w) { return __half2float(__ushort_as_half((uint16_t)(w >> 16))); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // NaN if either is
+        uint32_t d;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+};
 template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+struct Half<__nv_bfloat16> {
+    static constexpr uint32_t kSign = 0x80008000u;
+    static __device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+    static __device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+};
 
 __device__ __forceinline__ uint8_t* block_of(const Pool& pool, int d, int slot, int head, int* row) {
     const int block = slot / kBlock;
@@ -198,93 +216,111 @@ __device__ __forceinline__ bool slot_ok(const Pool& pool, int slot) {
     return slot >= 0 && slot / (kBlock * pool.page_blocks) < pool.pages;
 }
 
-// Quantises one row held by LANES lanes, 8 elements a lane, and stores it.  With lo = min(row, 0)
-// and hi = max(row, 0): scale = hi/15 - lo/15 (products with fp32 1/15, so that opposite extremes
-// of bf16 do not overflow) with its low four bits cleared, z = rint(-lo / scale), code =
-// clamp(rint(x / scale) + z, 0, 15); quotients are fp32 products with 1 / scale.  Every operation
-// is the IEEE one (no contraction), so the codes are a function of the row alone.  A scale
-// below the smallest normal number stores zeros; a row with an infinity or a NaN stores NaN.
-template <int LANES>
-__device__ __forceinline__ void store_row(const float (&x)[8], int lane, uint8_t* codes, uint8_t* word) {
-    float hi = 0.f, lo = 0.f;
-    bool finite = true;
+// Quantises one row held by LANES lanes, 8 elements (four pairs) a lane: the lane's word of codes,
+// and the row's word of scale and zero point.  With lo = min(row, 0) and hi = max(row, 0): scale =
+// hi/15 - lo/15 (products with fp32 1/15, so that opposite extremes of bf16 do not overflow) with
+// its low four bits cleared, z = rint(-lo / scale), code = clamp(rint(x / scale) + z, 0, 15);
+// quotients are fp32 products with 1 / scale.  Every operation is the IEEE one (no contraction), so
+// the codes are a function of the row alone.  A scale below the smallest normal number stores
+// zeros; a row with an infinity or a NaN stores NaN.
+//
+// The extremes are found on the 16-bit pairs, (max x, max -x) in one word across the lanes, so a
+// step takes one shuffle and one instruction.  rint(y) for |y| < 2^22 is the sum with 1.5 * 2^23, whose
+// low bits are the integer (rint and the conversion to int run at a quarter of that rate).
+template <int LANES, typename T>
+__device__ __forceinline__ void quantise(const uint32_t (&x)[4], uint32_t* codes, uint32_t* word) {
+    using H = Half<T>;
+    const uint32_t up = H::max2(H::max2(x[0], x[1]), H::max2(x[2], x[3]));
+    const uint32_t down = H::max2(H::max2(x[0] ^ H::kSign, x[1] ^ H::kSign), H::max2(x[2] ^ H::kSign, x[3] ^ H::kSign));
+    uint32_t ends = H::max2(__byte_perm(up, down, 0x5410), __byte_perm(up, down, 0x7632));
+    ends = H::max2(ends, 0u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi = fmaxf(hi, x[i]);
-        lo = fminf(lo, x[i]);
-        finite &= fabsf(x[i]) < INFINITY;
-    }
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o /= 2) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        finite &= __shfl_xor_sync(0xffffffffu, (int)finite, o) != 0;
-    }
-    constexpr float k15 = 1.0f / 15.0f;
-    float scale = __fsub_rn(__fmul_rn(hi, k15), __fmul_rn(lo, k15));
+    for (int o = LANES / 2; o > 0; o /= 2) ends = H::max2(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+    const float hi = H::low(ends), minus_lo = H::high(ends);
+    constexpr float k15 = 1.0f / 15.0f, kMagic = 12582912.f;
+    float scale = __fadd_rn(__fmul_rn(hi, k15), __fmul_rn(minus_lo, k15));
     scale = __uint_as_float(__float_as_uint(scale) & ~15u);
+    const bool finite = hi < INFINITY && minus_lo < INFINITY;
     const bool normal = finite && scale >= 1.17549435e-38f;
     const float inv = normal ? __frcp_rn(scale) : 0.f;
-    const float z = normal ? rintf(__fmul_rn(-lo, inv)) : 0.f;
-    uint32_t w = 0;
+    const float zm = normal ? __fadd_rn(__fmul_rn(minus_lo, inv), kMagic) : kMagic;  // kMagic + z
+    const float z = __fsub_rn(zm, kMagic);
+    uint32_t w = 0, ones = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float c = fminf(fmaxf(__fadd_rn(rintf(__fmul_rn(x[i], inv)), z), 0.f), 15.f);
-        w |= (normal ? (uint32_t)c : 0u) << (4 * i);
+    for (int i = 7; i >= 0; --i) {
+        const float v = (i & 1) ? H::high(x[i >> 1]) : H::low(x[i >> 1]);
+        const float c = fminf(fmaxf(__fadd_rn(__fadd_rn(__fmul_rn(v, inv), kMagic), z), kMagic), kMagic + 15.f);
+        w = w * 16u + __float_as_uint(c);  // the bits of kMagic are taken off at the end
+        ones = ones * 16u + 1u;
     }
-    if (lane >= 0) {
-        reinterpret_cast<uint32_t*>(codes)[lane] = w;
-        if (lane == 0)
-            *reinterpret_cast<uint32_t*>(word) =
-                normal ? __float_as_uint(scale) | (uint32_t)z : (finite ? 0u : 0x7fc00000u);
-    }
+    *codes = normal ? w - ones * 0x4b400000u : 0u;
+    *word = normal ? __float_as_uint(scale) | (__float_as_uint(zm) & 15u) : (finite ? 0u : 0x7fc00000u);
 }
 
 constexpr int kRowThreads = 256;
+constexpr int kRowItems = 2;  // (token, head) pairs of a group of lanes, whose loads are in flight together
 
-// One group of d / 8 lanes per (token, head): the group loads 16 bytes a lane of the K and of the
-// V row, reduces the extremes by shuffles and stores one 32-bit word of codes a lane.  Bound by
-// memory: 4d bytes read and d + 8 written a (token, head).
+struct Item {
+    int token, head, slot;
+    bool keep;
+};
+
+// Pair number `item` of the call (32-bit division where the count allows: a 64-bit one costs more
+// than the rest of the row).
+__device__ __forceinline__ Item item_of(const RowsParams& p, long long item, long long items) {
+    Item r = {0, 0, -1, false};
+    if (item >= items) return r;
+    r.token = items <= 0xffffffffll ? (int)((uint32_t)item / (uint32_t)p.pool.kv_heads) : (int)(item / p.pool.kv_heads);
+    r.head = (int)(item - (long long)r.token * p.pool.kv_heads);
+    r.slot = p.slots[r.token];
+    r.keep = slot_ok(p.pool, r.slot);
+    return r;
+}
+
+// One group of d / 8 lanes per (token, head), kRowItems of them at a time: a lane loads 16 bytes of
+// the K and of the V row and stores one 32-bit word of codes of each.  Bound by memory: 4d
+// bytes read and d + 8 written a pair.
 template <int D, typename T, bool VECTOR>
 __global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
     constexpr int LANES = D / 8, GROUPS = kRowThreads / LANES;
-    const long long item = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES;
     const long long items = (long long)p.rows * p.pool.kv_heads;
-    const bool inside = item < items;
-    const int token = inside ? (int)(item / p.pool.kv_heads) : 0;
-    const int head = inside ? (int)(item - (long long)token * p.pool.kv_heads) : 0;
-    const int slot = inside ? p.slots[token] : -1;
-    const bool keep = slot_ok(p.pool, slot);
-    float k[8], v[8];
-    const T* kp = static_cast<const T*>(p.k) + token * p.k_token + head * p.k_head + lane * 8;
-    const T* vp = static_cast<const T*>(p.v) + token * p.v_token + head * p.v_head + lane * 8;
-    if (keep) {
-        if (VECTOR) {
-            const uint4 a = *reinterpret_cast<const uint4*>(kp), b = *reinterpret_cast<const uint4*>(vp);
-            const T* at = reinterpret_cast<const T*>(&a);
-            const T* bt = reinterpret_cast<const T*>(&b);
+    const long long first = (long long)blockIdx.x * (GROUPS * kRowItems) + threadIdx.x / LANES;
+    Item at[kRowItems];
+    uint32_t k[kRowItems][4], v[kRowItems][4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                k[i] = to_float<T>(at[i]);
-                v[i] = to_float<T>(bt[i]);
-            }
-        } else {
+    for (int j = 0; j < kRowItems; ++j) at[j] = item_of(p, first + j * GROUPS, items);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                k[i] = to_float<T>(kp[i]);
-                v[i] = to_float<T>(vp[i]);
+    for (int j = 0; j < kRowItems; ++j) {
+        const T* kp = static_cast<const T*>(p.k) + at[j].token * p.k_token + at[j].head * p.k_head + lane * 8;
+        const T* vp = static_cast<const T*>(p.v) + at[j].token * p.v_token + at[j].head * p.v_head + lane * 8;
+        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        if (at[j].keep) {
+            if (VECTOR) {
+                a = *reinterpret_cast<const uint4*>(kp);
+                b = *reinterpret_cast<const uint4*>(vp);
+            } else {
+                const uint16_t *k16 = reinterpret_cast<const uint16_t*>(kp), *v16 = reinterpret_cast<const uint16_t*>(vp);
+                a = make_uint4(k16[0] | k16[1] << 16, k16[2] | k16[3] << 16, k16[4] | k16[5] << 16, k16[6] | k16[7] << 16);
+                b = make_uint4(v16[0] | v16[1] << 16, v16[2] | v16[3] << 16, v16[4] | v16[5] << 16, v16[6] | v16[7] << 16);
             }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+        k[j][0] = a.x, k[j][1] = a.y, k[j][2] = a.z, k[j][3] = a.w;
+        v[j][0] = b.x, v[j][1] = b.y, v[j][2] = b.z, v[j][3] = b.w;
     }
-    int row = 0;
-    uint8_t* block = keep ? block_of(p.pool, D, slot, head, &row) : p.pool.data;
-    const int who = keep ? lane : -1;  // every lane takes part in the shuffles
-    store_row<LANES>(k, who, block + row * row_bytes(D), block + k_words_at(D) + 4 * row);
-    store_row<LANES>(v, who, block + v_codes_at(D) + row * row_bytes(D), block + v_words_at(D) + 4 * row);
+#pragma unroll
+    for (int j = 0; j < kRowItems; ++j) {
+        uint32_t k_codes, k_word, v_codes, v_word;  // every lane takes part in the shuffles
+        quantise<LANES, T>(k[j], &k_codes, &k_word);
+        quantise<LANES, T>(v[j], &v_codes, &v_word);
+        if (!at[j].keep) continue;
+        int row;
+        uint8_t* block = block_of(p.pool, D, at[j].slot, at[j].head, &row);
+        reinterpret_cast<uint32_t*>(block + row * row_bytes(D))[lane] = k_codes;
+        reinterpret_cast<uint32_t*>(block + v_codes_at(D) + row * row_bytes(D))[lane] = v_codes;
+        if (lane == 0) *reinterpret_cast<uint32_t*>(block + k_words_at(D) + 4 * row) = k_word;
+        if (lane == 1) *reinterpret_cast<uint32_t*>(block + v_words_at(D) + 4 * row) = v_word;
+    }
 }
 
 template <typename T>
@@ -309,13 +345,12 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* to, const f
     *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
 }
 
-__device__ __forceinline__ void load_row(const uint8_t* codes, const uint8_t* word, int lane, float (&x)[8]) {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(codes)[lane];
-    const uint32_t sw = *reinterpret_cast<const uint32_t*>(word);
-    const float scale = __uint_as_float(sw & ~15u);
-    const int z = (int)(sw & 15u);
+// The eight values of a word of codes: 1.5 * 2^23 + code is the code in the low bits of that number.
+__device__ __forceinline__ void values_of(uint32_t codes, uint32_t word, float (&x)[8]) {
+    const float scale = __uint_as_float(word & ~15u), less = __uint_as_float(0x4b400000u | (word & 15u));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(scale, (float)((int)((w >> (4 * i)) & 15u) - z));
+    for (int i = 0; i < 8; ++i)
+        x[i] = __fmul_rn(scale, __fsub_rn(__uint_as_float(((codes >> (4 * i)) & 15u) | 0x4b400000u), less));
 }
 
 // The rows of `slots` as values, rounded once to the output's type; a slot outside the pool reads
@@ -323,27 +358,36 @@ __device__ __forceinline__ void load_row(const uint8_t* codes, const uint8_t* wo
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowThreads) kv4_read(const RowsParams p) {
     constexpr int LANES = D / 8, GROUPS = kRowThreads / LANES;
-    const long long item = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES;
     const int lane = threadIdx.x % LANES;
-    if (item >= (long long)p.rows * p.pool.kv_heads) return;
-    const int token = (int)(item / p.pool.kv_heads), head = (int)(item - (long long)token * p.pool.kv_heads);
-    const int slot = p.slots[token];
-    float k[8], v[8];
-    if (slot_ok(p.pool, slot)) {
-        int row;
-        const uint8_t* block = block_of(p.pool, D, slot, head, &row);
-        load_row(block + row * row_bytes(D), block + k_words_at(D) + 4 * row, lane, k);
-        load_row(block + v_codes_at(D) + row * row_bytes(D), block + v_words_at(D) + 4 * row, lane, v);
-    } else {
+    const long long items = (long long)p.rows * p.pool.kv_heads;
+    const long long first = (long long)blockIdx.x * (GROUPS * kRowItems) + threadIdx.x / LANES;
+    Item at[kRowItems];
+    uint32_t k[kRowItems] = {}, v[kRowItems] = {}, kw[kRowItems] = {}, vw[kRowItems] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) k[i] = v[i] = 0.f;
+    for (int j = 0; j < kRowItems; ++j) at[j] = item_of(p, first + j * GROUPS, items);
+#pragma unroll
+    for (int j = 0; j < kRowItems; ++j) {
+        if (!at[j].keep) continue;
+        int row;
+        const uint8_t* block = block_of(p.pool, D, at[j].slot, at[j].head, &row);
+        k[j] = reinterpret_cast<const uint32_t*>(block + row * row_bytes(D))[lane];
+        v[j] = reinterpret_cast<const uint32_t*>(block + v_codes_at(D) + row * row_bytes(D))[lane];
+        kw[j] = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row);
+        vw[j] = *reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row);
     }
-    store8<T>(static_cast<T*>(p.k) + token * p.k_token + head * p.k_head + lane * 8, k);
-    store8<T>(static_cast<T*>(p.v) + token * p.v_token + head * p.v_head + lane * 8, v);
+#pragma unroll
+    for (int j = 0; j < kRowItems; ++j) {
+        if (first + j * GROUPS >= items) continue;
+        float x[8];
+        values_of(k[j], kw[j], x);
+        store8<T>(static_cast<T*>(p.k) + at[j].token * p.k_token + at[j].head * p.k_head + lane * 8, x);
+        values_of(v[j], vw[j], x);
+        store8<T>(static_cast<T*>(p.v) + at[j].token * p.v_token + at[j].head * p.v_head + lane * 8, x);
+    }
 }
 
 unsigned row_blocks(int d, const RowsParams& p) {
-    const long long groups = kRowThreads / (d / 8);
+    const long long groups = kRowThreads / (d / 8) * kRowItems;
     return (unsigned)(((long long)p.rows * p.pool.kv_heads + groups - 1) / groups);
 }
 

@@ -634,7 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 
 template <int D, bool SPLIT_W>
 cudaError_t chunk_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_chunk<D, SPLIT_W>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+    static std::atomic<unsigned long long> done{0};
+    cudaError_t e = allow_smem(kv4_chunk<D, SPLIT_W>, Cfg<D>::SMEM, done);
     if (e != cudaSuccess) return e;
     kv4_chunk<D, SPLIT_W><<<p.ctas, kThreads, Cfg<D>::SMEM, stream>>>(p, g);
     return cudaGetLastError();
