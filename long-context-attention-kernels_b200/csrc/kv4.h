@@ -31,10 +31,27 @@ __host__ __device__ constexpr int v_codes_at(int d) { return kBlock * d / 2; }
 __host__ __device__ constexpr int k_words_at(int d) { return kBlock * d; }
 __host__ __device__ constexpr int v_words_at(int d) { return kBlock * d + 4 * kBlock; }
 
+// Division by a number that a call fixes, as a multiplication (Granlund and Montgomery 1994): for n and
+// d below 2^31, n / d = (n + floor(n m / 2^32)) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d)
+// + 1.
+struct Divisor {
+    uint32_t d, m, s;
+    explicit Divisor(uint32_t by = 1) : d(by), m(1), s(0) {
+        while ((1ull << s) < by) ++s;
+        m = (uint32_t)(((1ull << 32) * ((1ull << s) - by)) / by + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ int operator()(int n) const {
+        return (int)((__umulhi((uint32_t)n, m) + (uint32_t)n) >> s);
+    }
+#endif
+};
+
 struct Pool {
     uint8_t* data;
     int pages, kv_heads;
     int page_blocks;  // page_size / 16
+    Divisor per_page, per_token;  // by page_blocks, by kv_heads
 };
 
 struct LayoutParams {
@@ -75,6 +92,7 @@ struct AttnParams {
     const int32_t *table, *kv_lens, *cu;
     int batch, width;
     int rows, heads, group;  // query rows, query heads, query heads per KV head
+    Divisor per_group;
     int window, num_globals;
     float scale;
     int bf16, out_dtype;

@@ -92,14 +92,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
     if (threadIdx.x == 0) ptx::fence_mbar_init();
     ptx::griddep_launch();
 
-    const long long line = whole_line<C::ROWS, kTile, kThreads>(p, g, scratch);
-    long long per = divide(line + gridDim.x - 1, gridDim.x);
-    if (p.split) per = max(per, (long long)p.min_tiles);
-    long long at = per * blockIdx.x;
-    const long long end = min(at + per, line);
-    if (at >= end) return;
-    Place here = locate<C::ROWS, kTile, kThreads>(p, g, 0, 0, at, scratch, &found);
-    Request r = request_of<C::ROWS, kTile>(p, g, here.b);
+    const Share share = share_of<C::ROWS, kTile, kThreads>(p, g, scratch, &found);
+    if (share.at >= share.end) return;
+    const long long end = share.end;
+    long long at = share.at;
+    Place here = share.here;
+    Request r = here.r;
     // the next slot of the ring to fill, and the next to empty with its phase
     int fill = 0, drain = 0, phase = 0;
     bool ok = true;
@@ -135,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 const int tile = first_tile + kWarps * (i0 + (lane >> 1));
                 const int block = 2 * (span.first + tile) + (lane & 1);
                 if (i0 + (lane >> 1) >= mine || tile >= span.band || block > span.hi / kBlock) return -1;
-                const int page_at = block / p.pool.page_blocks, page = table[page_at];
+                const int page_at = p.pool.per_page(block), page = table[page_at];
                 if ((unsigned)page >= (unsigned)p.pool.pages) return -1;
                 return (page * p.pool.kv_heads + head) * p.pool.page_blocks + block - page_at * p.pool.page_blocks;
             };
@@ -171,10 +169,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     if (k < span.globals) {
                         const int pos = g.at[k], block = pos / kBlock;
                         row = pos % kBlock;
-                        const int page = table[block / p.pool.page_blocks];
+                        const int page = table[p.pool.per_page(block)];
                         if ((unsigned)page < (unsigned)p.pool.pages)
                             src = p.pool.data + (((long long)page * p.pool.kv_heads + head) * p.pool.page_blocks +
-                                                 block % p.pool.page_blocks) * block_bytes(D);
+                                                 block - p.pool.per_page(block) * p.pool.page_blocks) * block_bytes(D);
                     }
                     const uint32_t have = __ballot_sync(kAll, src != nullptr);
                     uint8_t* to = dst + (lane >> 4) * block_bytes(D);
@@ -212,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 const int row = q_tile * C::ROWS + 8 * nt + gq;
                 uint32_t raw[D / 8];
                 if (row < r.rows) {
-                    const int token = row / p.group, of = row - token * p.group;
+                    const int token = p.per_group(row), of = row - token * p.group;
                     const uint4* src = reinterpret_cast<const uint4*>(
                         static_cast<const uint16_t*>(p.q) + (r.q0 + token) * p.q_token +
                         (long long)(head * p.group + of) * p.q_head + t * (D / 4));
@@ -265,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 for (int e = 0; e < 2; ++e) {
                     q_scale[nt][e] = __shfl_sync(kAll, mult, 4 * (2 * t + e));
                     const int col = q_tile * C::ROWS + 8 * nt + 2 * t + e;
-                    const int pos = col < r.rows ? r.len - r.rows / p.group + col / p.group : -1;
+                    const int pos = col < r.rows ? r.len - p.per_group(r.rows) + p.per_group(col) : -1;
                     row_hi[nt][e] = pos;
                     row_lo[nt][e] = max(0, pos - p.window);
                     if (p.num_globals > 0 && span.first == 0) {
@@ -512,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
             }
             __syncthreads();
             const bool whole = t0 == 0 && t1 == r.tiles;
-            const int part = (int)(2 * blockIdx.x) + (at != per * blockIdx.x);
+            const int part = (int)(2 * blockIdx.x) + (at != share.at);
             for (int x = threadIdx.x; x < C::ROWS * (D / 4); x += kThreads) {
                 const int row = x / (D / 4), d = 4 * (x - row * (D / 4));
                 const int of = q_tile * C::ROWS + row;
@@ -531,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     v[0] += f * a.x, v[1] += f * a.y, v[2] += f * a.z, v[3] += f * a.w;
                 }
                 if (whole) {
-                    const int token = of / p.group, h = head * p.group + of - token * p.group;
+                    const int token = p.per_group(of), h = head * p.group + of - token * p.group;
                     const float inv = l == 0.f ? 0.f : 1.f / l;
                     if (l == 0.f) v[0] = v[1] = v[2] = v[3] = 0.f;
                     v[0] *= inv, v[1] *= inv, v[2] *= inv, v[3] *= inv;
@@ -552,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         if (at >= end) break;
         if (at >= here.start + line_of(p, r)) {
             here = locate<C::ROWS, kTile, kThreads>(p, g, here.b + 1, here.start + line_of(p, r), at, scratch, &found);
-            r = request_of<C::ROWS, kTile>(p, g, here.b);
+            r = here.r;
         }
     }
 }
@@ -579,7 +577,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
         const long long all = block_scan<THREADS>(mine, scratch, &before);
         const long long all_items = block_scan<THREADS>(count, scratch, &items_before);
         if (items + items_before <= id && id < items + items_before + count) {
-            found = {b0 + (int)threadIdx.x, line + before};
+            found = {b0 + (int)threadIdx.x, line + before, r};
             found_item = (int)(id - items - items_before);
         }
         line += all;
@@ -587,7 +585,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     }
     __syncthreads();
     if (found.b < 0) return;
-    const Request r = request_of<ROWS, TILE>(p, g, found.b);
+    const Request r = found.r;
     const int head = found_item / r.q_tiles, q_tile = found_item - head * r.q_tiles, of = q_tile * ROWS + row;
     if (of >= r.rows) return;
     const long long per = max(divide(line + p.ctas - 1, p.ctas), (long long)p.min_tiles);
@@ -634,7 +632,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] * inv;
-    const int token = of / p.group, h = head * p.group + of - token * p.group;
+    const int token = p.per_group(of), h = head * p.group + of - token * p.group;
     store_out(p, p.out_dtype, ((long long)(r.q0 + token) * p.heads + h) * D + 4 * threadIdx.x, v);
     if (p.lse != nullptr && threadIdx.x == 0)
         p.lse[(long long)h * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;

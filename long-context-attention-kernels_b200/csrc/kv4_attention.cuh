@@ -99,10 +99,10 @@ struct Span {
 template <int ROWS, int TILE>
 __device__ __forceinline__ Span span_of(const AttnParams& p, const Globals& g, const Request& r, int q_tile) {
     Span s;
-    const int n = r.rows / p.group;
+    const int n = p.per_group(r.rows);
     const int from = q_tile * ROWS, to = min(from + ROWS, r.rows) - 1;
-    s.lo = r.len - n + from / p.group;
-    s.hi = r.len - n + to / p.group;
+    s.lo = r.len - n + p.per_group(from);
+    s.hi = r.len - n + p.per_group(to);
     if (s.hi < 0) return {0, 0, 0, 0, s.lo, s.hi};
     int lo = max(0, s.lo - p.window);
     s.globals = 0;
@@ -180,8 +180,9 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch,
 }
 
 struct Place {
-    int b;             // request
+    int b;             // request; p.batch: none
     long long start;   // its first tile on the line
+    Request r;
 };
 
 // The request that holds position `at` of the line, searched from `from` on, whose own part of the
@@ -190,11 +191,13 @@ template <int ROWS, int TILE, int THREADS>
 __device__ __forceinline__ Place locate(const AttnParams& p, const Globals& g, int from, long long start, long long at,
                                         long long* scratch, Place* found) {
     for (int b0 = from; b0 < p.batch; b0 += THREADS) {
-        const long long mine = line_of(p, request_of<ROWS, TILE>(p, g, b0 + (int)threadIdx.x));
+        const Request mine = request_of<ROWS, TILE>(p, g, b0 + (int)threadIdx.x);
+        const long long line = line_of(p, mine);
         long long before;
-        const long long all = block_scan<THREADS>(mine, scratch, &before);
+        const long long all = block_scan<THREADS>(line, scratch, &before);
         if (at < start + all) {
-            if (start + before <= at && at < start + before + mine) *found = {b0 + (int)threadIdx.x, start + before};
+            if (start + before <= at && at < start + before + line)
+                *found = {b0 + (int)threadIdx.x, start + before, mine};
             __syncthreads();
             const Place r = *found;
             __syncthreads();
@@ -202,14 +205,41 @@ __device__ __forceinline__ Place locate(const AttnParams& p, const Globals& g, i
         }
         start += all;
     }
-    return {p.batch, start};
+    return {p.batch, start, {0, 0, 0, 0, 1}};
 }
 
+// A CTA's share [at, end) of the line, and where it begins.  One pass over the lengths where a
+// thread holds one request, else one for the total and one for the place.
+struct Share {
+    long long per, at, end;
+    Place here;
+};
+
 template <int ROWS, int TILE, int THREADS>
-__device__ __forceinline__ long long whole_line(const AttnParams& p, const Globals& g, long long* scratch) {
-    long long sum = 0, before;
-    for (int b = threadIdx.x; b < p.batch; b += THREADS) sum += line_of(p, request_of<ROWS, TILE>(p, g, b));
-    return block_scan<THREADS>(sum, scratch, &before);
+__device__ __forceinline__ Share share_of(const AttnParams& p, const Globals& g, long long* scratch, Place* found) {
+    Share s;
+    Request mine = {0, 0, 0, 0, 0};
+    long long line = 0, before;
+    for (int b = threadIdx.x; b < p.batch; b += THREADS) {
+        mine = request_of<ROWS, TILE>(p, g, b);
+        line += line_of(p, mine);
+    }
+    const long long all = block_scan<THREADS>(line, scratch, &before);
+    s.per = divide(all + gridDim.x - 1, gridDim.x);
+    if (p.split) s.per = max(s.per, (long long)p.min_tiles);
+    s.at = s.per * blockIdx.x;
+    s.end = min(s.at + s.per, all);
+    s.here.b = p.batch;
+    if (s.at >= s.end) return s;
+    if (p.batch <= THREADS) {
+        if (before <= s.at && s.at < before + line) *found = {(int)threadIdx.x, before, mine};
+        __syncthreads();
+        s.here = *found;
+        __syncthreads();
+    } else {
+        s.here = locate<ROWS, TILE, THREADS>(p, g, 0, 0, s.at, scratch, found);
+    }
+    return s;
 }
 
 // Dynamic shared memory beyond 48 KB for a kernel, asked for once per device.

@@ -5,7 +5,7 @@
 
 #include <algorithm>
 
-#include "kv4.h"
+#include "kv4_attention.cuh"
 
 namespace lca {
 namespace kv4 {
@@ -205,17 +205,6 @@ struct Half<__nv_bfloat16> {
     }
 };
 
-__device__ __forceinline__ uint8_t* block_of(const Pool& pool, int d, int slot, int head, int* row) {
-    const int block = slot / kBlock;
-    *row = slot - block * kBlock;
-    const int page = block / pool.page_blocks, in = block - page * pool.page_blocks;
-    return pool.data + (((long long)page * pool.kv_heads + head) * pool.page_blocks + in) * block_bytes(d);
-}
-
-__device__ __forceinline__ bool slot_ok(const Pool& pool, int slot) {
-    return slot >= 0 && slot / (kBlock * pool.page_blocks) < pool.pages;
-}
-
 // Quantises one row held by LANES lanes, 8 elements (four pairs) a lane: the lane's word of codes,
 // and the row's word of scale and zero point.  With lo = min(row, 0) and hi = max(row, 0): scale =
 // hi/15 - lo/15 (products with fp32 1/15, so that opposite extremes of bf16 do not overflow) with
@@ -245,15 +234,18 @@ __device__ __forceinline__ void quantise(const uint32_t (&x)[4], uint32_t* codes
     const float inv = normal ? __frcp_rn(scale) : 0.f;
     const float zm = normal ? __fadd_rn(__fmul_rn(minus_lo, inv), kMagic) : kMagic;  // kMagic + z
     const float z = __fsub_rn(zm, kMagic);
-    uint32_t w = 0, ones = 0;
+    const uint64_t magic2 = ptx::f2_pack(kMagic, kMagic), z2 = ptx::f2_pack(z, z);
+    uint32_t w = 0;
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-        const float v = (i & 1) ? H::high(x[i >> 1]) : H::low(x[i >> 1]);
-        const float c = fminf(fmaxf(__fadd_rn(__fadd_rn(__fmul_rn(v, inv), kMagic), z), kMagic), kMagic + 15.f);
-        w = w * 16u + __float_as_uint(c);  // the bits of kMagic are taken off at the end
-        ones = ones * 16u + 1u;
+    for (int i = 3; i >= 0; --i) {
+        // the products one by one: a packed product and sum would be contracted into one operation
+        const uint64_t y = ptx::f2_pack(__fmul_rn(H::low(x[i]), inv), __fmul_rn(H::high(x[i]), inv));
+        const uint64_t c = ptx::f2_add(ptx::f2_add(y, magic2), z2);
+        // never below 0: the least element rounds to -z itself
+        w = w * 16u + __float_as_uint(fminf(ptx::f2_hi(c), kMagic + 15.f));
+        w = w * 16u + __float_as_uint(fminf(ptx::f2_lo(c), kMagic + 15.f));
     }
-    *codes = normal ? w - ones * 0x4b400000u : 0u;
+    *codes = normal ? w - 0x11111111u * 0x4b400000u : 0u;  // less the bits of kMagic in each
     *word = normal ? __float_as_uint(scale) | (__float_as_uint(zm) & 15u) : (finite ? 0u : 0x7fc00000u);
 }
 
@@ -261,19 +253,24 @@ constexpr int kRowThreads = 256;
 constexpr int kRowItems = 2;  // (token, head) pairs of a group of lanes, whose loads are in flight together
 
 struct Item {
-    int token, head, slot;
-    bool keep;
+    int token, head, row;
+    uint8_t* block;  // NULL: a slot outside the pool
 };
 
-// Pair number `item` of the call (32-bit division where the count allows: a 64-bit one costs more
-// than the rest of the row).
+// Pair number `item` of the call.
+template <int D>
 __device__ __forceinline__ Item item_of(const RowsParams& p, long long item, long long items) {
-    Item r = {0, 0, -1, false};
+    Item r = {0, 0, 0, nullptr};
     if (item >= items) return r;
-    r.token = items <= 0xffffffffll ? (int)((uint32_t)item / (uint32_t)p.pool.kv_heads) : (int)(item / p.pool.kv_heads);
+    r.token = items <= 0x7fffffffll ? p.pool.per_token((int)item) : (int)(item / p.pool.kv_heads);
     r.head = (int)(item - (long long)r.token * p.pool.kv_heads);
-    r.slot = p.slots[r.token];
-    r.keep = slot_ok(p.pool, r.slot);
+    const int slot = p.slots[r.token];
+    if (slot < 0) return r;
+    const int block = slot / kBlock, page = p.pool.per_page(block);
+    r.row = slot % kBlock;
+    if (page < p.pool.pages)
+        r.block = p.pool.data + (long long)((page * p.pool.kv_heads + r.head) * p.pool.page_blocks +
+                                            block - page * p.pool.page_blocks) * block_bytes(D);
     return r;
 }
 
@@ -289,13 +286,13 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
     Item at[kRowItems];
     uint32_t k[kRowItems][4], v[kRowItems][4];
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) at[j] = item_of(p, first + j * GROUPS, items);
+    for (int j = 0; j < kRowItems; ++j) at[j] = item_of<D>(p, first + j * GROUPS, items);
 #pragma unroll
     for (int j = 0; j < kRowItems; ++j) {
         const T* kp = static_cast<const T*>(p.k) + at[j].token * p.k_token + at[j].head * p.k_head + lane * 8;
         const T* vp = static_cast<const T*>(p.v) + at[j].token * p.v_token + at[j].head * p.v_head + lane * 8;
         uint4 a = make_uint4(0, 0, 0, 0), b = a;
-        if (at[j].keep) {
+        if (at[j].block != nullptr) {
             if (VECTOR) {
                 a = *reinterpret_cast<const uint4*>(kp);
                 b = *reinterpret_cast<const uint4*>(vp);
@@ -313,9 +310,9 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
         uint32_t k_codes, k_word, v_codes, v_word;  // every lane takes part in the shuffles
         quantise<LANES, T>(k[j], &k_codes, &k_word);
         quantise<LANES, T>(v[j], &v_codes, &v_word);
-        if (!at[j].keep) continue;
-        int row;
-        uint8_t* block = block_of(p.pool, D, at[j].slot, at[j].head, &row);
+        if (at[j].block == nullptr) continue;
+        const int row = at[j].row;
+        uint8_t* block = at[j].block;
         reinterpret_cast<uint32_t*>(block + row * row_bytes(D))[lane] = k_codes;
         reinterpret_cast<uint32_t*>(block + v_codes_at(D) + row * row_bytes(D))[lane] = v_codes;
         if (lane == 0) *reinterpret_cast<uint32_t*>(block + k_words_at(D) + 4 * row) = k_word;
@@ -345,12 +342,17 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* to, const f
     *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(h);
 }
 
-// The eight values of a word of codes: 1.5 * 2^23 + code is the code in the low bits of that number.
+// The eight values of a word of codes: c - z exactly in fp16 pairs, then one fp32 product each.
 __device__ __forceinline__ void values_of(uint32_t codes, uint32_t word, float (&x)[8]) {
-    const float scale = __uint_as_float(word & ~15u), less = __uint_as_float(0x4b400000u | (word & 15u));
+    const float scale = __uint_as_float(word & ~15u);
+    const Zero z = zero_pair((word & 15u) * 0x10001u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = __fmul_rn(scale, __fsub_rn(__uint_as_float(((codes >> (4 * i)) & 15u) | 0x4b400000u), less));
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t pair = codes_pair(codes, i, z);  // elements i and i + 4
+        const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+        x[i] = __fmul_rn(scale, c.x);
+        x[i + 4] = __fmul_rn(scale, c.y);
+    }
 }
 
 // The rows of `slots` as values, rounded once to the output's type; a slot outside the pool reads
@@ -364,12 +366,12 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read(const RowsParams p) {
     Item at[kRowItems];
     uint32_t k[kRowItems] = {}, v[kRowItems] = {}, kw[kRowItems] = {}, vw[kRowItems] = {};
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) at[j] = item_of(p, first + j * GROUPS, items);
+    for (int j = 0; j < kRowItems; ++j) at[j] = item_of<D>(p, first + j * GROUPS, items);
 #pragma unroll
     for (int j = 0; j < kRowItems; ++j) {
-        if (!at[j].keep) continue;
-        int row;
-        const uint8_t* block = block_of(p.pool, D, at[j].slot, at[j].head, &row);
+        if (at[j].block == nullptr) continue;
+        const int row = at[j].row;
+        const uint8_t* block = at[j].block;
         k[j] = reinterpret_cast<const uint32_t*>(block + row * row_bytes(D))[lane];
         v[j] = reinterpret_cast<const uint32_t*>(block + v_codes_at(D) + row * row_bytes(D))[lane];
         kw[j] = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row);

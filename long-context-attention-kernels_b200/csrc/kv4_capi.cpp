@@ -76,6 +76,8 @@ int check_pool(lca::kv4::Pool* pool, const void* data, int64_t pages, int64_t kv
     pool->pages = (int)pages;
     pool->kv_heads = (int)kv_heads;
     pool->page_blocks = (int)(page_size / lca::kv4::kBlock);
+    pool->per_page = lca::kv4::Divisor((uint32_t)pool->page_blocks);
+    pool->per_token = lca::kv4::Divisor((uint32_t)kv_heads);
     return LCA_OK;
 }
 
@@ -305,6 +307,7 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     p.rows = (int)num_rows;
     p.heads = (int)heads;
     p.group = (int)(heads / kv_heads);
+    p.per_group = lca::kv4::Divisor((uint32_t)p.group);
     p.window = (int)std::min<int64_t>(window_size, (int64_t)1 << 30);
     p.num_globals = n;
     p.scale = scale;

@@ -1,6 +1,7 @@
 // kv4_chunk.cu -- attention of many new tokens a request (a prompt's chunk) over the paged 4-bit KV
 // cache, on tcgen05.  Mathematics as in kv4_attention.cu: products over the exact integers c - z,
-// scales outside them in fp32.
+// scales outside them in fp32.  Q enters as it is, in its own type, which K then shares (the integers
+// are exact in bf16 too); V and the weights are fp16.
 //
 // A CTA takes 256 query rows (tokens x the heads of a group) of one KV head at a time, as two
 // tiles A and B of 128 rows, over tiles of 64 keys:
@@ -9,12 +10,13 @@
 //   MMA warp (1 lane)  S = Q K^T into one of two buffers in TMEM, then O += W V of the tile before, W
 //                      read from TMEM where it lies over its S
 //   softmax warps (8)  a thread per row: scores times scales, the running maximum, weights to fp16
+//   query warps (3)    the next item's query rows into the other of two buffers
 // Barriers with one phase per tile of one parity (n & 1), so that a wait for tile n - 1 cannot be
 // answered by a phase before or after it.
 // A tile of codes is unpacked once for 256 rows, and the products of one tile run under
-// the softmax of the other.  K, V and Q are held with the elements of each group of 8 in the order
-// 0 4 1 5 2 6 3 7, in which the codes come out of a word; Q is stored so too, and the output put
-// back in order as it is read.
+// the softmax of the other.  V is held with the elements of each group of 8 in the order 0 4 1 5 2 6
+// 3 7, in which the codes come out of a word most cheaply; the output is put back in order as it
+// is read.
 #include <algorithm>
 
 #include "kv4_attention.cuh"
@@ -25,9 +27,9 @@ namespace {
 
 constexpr int kHalfRows = 128;            // rows of a tile A or B
 constexpr int kKeys = kChunkKeys;         // keys of a tile
-constexpr int kRing = 3;                  // unpacked tiles
-constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4, kMmaWarp = kSoftmaxWarps + kUnpackWarps;
-constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, products
+constexpr int kRing = 2;                  // unpacked tiles
+constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4, kMmaWarp = kSoftmaxWarps + kUnpackWarps, kQueryWarps = 3;
+constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, products and queries
 // registers a thread of each: 2 * 176 + 96 + 64 = 4 * 128, what the block is launched with
 constexpr int kSoftmaxRegs = 176, kUnpackRegs = 96, kMmaRegs = 64;
 constexpr uint32_t kTmemCols = 512;
@@ -36,9 +38,9 @@ template <int D>
 struct Cfg {
     static constexpr int Q_PANEL = kHalfRows * 128, KV_PANEL = kKeys * 128;  // 64 elements of every row
     static constexpr int Q_BYTES = D / 64 * Q_PANEL, KV_BYTES = D / 64 * KV_PANEL;
-    static constexpr int OFF_KV = 2 * Q_BYTES;
+    static constexpr int OFF_KV = 4 * Q_BYTES;  // two buffers of A and B
     static constexpr int OFF_TABLE = OFF_KV + kRing * 2 * KV_BYTES;  // [kRing][3][kKeys] sk, log2 sv, sv
-    static constexpr int OFF_HAVE = OFF_TABLE + kRing * 3 * kKeys * 4;  // [kRing][4] keys that are there
+    static constexpr int OFF_HAVE = OFF_TABLE + kRing * 3 * kKeys * 4;  // [kRing][4] keys that are there, and global ones
     static constexpr int OFF_BAR = OFF_HAVE + kRing * 16;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;  // and the alignment of the panels
 };
@@ -55,7 +57,8 @@ template <int ROWS, int TILE>
 __device__ __forceinline__ Place locate_warp(const AttnParams& p, const Globals& g, int from, long long start, long long at) {
     const int lane = threadIdx.x & 31;
     for (int b0 = from; b0 < p.batch; b0 += 32) {
-        const long long mine = line_of(p, request_of<ROWS, TILE>(p, g, b0 + lane));
+        const Request one = request_of<ROWS, TILE>(p, g, b0 + lane);
+        const long long mine = line_of(p, one);
         long long inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -65,11 +68,17 @@ __device__ __forceinline__ Place locate_warp(const AttnParams& p, const Globals&
         const uint32_t hit = __ballot_sync(kAll, at < start + inc);
         if (hit) {
             const int who = __ffs(hit) - 1;
-            return {b0 + who, __shfl_sync(kAll, start + inc - mine, who)};
+            Place r = {b0 + who, __shfl_sync(kAll, start + inc - mine, who), {}};
+            r.r.q0 = __shfl_sync(kAll, one.q0, who);
+            r.r.len = __shfl_sync(kAll, one.len, who);
+            r.r.rows = __shfl_sync(kAll, one.rows, who);
+            r.r.q_tiles = __shfl_sync(kAll, one.q_tiles, who);
+            r.r.tiles = __shfl_sync(kAll, one.tiles, who);
+            return r;
         }
         start += __shfl_sync(kAll, inc, 31);
     }
-    return {p.batch, start};
+    return {p.batch, start, {0, 0, 0, 0, 1}};
 }
 
 // The next item (or part of one) of the walk, or false.
@@ -78,7 +87,7 @@ __device__ __forceinline__ bool next_item(const AttnParams& p, const Globals& g,
         const long long stop = w.here.start + line_of(p, w.r);
         if (w.at >= stop) {
             w.here = locate_warp<kChunkRows, kKeys>(p, g, w.here.b + 1, stop, w.at);
-            w.r = request_of<kChunkRows, kKeys>(p, g, w.here.b);
+            w.r = w.here.r;
             continue;
         }
         const long long in = w.at - w.here.start;
@@ -94,6 +103,30 @@ __device__ __forceinline__ bool next_item(const AttnParams& p, const Globals& g,
         return true;
     }
     return false;
+}
+
+// Codes of a word minus the zero point, as pairs in their own order (0 1, 2 3, 4 5, 6 7), in fp16 or bf16:
+// 0x6400 | c is 1024 + c in the one, 0x4300 | c is 128 + c in the other.
+template <bool BF16>
+__device__ __forceinline__ uint4 codes_in_order(uint32_t w, uint32_t zero) {  // zero: 0x10001 times the zero point
+    const uint32_t a = __byte_perm(w, w << 12, 0x7610), b = __byte_perm(w, w >> 4, 0x7632);
+    const uint32_t magic = BF16 ? 0x43004300u : 0x64006400u, z = magic + zero;
+    auto pair = [&](uint32_t v) {
+        const uint32_t x = and_or(v, 0x000f000fu, magic);
+        uint32_t y;
+        if (BF16)
+            asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(z));
+        else
+            y = hsub2(x, z);
+        return y;
+    };
+    return make_uint4(pair(a), pair(a >> 8), pair(b), pair(b >> 8));
+}
+
+// 16 bytes to shared memory; `valid` false writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0)
+                 : "memory");
 }
 
 // One row of 64 keys' bits below key index n.
@@ -112,7 +145,7 @@ __device__ __forceinline__ void read_out(float (&x)[32], uint32_t taddr, bool so
     for (int j = 0; j < 32; ++j) x[j] = some ? x[j] * inv : 0.f;
 }
 
-template <int D, bool SPLIT_W>
+template <int D, bool BF16, bool SPLIT_W>
 __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, const __grid_constant__ Globals g) {
     using C = Cfg<D>;
     extern __shared__ uint8_t raw_smem[];
@@ -120,8 +153,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
     volatile uint32_t* have_at = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_HAVE);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-    uint64_t *q_full = bars, *kv_full = bars + 2, *kv_free = kv_full + kRing, *s_full = kv_free + kRing, *p_full = s_full + 4,
-             *pv_done = p_full + 4, *drain = pv_done + 4;
+    uint64_t *q_full = bars, *q_free = bars + 2, *kv_full = bars + 4, *kv_free = kv_full + kRing, *s_full = kv_free + kRing,
+             *p_full = s_full + 4, *pv_done = p_full + 4, *drain = pv_done + 4;
     __shared__ long long scratch[kThreads / 32];
     __shared__ Place found;
     __shared__ uint32_t s_tmem;
@@ -129,7 +162,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) ptx::mbar_init(&q_full[i], 4);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&q_full[i], kQueryWarps);
+            ptx::mbar_init(&q_free[i], kSoftmaxWarps);
+        }
         for (int i = 0; i < kRing; ++i) {
             ptx::mbar_init(&kv_full[i], kUnpackWarps);
             ptx::mbar_init(&kv_free[i], 1);
@@ -146,14 +182,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     ptx::griddep_launch();
     Walk walk;
     {
-        const long long line = whole_line<kChunkRows, kKeys, kThreads>(p, g, scratch);
-        long long per = divide(line + gridDim.x - 1, gridDim.x);
-        if (p.split) per = max(per, (long long)p.min_tiles);
-        walk.at = per * blockIdx.x;
-        walk.end = min(walk.at + per, line);
-        if (walk.at >= walk.end) return;
-        walk.here = locate<kChunkRows, kKeys, kThreads>(p, g, 0, 0, walk.at, scratch, &found);
-        walk.r = request_of<kChunkRows, kKeys>(p, g, walk.here.b);
+        const Share share = share_of<kChunkRows, kKeys, kThreads>(p, g, scratch, &found);
+        if (share.at >= share.end) return;
+        walk.at = share.at;
+        walk.end = share.end;
+        walk.here = share.here;
+        walk.r = share.here.r;
     }
     const long long line_at = walk.at;
     if (warp == kMmaWarp) {
@@ -186,14 +220,41 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     } else {
         ptx::setmaxnreg_inc<kSoftmaxRegs>();
     }
+    int items = 0;  // items with tiles since the start: query buffer items & 1, the same in every role
     if (warp > kMmaWarp) {
-        // the rest of the products' warpgroup has nothing to do
+        // ============================================================ queries
+        // D / 8 lanes a row, 16 bytes each, copied asynchronously into the swizzled tile.
+        constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+        const int piece = lane % LANES, sub = lane / LANES;
+        while (ok && next_item(p, g, walk)) {
+            Span span;
+            const int tiles = tiles_of(span);
+            walk.at += walk.t1 - walk.t0;
+            if (tiles == 0) continue;
+            const int buf = items & 1;
+            if (items >= 2) wait_all(&q_free[buf], items / 2 - 1);
+            if (!ok) break;
+            uint8_t* to = smem + 2 * buf * C::Q_BYTES + (piece >> 3) * C::Q_PANEL;
+            const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)walk.r.q0 * p.q_token +
+                                  (long long)walk.head * p.group * p.q_head + 8 * piece;
+#pragma unroll 4
+            for (int row = (warp - kMmaWarp - 1) * AT_ONCE + sub; row < kChunkRows; row += kQueryWarps * AT_ONCE) {
+                const int x = walk.q_tile * kChunkRows + row, tok = p.per_group(x), in = row & (kHalfRows - 1);
+                const bool there = x < walk.r.rows;
+                cp_async_16(to + (row / kHalfRows) * C::Q_BYTES + in * 128 + (((piece & 7) ^ (in & 7)) << 4),
+                            there ? src + tok * p.q_token + (x - tok * p.group) * p.q_head : p.q, there);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&q_full[buf]);
+            ++items;
+        }
     } else if (warp == kMmaWarp) {
         // ============================================================ products
         const uint32_t hi = ptx::smem_desc_sw128_hi(1024);
-        const uint32_t idesc_s = ptx::idesc_f16(false, kHalfRows, kKeys, false);
+        const uint32_t idesc_s = ptx::idesc_f16(BF16, kHalfRows, kKeys, false);
         const uint32_t idesc_o = ptx::idesc_f16(false, kHalfRows, D, true);
-        int items = 0;
         auto accumulate = [&](int m, bool first) {  // O += W V of tile m
             const uint32_t v = ptx::smem_u32(smem + C::OFF_KV + (m % kRing) * 2 * C::KV_BYTES + C::KV_BYTES);
             const uint32_t v_lo = ptx::smem_desc_sw128_lo(v, C::KV_PANEL);
@@ -219,8 +280,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             walk.at += walk.t1 - walk.t0;
             if (tiles == 0) continue;
             if (lane == 0) {
-                wait(&q_full[0], items);
-                wait(&q_full[1], items);
+                const uint8_t* q_tile = smem + 2 * (items & 1) * C::Q_BYTES;
+                wait(&q_full[items & 1], items >> 1);
                 for (int i = 0; i < tiles && ok; ++i, ++n) {
                     wait(&kv_full[n % kRing], n / kRing);
                     if (!ok) break;
@@ -229,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                         ptx::smem_desc_sw128_lo(ptx::smem_u32(smem + C::OFF_KV + (n % kRing) * 2 * C::KV_BYTES), 0);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t q_lo = ptx::smem_desc_sw128_lo(ptx::smem_u32(smem + h * C::Q_BYTES), 0);
+                        const uint32_t q_lo = ptx::smem_desc_sw128_lo(ptx::smem_u32(q_tile + h * C::Q_BYTES), 0);
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k)
                             ptx::mma_f16_ss(tmem + 256 * h + 128 + 64 * (n & 1),
@@ -253,6 +314,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     } else if (warp >= kSoftmaxWarps) {
         // ============================================================ unpacking
         const int w = warp - kSoftmaxWarps, row = lane & 15, side = lane >> 4;
+        // the factor of the scores is positive and finite (`factor` of the softmax), so that it leaves the -inf of a
+        // masked one alone: the softmax scale's sign, a zero and a NaN go with the scales of K
+        const float mult = fabsf(p.scale) * kLog2e;
+        const float sign = !(mult < INFINITY) ? NAN : (mult < 1.17549435e-38f ? 0.f : copysignf(1.f, p.scale));
         constexpr int CHUNKS = D / 64;  // 16-byte pieces of a code row per lane
         struct Raw {
             uint4 k[CHUNKS], v[CHUNKS];
@@ -265,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             walk.at += walk.t1 - walk.t0;
             // the pool's block of a position, or -1
             auto block_at = [&](int block) {
-                const int page_at = block / p.pool.page_blocks, page = pages[page_at];
+                const int page_at = p.pool.per_page(block), page = pages[page_at];
                 if ((unsigned)page >= (unsigned)p.pool.pages) return -1;
                 return (page * p.pool.kv_heads + walk.head) * p.pool.page_blocks + block - page_at * p.pool.page_blocks;
             };
@@ -287,7 +352,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                         of = g.at[k] % kBlock;
                     }
                 }
-                x.have = __ballot_sync(kAll, at >= 0) & 0xffffu;
+                // the block's keys that are there, and above them those that are global and in the band
+                uint32_t glob = 0;
+                if (p.num_globals > 0 && t0 + i < band) {
+                    const int key = (span.first + t0 + i) * kKeys + kBlock * w + row, k = lower_bound(g.at, p.num_globals, key);
+                    glob = __ballot_sync(kAll, k < p.num_globals && g.at[k] == key);
+                }
+                x.have = (__ballot_sync(kAll, at >= 0) & 0xffffu) | (glob << 16);
                 const uint8_t* src = p.pool.data + (long long)at * block_bytes(D);
                 if (at >= 0) {
                     x.word = *reinterpret_cast<const uint32_t*>(src + (side ? v_words_at(D) : k_words_at(D)) + 4 * of);
@@ -310,14 +381,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 float* sk = table + slot * 3 * kKeys;
                 const float scale = __uint_as_float(x.word & ~15u);
                 if (side == 0) {
-                    sk[kBlock * w + row] = scale;
+                    sk[kBlock * w + row] = scale * sign;
                 } else {
                     sk[kKeys + kBlock * w + row] = fmaxf(lg2(fabsf(scale)), -100.f);
                     sk[2 * kKeys + kBlock * w + row] = scale;
                 }
                 if (lane == 0) have_at[slot * 4 + w] = x.have;
                 const uint32_t word_k = __shfl_sync(kAll, x.word, row), word_v = __shfl_sync(kAll, x.word, row + 16);
-                const Zero zk = zero_pair((word_k & 15u) * 0x10001u), zv = zero_pair((word_v & 15u) * 0x10001u);
+                const Zero zv = zero_pair((word_v & 15u) * 0x10001u);
                 uint8_t* k_tile = smem + C::OFF_KV + slot * 2 * C::KV_BYTES;
                 const int r = kBlock * w + row;
 #pragma unroll
@@ -329,8 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                         // word 4 (side + 2c) + j of the row: 8 elements, 16 bytes of a panel's row
                         const int word = 4 * (side + 2 * c) + j;
                         uint8_t* to = k_tile + (word >> 3) * C::KV_PANEL + r * 128 + (((word & 7) ^ (r & 7)) << 4);
-                        *reinterpret_cast<uint4*>(to) = make_uint4(codes_pair(kw[j], 0, zk), codes_pair(kw[j], 1, zk),
-                                                                   codes_pair(kw[j], 2, zk), codes_pair(kw[j], 3, zk));
+                        *reinterpret_cast<uint4*>(to) = codes_in_order<BF16>(kw[j], (word_k & 15u) * 0x10001u);
                         *reinterpret_cast<uint4*>(to + C::KV_BYTES) =
                             make_uint4(codes_pair(vw[j], 0, zv), codes_pair(vw[j], 1, zv), codes_pair(vw[j], 2, zv),
                                        codes_pair(vw[j], 3, zv));
@@ -355,6 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     } else {
         // ============================================================ softmax
         const int h = warp >> 2, in_half = 32 * (warp & 3) + lane;
+        const float mult = fabsf(p.scale) * kLog2e, factor = mult >= 1.17549435e-38f && mult < INFINITY ? mult : 1.f;
+        const uint64_t factor2 = ptx::f2_pack(factor, factor);
         const uint32_t mine = tmem + 256 * h + ((uint32_t)(32 * (warp & 3)) << 16);
         while (ok && next_item(p, g, walk)) {
             Span span;
@@ -362,69 +434,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             const Request& r = walk.r;
             const int of = walk.q_tile * kChunkRows + h * kHalfRows + in_half;
             const bool valid = of < r.rows;
-            const int token = of / p.group, head = walk.head * p.group + of - token * p.group;
-            const int pos = valid ? r.len - r.rows / p.group + token : -1;
+            const int token = p.per_group(of), head = walk.head * p.group + of - token * p.group;
+            const int pos = valid ? r.len - p.per_group(r.rows) + token : -1;
             int row_lo = max(0, pos - p.window);
-            float factor = 1.f, top = -INFINITY;
+            float top = -INFINITY;
+            bool finite = true, any = false;  // the row of q; whether it sees a key
             uint64_t sum2 = ptx::f2_pack(0.f, 0.f);
             if (tiles > 0) {
                 if (p.num_globals > 0 && span.first == 0 && valid) {
                     const int k = lower_bound(g.at, p.num_globals, pos);
                     if (k < p.num_globals && g.at[k] == pos) row_lo = 0;
                 }
-                // ---- the warp's 32 query rows, D / 8 lanes a row (a thread per row would touch 32 lines an
-                // instruction).  As in kv4_attention.cu: fp16 as it is, bf16 moved by a power of two, the
-                // scale's sign in the row, a factor that is positive and finite.
-                constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
-                const int piece = lane % LANES, sub = lane / LANES;
-                const int first_of = walk.q_tile * kChunkRows + h * kHalfRows + 32 * (warp & 3);
-                uint4 raw[LANES];
+                wait_all(&q_full[items & 1], items >> 1);
+                const uint8_t* q_row = smem + (2 * (items & 1) + h) * C::Q_BYTES + in_half * 128;
+                uint32_t most = 0;
 #pragma unroll
-                for (int i = 0; i < LANES; ++i) {
-                    const int x = first_of + AT_ONCE * i + sub, tok = x / p.group;
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (x < r.rows)
-                        raw[i] = *reinterpret_cast<const uint4*>(
-                            static_cast<const uint16_t*>(p.q) + (long long)(r.q0 + tok) * p.q_token +
-                            (long long)(walk.head * p.group + x - tok * p.group) * p.q_head + 8 * piece);
+                for (int i = 0; i < D / 8; ++i) {  // in any order of the row's pieces
+                    const uint4 v = *reinterpret_cast<const uint4*>(q_row + (i >> 3) * C::Q_PANEL + (((i ^ in_half) & 7) << 4));
+                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
                 }
-#pragma unroll
-                for (int i = 0; i < LANES; ++i) {
-                    uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w}, most = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) most = max(most, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
-#pragma unroll
-                    for (int o = 1; o < LANES; o *= 2) most = max(most, __shfl_xor_sync(kAll, most, o));
-                    float mult = fabsf(p.scale) * kLog2e, up = 1.f;
-                    if (p.bf16) {
-                        const int e = max((int)(most >> 7) - 127, -100);
-                        up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-                        mult *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
-                    }
-                    const bool finite = most < (p.bf16 ? 0x7f80u : 0x7c00u) && mult < INFINITY;
-                    const bool zero = mult < 1.17549435e-38f;
-                    if (!finite || zero) mult = 1.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (p.bf16)
-                            x[j] = ptx::pack_f16x2(__uint_as_float(x[j] << 16) * up, __uint_as_float(x[j] & 0xffff0000u) * up);
-                        if (p.scale < 0.f) x[j] ^= 0x80008000u;
-                        if (zero) x[j] = 0;
-                        if (!finite) x[j] = 0x7e007e00u;
-                    }
-                    const int to_row = 32 * (warp & 3) + AT_ONCE * i + sub;
-                    *reinterpret_cast<uint4*>(smem + h * C::Q_BYTES + (piece >> 3) * C::Q_PANEL + to_row * 128 +
-                                              (((piece & 7) ^ (to_row & 7)) << 4)) =
-                        make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632),
-                                   __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632));
-                    const float of_row = __shfl_sync(kAll, mult, (lane % AT_ONCE) * LANES);
-                    if (lane / AT_ONCE == i) factor = of_row;
-                }
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&q_full[h]);
+                finite = max(most & 0xffffu, most >> 16) < (BF16 ? 0x7f80u : 0x7c00u);
             }
-            const uint64_t factor2 = ptx::f2_pack(factor, factor);
 
 #pragma unroll 1
             for (int i = 0; i < tiles; ++i, ++n) {
@@ -457,26 +488,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // ---- visibility
                 const bool in_band = tile < span.band;
                 const int key0 = (span.first + tile) * kKeys;
-                const uint64_t have = (uint64_t)(have_at[slot * 4] | (have_at[slot * 4 + 1] << 16)) |
-                                      ((uint64_t)(have_at[slot * 4 + 2] | (have_at[slot * 4 + 3] << 16)) << 32);
+                const uint32_t h0 = have_at[slot * 4], h1 = have_at[slot * 4 + 1], h2 = have_at[slot * 4 + 2], h3 = have_at[slot * 4 + 3];
+                const uint64_t have = (uint64_t)__byte_perm(h0, h1, 0x5410) | ((uint64_t)__byte_perm(h2, h3, 0x5410) << 32);
                 const bool full = __all_sync(kAll, have == ~0ull && (!valid || !in_band || (row_lo <= key0 && pos >= key0 + kKeys - 1)));
                 uint64_t seen = ~0ull;
-                if (!full) {
-                    uint64_t glob = 0;
-                    if (in_band && p.num_globals > 0) {
-                        uint32_t part[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int key = key0 + 32 * e + lane, k = lower_bound(g.at, p.num_globals, key);
-                            part[e] = __ballot_sync(kAll, k < p.num_globals && g.at[k] == key);
-                        }
-                        glob = part[0] | (uint64_t)part[1] << 32;
-                    }
+                if (full) {
+                    any = true;
+                } else {
+                    const uint64_t glob = (uint64_t)__byte_perm(h0, h1, 0x7632) | ((uint64_t)__byte_perm(h2, h3, 0x7632) << 32);
                     if (in_band)
                         seen = bits_below(pos - key0 + 1) & (~bits_below(row_lo - key0) | glob);
                     else
                         seen = pos >= 0 ? ~0ull : 0ull;
                     seen &= have;
+                    any |= seen != 0;
 #pragma unroll
                     for (int j = 0; j < kKeys / 2; ++j) {
                         const float x = (seen >> (2 * j)) & 1 ? ptx::f2_lo(s[j]) : -INFINITY;
@@ -557,7 +582,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 ptx::tc_fence_after();
             }
             if (!ok) break;
-            const float sum = ptx::f2_lo(sum2) + ptx::f2_hi(sum2);
+            float sum = ptx::f2_lo(sum2) + ptx::f2_hi(sum2);
+            if (any && !finite) sum = NAN;
             const bool whole = walk.t0 == 0 && walk.t1 == r.tiles;
             const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
             const long long part = (long long)(2 * blockIdx.x + (walk.at != line_at)) * kChunkRows + h * kHalfRows + in_half;
@@ -573,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // 16-bit rows go through the warp's own rows of the query tile, which nothing reads any more,
                 // and leave as whole rows, D / 8 lanes each
                 auto stage = [&](int row, int piece) {
-                    return reinterpret_cast<uint4*>(smem + h * C::Q_BYTES + (piece >> 3) * C::Q_PANEL +
+                    return reinterpret_cast<uint4*>(smem + (2 * (items & 1) + h) * C::Q_BYTES + (piece >> 3) * C::Q_PANEL +
                                                     (32 * (warp & 3) + row) * 128 + (((piece & 7) ^ (row & 7)) << 4));
                 };
 #pragma unroll 1
@@ -596,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 #pragma unroll 4
                 for (int i = 0; i < LANES; ++i) {
                     const int row = AT_ONCE * i + lane / LANES, piece = lane % LANES;
-                    const int x = walk.q_tile * kChunkRows + h * kHalfRows + 32 * (warp & 3) + row, tok = x / p.group;
+                    const int x = walk.q_tile * kChunkRows + h * kHalfRows + 32 * (warp & 3) + row, tok = p.per_group(x);
                     if (x < r.rows)
                         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
                                                   ((long long)(r.q0 + tok) * p.heads + walk.head * p.group + x - tok * p.group) * D +
@@ -621,6 +647,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 }
             }
             ptx::tc_fence_before();  // the next item's products overwrite what was read here
+            if (tiles > 0) {
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(&q_free[items & 1]);
+                ++items;
+            }
             walk.at += walk.t1 - walk.t0;
         }
     }
@@ -632,21 +663,26 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     }
 }
 
-template <int D, bool SPLIT_W>
+template <int D, bool BF16, bool SPLIT_W>
 cudaError_t chunk_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = allow_smem(kv4_chunk<D, SPLIT_W>, Cfg<D>::SMEM, done);
+    cudaError_t e = allow_smem(kv4_chunk<D, BF16, SPLIT_W>, Cfg<D>::SMEM, done);
     if (e != cudaSuccess) return e;
-    kv4_chunk<D, SPLIT_W><<<p.ctas, kThreads, Cfg<D>::SMEM, stream>>>(p, g);
+    kv4_chunk<D, BF16, SPLIT_W><<<p.ctas, kThreads, Cfg<D>::SMEM, stream>>>(p, g);
     return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t chunk_types(const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;
+    if (p.bf16) return split_w ? chunk_of<D, true, true>(p, g, stream) : chunk_of<D, true, false>(p, g, stream);
+    return split_w ? chunk_of<D, false, true>(p, g, stream) : chunk_of<D, false, false>(p, g, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_chunk(int d, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;
-    if (d == 64) return split_w ? chunk_of<64, true>(p, g, stream) : chunk_of<64, false>(p, g, stream);
-    return split_w ? chunk_of<128, true>(p, g, stream) : chunk_of<128, false>(p, g, stream);
+    return d == 64 ? chunk_types<64>(p, g, stream) : chunk_types<128>(p, g, stream);
 }
 
 }  // namespace kv4
