@@ -30,8 +30,8 @@ constexpr int kKeys = kChunkKeys;         // keys of a tile
 constexpr int kRing = 2;                  // unpacked tiles
 constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4, kMmaWarp = kSoftmaxWarps + kUnpackWarps, kQueryWarps = 3;
 constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, products and queries
-// registers a thread of each: 2 * 176 + 96 + 64 = 4 * 128, what the block is launched with
-constexpr int kSoftmaxRegs = 176, kUnpackRegs = 96, kMmaRegs = 64;
+// registers a thread of each: 2 * 184 + 80 + 64 = 4 * 128, what the block is launched with
+constexpr int kSoftmaxRegs = 184, kUnpackRegs = 80, kMmaRegs = 64;
 constexpr uint32_t kTmemCols = 512;
 
 template <int D>
