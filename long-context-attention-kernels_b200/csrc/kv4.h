@@ -109,6 +109,7 @@ struct AttnParams {
 
 struct AttnPlan {
     int tile_rows;  // query rows of an item: 8, 16 or 32 (kv4_attention.cu) or kChunkRows (kv4_chunk.cu)
+    int tile_keys;  // keys of a tile
     int ctas, min_tiles;
     bool split;
     int64_t items;
@@ -122,7 +123,8 @@ cudaError_t launch_read(int d, int out_dtype, const RowsParams& p, cudaStream_t 
 AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t batch, int64_t capacity,
                         int64_t window, int64_t num_globals);
 cudaError_t launch_chunk(int d, const AttnParams& p, const Globals& g, cudaStream_t stream);
-cudaError_t launch_attention(int d, int tile_rows, const AttnParams& p, const Globals& g, cudaStream_t stream);
+cudaError_t launch_attention(int d, int tile_rows, int tile_keys, const AttnParams& p, const Globals& g,
+                             cudaStream_t stream);
 
 }  // namespace kv4
 

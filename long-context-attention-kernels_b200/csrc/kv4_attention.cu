@@ -20,12 +20,10 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = 32;    // keys per tile: two blocks, one warp's step
-constexpr int kStages = 3;   // tiles in flight per warp
-constexpr int kMinTiles = 8; // least tiles of a CTA where items are split
-constexpr int kWholeTiles = 48;  // items of up to this many tiles are not split
+constexpr int kWholeKeys = 1536; // items of up to this many keys are not split
 constexpr int kChunkFrom = 64;   // mean rows a request from which the tcgen05 kernel takes the call
 constexpr int kSms = 148;
+constexpr int kCtas64 = 6;
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -47,22 +45,29 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     return d;
 }
 
-template <int D, int NT>
+// Resident CTAs of the streaming kernel on an SM: what its registers and its ring allow.
+constexpr int ctas_per_sm(int d, int rows, int keys) {
+    return rows == 8 ? (keys == 64 ? 3 : (d == 64 ? kCtas64 : 4)) : (rows == 16 ? 3 : 2);
+}
+
+// KB_: blocks of 16 keys per tile, one warp's step.
+template <int D, int NT, int KB_>
 struct Cfg {
     static constexpr int ROWS = 8 * NT;
-    static constexpr int STAGE = 2 * block_bytes(D);
-    static constexpr int RING = kWarps * kStages * STAGE;
+    static constexpr int KB = KB_, TILE = 16 * KB, STAGES = KB == 2 ? 3 : 2;  // tiles in flight per warp
+    static constexpr int STAGE = KB * block_bytes(D);
+    static constexpr int RING = kWarps * STAGES * STAGE;
     static constexpr int PITCH = D + 4;  // floats of one row in the merge buffer
     static constexpr int MERGE = kWarps * ROWS * (PITCH + 2) * 4;
     static constexpr int MAIN = RING > MERGE ? RING : MERGE;
-    static constexpr int SMEM = MAIN + kWarps * kStages * 12 + 128;
+    static constexpr int SMEM = MAIN + kWarps * STAGES * 16;  // and the ring's barriers and key masks
 };
 
 // Position of slot s of a block in the products: the codes of slots 2t and 2t + 1 (V) and of slots
 // g (K) are then read from shared memory with the fewest conflicts that a plain layout allows.
 __device__ __forceinline__ int slot_row(int s) { return s ^ ((s >> 1) & 1); }
 
-// One warp streams tiles of 32 keys through its own ring of bulk copies and keeps the running
+// One warp streams tiles of 64 (or 32) keys through its own ring of bulk copies and keeps the running
 // softmax of 8 * NT query rows; the four warps of a CTA take the tiles of a segment in turn and
 // merge at its end.  Per tile: scores S^T = K Q^T (keys are the 16 rows of the product, queries
 // its 8 columns), weights, then O^T += V^T P^T.  The score fragment of a thread holds two
@@ -72,27 +77,29 @@ __device__ __forceinline__ int slot_row(int s) { return s ^ ((s >> 1) & 1); }
 // product as fp16 are at most 1 (2^8 between rescalings) whatever the sizes of V; p itself, which the
 // sum l takes, stays within 2^100 of it because log2(sv) is cut at -100.  Rounding: w to fp16
 // (2^-11); with an fp32 output the remainder w - fp16(w) goes through a second product (2^-22).
-template <int D, int NT, bool SPLIT_W>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
+template <int D, int NT, int KB_, bool SPLIT_W>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
     kv4_attention(const AttnParams p, const __grid_constant__ Globals g) {
-    using C = Cfg<D, NT>;
+    using C = Cfg<D, NT, KB_>;
     constexpr int STEPS = D / 16;  // products over d of a score, and 16-element tiles of O
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::MAIN);
-    uint32_t* masks = reinterpret_cast<uint32_t*>(bars + kWarps * kStages);
+    uint64_t* masks = bars + kWarps * C::STAGES;
     __shared__ long long scratch[kWarps];
     __shared__ Place found;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
     const uint32_t pair_order = (t & 1) ? 0x1054u : 0x5410u;
-    uint8_t* ring = smem + warp * kStages * C::STAGE;
-    uint64_t* bar = bars + warp * kStages;
-    volatile uint32_t* mask = masks + warp * kStages;
-    if (threadIdx.x < kWarps * kStages) ptx::mbar_init(&bars[threadIdx.x], 1);
-    if (threadIdx.x == 0) ptx::fence_mbar_init();
+    uint8_t* ring = smem + warp * C::STAGES * C::STAGE;
+    uint64_t* bar = bars + warp * C::STAGES;
+    uint64_t* mask = masks + warp * C::STAGES;  // keys of a tile that are there
+    if (threadIdx.x < kWarps * C::STAGES) {
+        ptx::mbar_init(&bars[threadIdx.x], 1);
+        ptx::fence_mbar_init();
+    }
     ptx::griddep_launch();
 
-    const Share share = share_of<C::ROWS, kTile, kThreads>(p, g, scratch, &found);
+    const Share share = share_of<C::ROWS, C::TILE, kThreads>(p, g, scratch, &found);
     if (share.at >= share.end) return;
     const long long end = share.end;
     long long at = share.at;
@@ -117,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         const bool in_request = item < r.q_tiles * p.pool.kv_heads;
         if (in_request) {
             const int head = item / r.q_tiles, q_tile = item - head * r.q_tiles;
-            Span span = span_of<C::ROWS, kTile>(p, g, r, q_tile);
+            Span span = span_of<C::ROWS, C::TILE>(p, g, r, q_tile);
             span.first = uniform(span.first), span.band = uniform(span.band);
             span.lo = uniform(span.lo), span.hi = uniform(span.hi);
             const int tiles = min(t1, span.band + span.gathered);
@@ -125,81 +132,104 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
             const int32_t* table = p.table + (long long)here.b * p.width;
 
             // ---- loads: tile t0 + warp + 4 i of the item into the ring
-            // Where 16 tiles of this warp lie, two blocks each, a lane per block: index of the block in
-            // the pool (a pool of 2^31 blocks would be 2 TB), -1 where there is none.  Fetched 8 tiles
-            // ahead, so that neither the table's latency nor the divisions are paid per tile.
+            // Where the next tiles of this warp lie, a lane per block: index of the block in the pool (a
+            // pool of 2^31 blocks would be 2 TB), -1 where there is none.  Fetched half of them ahead, so
+            // that neither the table's latency nor the divisions are paid per tile.
+            constexpr int KB = C::KB, AHEAD = 32 / KB;
             int where = -1, where_next = -1;
             auto fetch = [&](int i0) {
-                const int tile = first_tile + kWarps * (i0 + (lane >> 1));
-                const int block = 2 * (span.first + tile) + (lane & 1);
-                if (i0 + (lane >> 1) >= mine || tile >= span.band || block > span.hi / kBlock) return -1;
+                const int i = i0 + lane / KB, tile = first_tile + kWarps * i, block = KB * (span.first + tile) + lane % KB;
+                if (i >= mine || tile >= span.band || block > span.hi / kBlock) return -1;
                 const int page_at = p.pool.per_page(block), page = table[page_at];
                 if ((unsigned)page >= (unsigned)p.pool.pages) return -1;
                 return (page * p.pool.kv_heads + head) * p.pool.page_blocks + block - page_at * p.pool.page_blocks;
             };
             auto issue = [&](int i) {
-                if ((i & 15) == 0) {
+                if (i % AHEAD == 0) {
                     where = i == 0 ? fetch(0) : where_next;
-                } else if ((i & 15) == 8) {
-                    where_next = fetch((i & ~15) + 16);
+                } else if (i % AHEAD == AHEAD / 2) {
+                    where_next = fetch(i - AHEAD / 2 + AHEAD);
                 }
                 const int slot = fill;
-                fill = fill + 1 == kStages ? 0 : fill + 1;
+                fill = fill + 1 == C::STAGES ? 0 : fill + 1;
                 uint8_t* dst = ring + slot * C::STAGE;
                 const int tile = first_tile + kWarps * i;
                 if (tile < span.band) {
-                    const int at0 = __shfl_sync(kAll, where, 2 * (i & 15)), at1 = __shfl_sync(kAll, where, 2 * (i & 15) + 1);
+                    int at[KB];
+#pragma unroll
+                    for (int k = 0; k < KB; ++k) at[k] = __shfl_sync(kAll, where, KB * (i % AHEAD) + k);
                     if (lane == 0) {
-                        const uint8_t* src = p.pool.data + (long long)at0 * block_bytes(D);
-                        mask[slot] = (at0 >= 0 ? 0xffffu : 0u) | (at1 >= 0 ? 0xffff0000u : 0u);
-                        ptx::mbar_arrive_expect_tx(&bar[slot], ((at0 >= 0) + (at1 >= 0)) * block_bytes(D));
-                        if (at0 >= 0 && at1 == at0 + 1) {
-                            bulk_load(dst, src, 2 * block_bytes(D), &bar[slot]);
+                        bool run = at[0] >= 0;
+                        uint64_t have = 0;
+                        int count = 0;
+#pragma unroll
+                        for (int k = 0; k < KB; ++k) {
+                            run &= at[k] == at[0] + k;
+                            have |= at[k] >= 0 ? 0xffffull << (16 * k) : 0ull;
+                            count += at[k] >= 0;
+                        }
+                        mask[slot] = have;
+                        ptx::mbar_arrive_expect_tx(&bar[slot], count * block_bytes(D));
+                        if (run) {  // blocks of one page follow one another
+                            bulk_load(dst, p.pool.data + (long long)at[0] * block_bytes(D), C::STAGE, &bar[slot]);
                         } else {
-                            if (at0 >= 0) bulk_load(dst, src, block_bytes(D), &bar[slot]);
-                            if (at1 >= 0)
-                                bulk_load(dst + block_bytes(D), p.pool.data + (long long)at1 * block_bytes(D), block_bytes(D),
-                                          &bar[slot]);
+#pragma unroll
+                            for (int k = 0; k < KB; ++k)
+                                if (at[k] >= 0)
+                                    bulk_load(dst + k * block_bytes(D), p.pool.data + (long long)at[k] * block_bytes(D),
+                                              block_bytes(D), &bar[slot]);
                         }
                     }
-                } else {  // a lane per global token
-                    const int k = (tile - span.band) * kTile + lane;
-                    const uint8_t* src = nullptr;
-                    int row = 0;
-                    if (k < span.globals) {
-                        const int pos = g.at[k], block = pos / kBlock;
-                        row = pos % kBlock;
-                        const int page = table[p.pool.per_page(block)];
-                        if ((unsigned)page < (unsigned)p.pool.pages)
-                            src = p.pool.data + (((long long)page * p.pool.kv_heads + head) * p.pool.page_blocks +
-                                                 block - p.pool.per_page(block) * p.pool.page_blocks) * block_bytes(D);
+                } else {  // gathered global tokens, a lane for every 32nd
+                    const uint8_t* src[KB / 2];
+                    int row[KB / 2];
+                    uint64_t have = 0;
+#pragma unroll
+                    for (int e = 0; e < KB / 2; ++e) {
+                        const int k = (tile - span.band) * C::TILE + 32 * e + lane;
+                        src[e] = nullptr;
+                        row[e] = 0;
+                        if (k < span.globals) {
+                            const int pos = g.at[k], block = pos / kBlock, page_at = p.pool.per_page(block);
+                            row[e] = pos % kBlock;
+                            const int page = table[page_at];
+                            if ((unsigned)page < (unsigned)p.pool.pages)
+                                src[e] = p.pool.data + (long long)((page * p.pool.kv_heads + head) * p.pool.page_blocks + block -
+                                                                   page_at * p.pool.page_blocks) * block_bytes(D);
+                        }
+                        have |= (uint64_t)__ballot_sync(kAll, src[e] != nullptr) << (32 * e);
                     }
-                    const uint32_t have = __ballot_sync(kAll, src != nullptr);
                     uint8_t* to = dst + (lane >> 4) * block_bytes(D);
                     const int to_row = lane & 15;
-                    if (src != nullptr) {
-                        *reinterpret_cast<uint32_t*>(to + k_words_at(D) + 4 * to_row) =
-                            *reinterpret_cast<const uint32_t*>(src + k_words_at(D) + 4 * row);
-                        *reinterpret_cast<uint32_t*>(to + v_words_at(D) + 4 * to_row) =
-                            *reinterpret_cast<const uint32_t*>(src + v_words_at(D) + 4 * row);
-                        ptx::fence_proxy_async_smem();  // a later copy may land on these words
+#pragma unroll
+                    for (int e = 0; e < KB / 2; ++e) {
+                        if (src[e] == nullptr) continue;
+                        uint8_t* words = to + 2 * e * block_bytes(D) + 4 * to_row;
+                        *reinterpret_cast<uint32_t*>(words + k_words_at(D)) =
+                            *reinterpret_cast<const uint32_t*>(src[e] + k_words_at(D) + 4 * row[e]);
+                        *reinterpret_cast<uint32_t*>(words + v_words_at(D)) =
+                            *reinterpret_cast<const uint32_t*>(src[e] + v_words_at(D) + 4 * row[e]);
                     }
+                    ptx::fence_proxy_async_smem();  // a later copy may land on these words
                     if (lane == 0) {
                         mask[slot] = have;
-                        ptx::mbar_arrive_expect_tx(&bar[slot], __popc(have) * D);
+                        ptx::mbar_arrive_expect_tx(&bar[slot], __popcll(have) * D);
                     }
                     __syncwarp();
-                    if (src != nullptr) {
-                        bulk_load(to + to_row * row_bytes(D), src + row * row_bytes(D), row_bytes(D), &bar[slot]);
-                        bulk_load(to + v_codes_at(D) + to_row * row_bytes(D), src + v_codes_at(D) + row * row_bytes(D),
-                                  row_bytes(D), &bar[slot]);
+#pragma unroll
+                    for (int e = 0; e < KB / 2; ++e) {
+                        if (src[e] == nullptr) continue;
+                        uint8_t* codes = to + 2 * e * block_bytes(D) + to_row * row_bytes(D);
+                        bulk_load(codes, src[e] + row[e] * row_bytes(D), row_bytes(D), &bar[slot]);
+                        bulk_load(codes + v_codes_at(D), src[e] + v_codes_at(D) + row[e] * row_bytes(D), row_bytes(D),
+                                  &bar[slot]);
                     }
                 }
                 __syncwarp();
             };
             int issued = 0;
             if (ok)
-                for (; issued < min(mine, kStages); ++issued) issue(issued);
+                for (; issued < min(mine, C::STAGES); ++issued) issue(issued);
 
             // ---- queries: rows of the tile as the second operand, in the order of the K codes
             uint32_t q[NT][STEPS][2];
@@ -288,21 +318,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 if (!ptx::mbar_wait(&bar[slot], phase, nullptr, p.err_word, LCA_DEVERR_TIMEOUT_CACHE,
                                     p.wait_ns))
                     ok = false;
-                drain = drain + 1 == kStages ? 0 : drain + 1;
+                drain = drain + 1 == C::STAGES ? 0 : drain + 1;
                 phase ^= drain == 0;
                 ok = __all_sync(kAll, ok);
                 if (!ok) continue;  // results are invalid; the copies still in flight are waited for
                 const uint8_t* stage = ring + slot * C::STAGE;
                 const int tile = first_tile + kWarps * i;
-                const int key0 = (span.first + tile) * kTile;
-                const uint32_t have = uniform(mask[slot]);
+                const int key0 = (span.first + tile) * C::TILE;
+                const uint64_t have = mask[slot];
                 const int row0 = slot_row(gq);
 
                 // ---- scores
-                float s[2][NT][4];
-                float sk[4], sv[4];
+                float s[KB][NT][4];
+                float sk[2 * KB], sv[2 * KB];
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
+                for (int m = 0; m < KB; ++m) {
                     const uint8_t* block = stage + m * block_bytes(D);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) s[m][nt][0] = s[m][nt][1] = s[m][nt][2] = s[m][nt][3] = 0.f;
@@ -339,19 +369,23 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
 
                 // ---- visibility: nothing to do where the whole tile is visible to every row
                 const bool band = tile < span.band;
-                const bool full = have == kAll && (!band || (key0 + kTile - 1 <= span.lo && key0 >= span.hi - p.window));
+                const bool full = __all_sync(kAll, have == (KB == 4 ? ~0ull : 0xffffffffull)) &&
+                                  (!band || (key0 + C::TILE - 1 <= span.lo && key0 >= span.hi - p.window));
                 uint32_t seen[NT];  // bit c = 4 m + 2 (second row) + column
                 if (!full) {
-                    uint32_t glob = 0;  // global keys of the tile, which rows outside whose band they lie see
+                    uint64_t glob = 0;  // global keys of the tile, which rows outside whose band they lie see
                     if (band && p.num_globals > 0) {
-                        const int k = lower_bound(g.at, p.num_globals, key0 + lane);
-                        glob = __ballot_sync(kAll, k < p.num_globals && g.at[k] == key0 + lane);
+#pragma unroll
+                        for (int e = 0; e < KB / 2; ++e) {
+                            const int key = key0 + 32 * e + lane, k = lower_bound(g.at, p.num_globals, key);
+                            glob |= (uint64_t)__ballot_sync(kAll, k < p.num_globals && g.at[k] == key) << (32 * e);
+                        }
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         seen[nt] = 0;
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
+                        for (int c = 0; c < 4 * KB; ++c) {
                             const int k = 16 * (c >> 2) + 8 * ((c >> 1) & 1) + row0, e = c & 1;
                             const bool there = (have >> k) & 1;
                             const int j = key0 + k;
@@ -363,25 +397,27 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                 }
 
                 // ---- softmax
-                float lam[4];
+                float lam[2 * KB];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) lam[c] = fmaxf(lg2(fabsf(sv[c])), -100.f);
+                for (int c = 0; c < 2 * KB; ++c) lam[c] = fmaxf(lg2(fabsf(sv[c])), -100.f);
                 bool raise = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) s[c >> 2][nt][c & 3] *= sk[c >> 1];
+                    for (int c = 0; c < 4 * KB; ++c) s[c >> 2][nt][c & 3] *= sk[c >> 1];
                     if (!full) {
 #pragma unroll
-                        for (int c = 0; c < 8; ++c)
+                        for (int c = 0; c < 4 * KB; ++c)
                             if (!((seen[nt] >> c) & 1)) s[c >> 2][nt][c & 3] = -INFINITY;
                     }
                 }
                 auto peaks = [&](int nt, int e) {  // of this thread's keys
-                    float m = s[0][nt][e] * q_scale[nt][e] + lam[0];
-                    m = fmaxf(m, s[0][nt][2 + e] * q_scale[nt][e] + lam[1]);
-                    m = fmaxf(m, s[1][nt][e] * q_scale[nt][e] + lam[2]);
-                    return fmaxf(m, s[1][nt][2 + e] * q_scale[nt][e] + lam[3]);
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < KB; ++k)
+                        m = ptx::fmax3(m, s[k][nt][e] * q_scale[nt][e] + lam[2 * k],
+                                       s[k][nt][2 + e] * q_scale[nt][e] + lam[2 * k + 1]);
+                    return m;
                 };
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) raise |= peaks(nt, 0) > top[nt][0] + 8.f || peaks(nt, 1) > top[nt][1] + 8.f;
@@ -406,14 +442,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                         }
                     }
                 }
-                uint32_t w_hi[NT][4], w_lo[NT][4];
+                uint32_t w_hi[NT][2 * KB], w_lo[NT][2 * KB];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float ref0 = top[nt][0] == -INFINITY ? 0.f : top[nt][0];
                     const float ref1 = top[nt][1] == -INFINITY ? 0.f : top[nt][1];
-                    float w[8];
+                    float w[4 * KB];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {  // key row c of this thread, both columns
+                    for (int c = 0; c < 2 * KB; ++c) {  // key row c of this thread, both columns
                         const float* x = &s[c >> 1][nt][2 * (c & 1)];
                         const float p0 = ptx::ex2(x[0] * q_scale[nt][0] - ref0), p1 = ptx::ex2(x[1] * q_scale[nt][1] - ref1);
                         sum[nt][0] += p0;
@@ -423,11 +459,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
                     }
                     if (!full) {  // 0 also where the scale of a key that is not there is not finite
 #pragma unroll
-                        for (int c = 0; c < 8; ++c)
+                        for (int c = 0; c < 4 * KB; ++c)
                             if (!((seen[nt] >> c) & 1)) w[c] = 0.f;
                     }
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 2 * KB; ++c) {
                         const uint32_t hi = ptx::pack_f16x2(w[2 * c], w[2 * c + 1]);
                         w_hi[nt][c] = transpose8(hi);
                         if (SPLIT_W) {
@@ -439,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
 
                 // ---- product with V
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
+                for (int m = 0; m < KB; ++m) {
                     const uint8_t* block = stage + m * block_bytes(D);
                     const int r0 = slot_row(2 * t), r1 = slot_row(2 * t + 1);
                     // r0 and r1 are 2t and 2t + 1, in that order for an even t
@@ -549,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : (NT == 2 ? 3 : 2))
         if (!in_request) at = here.start + line_of(p, r);
         if (at >= end) break;
         if (at >= here.start + line_of(p, r)) {
-            here = locate<C::ROWS, kTile, kThreads>(p, g, here.b + 1, here.start + line_of(p, r), at, scratch, &found);
+            here = locate<C::ROWS, C::TILE, kThreads>(p, g, here.b + 1, here.start + line_of(p, r), at, scratch, &found);
             r = here.r;
         }
     }
@@ -652,26 +688,30 @@ cudaError_t merge_of(const AttnParams& p, const Globals& g, cudaStream_t stream)
     return cudaLaunchKernelEx(&cfg, kv4_attention_merge<D, ROWS, TILE>, p, g);
 }
 
-template <int D, int NT, bool SPLIT_W>
+template <int D, int NT, int KB, bool SPLIT_W>
 cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const int smem = Cfg<D, NT>::SMEM;
+    const int smem = Cfg<D, NT, KB>::SMEM;
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = allow_smem(kv4_attention<D, NT, SPLIT_W>, smem, done);
+    cudaError_t e = allow_smem(kv4_attention<D, NT, KB, SPLIT_W>, smem, done);
     if (e != cudaSuccess) return e;
-    kv4_attention<D, NT, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
+    kv4_attention<D, NT, KB, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
     e = cudaGetLastError();
-    return e != cudaSuccess || !p.split ? e : merge_of<D, 8 * NT, kTile>(p, g, stream);
+    return e != cudaSuccess || !p.split ? e : merge_of<D, 8 * NT, 16 * KB>(p, g, stream);
+}
+
+template <int D, int NT, int KB>
+cudaError_t attention_tiles(const AttnParams& p, const Globals& g, cudaStream_t stream) {
+    // bf16 is rounded more coarsely than the weights are
+    return p.out_dtype != LCA_DTYPE_BF16 ? attention_of<D, NT, KB, true>(p, g, stream)
+                                         : attention_of<D, NT, KB, false>(p, g, stream);
 }
 
 template <int D>
-cudaError_t attention_rows(int tile_rows, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    const bool split_w = p.out_dtype != LCA_DTYPE_BF16;  // bf16 is rounded more coarsely than the weights
+cudaError_t attention_rows(int tile_rows, int tile_keys, const AttnParams& p, const Globals& g, cudaStream_t stream) {
     if (tile_rows == 8)
-        return split_w ? attention_of<D, 1, true>(p, g, stream) : attention_of<D, 1, false>(p, g, stream);
-    if (tile_rows == 16)
-        return split_w ? attention_of<D, 2, true>(p, g, stream) : attention_of<D, 2, false>(p, g, stream);
-    if (tile_rows == 32)
-        return split_w ? attention_of<D, 4, true>(p, g, stream) : attention_of<D, 4, false>(p, g, stream);
+        return tile_keys == 64 ? attention_tiles<D, 1, 4>(p, g, stream) : attention_tiles<D, 1, 2>(p, g, stream);
+    if (tile_rows == 16) return attention_tiles<D, 2, 2>(p, g, stream);
+    if (tile_rows == 32) return attention_tiles<D, 4, 2>(p, g, stream);
     const cudaError_t e = launch_chunk(D, p, g, stream);
     return e != cudaSuccess || !p.split ? e : merge_of<D, kChunkRows, kChunkKeys>(p, g, stream);
 }
@@ -689,18 +729,20 @@ AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t h
     const int64_t mean = (rows + batch - 1) / batch * group;
     const bool chunk = mean >= kChunkFrom;
     a.tile_rows = chunk ? kChunkRows : (mean <= 8 ? 8 : (mean <= 16 ? 16 : 32));
-    const int64_t tile = chunk ? kChunkKeys : kTile;
     // at most one partial item a request and head, and a row's heads need so many at least
     const int64_t items = kv_heads * std::min(rows * ((group + a.tile_rows - 1) / a.tile_rows), batch + rows * group / a.tile_rows);
     const int64_t tokens = (a.tile_rows - 2) / group + 2;
-    const int64_t band = std::min((std::min(window, capacity) + tokens - 1) / tile + 2, capacity / tile + 1);
-    const int64_t longest = band + (num_globals + tile - 1) / tile;
+    // the longest item, in keys
+    const int64_t longest = std::min(std::min(window, capacity) + tokens + 63, capacity) + num_globals;
     // Long items are cut wherever a CTA's share of the line ends, and merged by a second kernel;
     // short ones (a band) stay whole, which saves that launch.
     // Many long items of many rows balance by themselves, and their parts are large.
-    a.split = longest > kWholeTiles && (!chunk || items < 4 * kSms);
-    a.min_tiles = chunk ? 4 : kMinTiles;
-    const int per_sm = chunk ? 1 : (a.tile_rows == 8 ? 4 : (a.tile_rows == 16 ? 3 : 2));
+    a.split = longest > kWholeKeys && (!chunk || items < 4 * kSms);
+    // A step of 64 keys shares what it costs besides its keys (waiting, issuing, the vote on the maximum),
+    // where the scores of 64 leave the registers for it and items are long enough to fill the warps.
+    a.tile_keys = chunk ? kChunkKeys : (a.tile_rows == 8 && a.split ? 64 : 32);
+    a.min_tiles = 256 / a.tile_keys;
+    const int per_sm = chunk ? 1 : ctas_per_sm((int)head_dim, a.tile_rows, a.tile_keys);
     a.items = std::min<int64_t>(items, 0x7fffffff);
     a.ctas = (int)(a.split || chunk ? kSms * per_sm : std::min<int64_t>(items, (int64_t)kSms * per_sm * 16));
     if (a.split) {
@@ -710,8 +752,10 @@ AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t h
     return a;
 }
 
-cudaError_t launch_attention(int d, int tile_rows, const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    return d == 64 ? attention_rows<64>(tile_rows, p, g, stream) : attention_rows<128>(tile_rows, p, g, stream);
+cudaError_t launch_attention(int d, int tile_rows, int tile_keys, const AttnParams& p, const Globals& g,
+                             cudaStream_t stream) {
+    return d == 64 ? attention_rows<64>(tile_rows, tile_keys, p, g, stream)
+                   : attention_rows<128>(tile_rows, tile_keys, p, g, stream);
 }
 
 }  // namespace kv4

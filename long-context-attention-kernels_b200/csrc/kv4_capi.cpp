@@ -313,7 +313,8 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     p.scale = scale;
     p.out = out;
     p.lse = lse;
-    return after_launch(lca::kv4::launch_attention((int)head_dim, a.tile_rows, p, g, static_cast<cudaStream_t>(stream)),
+    return after_launch(lca::kv4::launch_attention((int)head_dim, a.tile_rows, a.tile_keys, p, g,
+                                                   static_cast<cudaStream_t>(stream)),
                         "cached attention launch");
 }
 
