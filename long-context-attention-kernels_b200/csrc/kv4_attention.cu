@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
         ptx::mbar_init(&bars[threadIdx.x], 1);
         ptx::fence_mbar_init();
     }
-    ptx::griddep_launch();
+    ptx::griddep_wait();
 
     const Share share = share_of<C::ROWS, C::TILE, kThreads>(p, g, scratch, &found);
     if (share.at >= share.end) return;
@@ -524,6 +524,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
             }
             // ---- the four warps' parts of the segment
             __syncthreads();
+            // The next kernel may be set up now.  Not earlier: its CTAs would take the places that are free
+            // while this grid runs, which are not spread evenly, and keep them.
+            if (at + (t1 - t0) >= end) ptx::griddep_launch();
             float* buf = reinterpret_cast<float*>(smem);
             float2* stats = reinterpret_cast<float2*>(buf + kWarps * C::ROWS * C::PITCH);
 #pragma unroll
@@ -676,16 +679,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
 
 template <int D, int ROWS, int TILE>
 cudaError_t merge_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.items, ROWS);
-    cfg.blockDim = dim3(32 * kMergeWarps);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv4_attention_merge<D, ROWS, TILE>, p, g);
+    return launch_early(kv4_attention_merge<D, ROWS, TILE>, dim3((unsigned)p.items, ROWS), 32 * kMergeWarps, 0, stream, p, g);
 }
 
 template <int D, int NT, int KB, bool SPLIT_W>
@@ -694,8 +688,7 @@ cudaError_t attention_of(const AttnParams& p, const Globals& g, cudaStream_t str
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = allow_smem(kv4_attention<D, NT, KB, SPLIT_W>, smem, done);
     if (e != cudaSuccess) return e;
-    kv4_attention<D, NT, KB, SPLIT_W><<<p.ctas, kThreads, smem, stream>>>(p, g);
-    e = cudaGetLastError();
+    e = launch_early(kv4_attention<D, NT, KB, SPLIT_W>, dim3(p.ctas), kThreads, smem, stream, p, g);
     return e != cudaSuccess || !p.split ? e : merge_of<D, 8 * NT, 16 * KB>(p, g, stream);
 }
 

@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <cstdlib>
+#include <utility>
 
 #include "kv4.h"
 #include "sm100_ptx.cuh"
@@ -240,6 +242,29 @@ __device__ __forceinline__ Share share_of(const AttnParams& p, const Globals& g,
         s.here = locate<ROWS, TILE, THREADS>(p, g, 0, 0, s.at, scratch, found);
     }
     return s;
+}
+
+// Launch with programmatic stream serialisation: the kernel may be set up while the one before it in
+// the stream drains.  Every kernel launched so calls griddep_wait before it touches memory, so the order
+// of the stream's effects is unchanged.  LCA_PDL=0 in the environment launches in plain order.
+template <typename... K, typename... A>
+inline cudaError_t launch_early(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
+                                A&&... args) {
+    static const bool on = [] {
+        const char* e = getenv("LCA_PDL");
+        return !(e != nullptr && e[0] == '0');
+    }();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = on ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
 }
 
 // Dynamic shared memory beyond 48 KB for a kernel, asked for once per device.

@@ -59,6 +59,8 @@ __global__ void __launch_bounds__(kLayoutThreads) kv_layout(const LayoutParams p
     __shared__ uint32_t warp_sums[kLayoutThreads / 32];
     int32_t* s_end = sm;              // end of request b's rows
     int32_t* s_take = sm + p.batch;   // free pages handed out before b; -1: not placed
+    ptx::griddep_wait();
+    ptx::griddep_launch();
     const int per = (p.batch + kLayoutThreads - 1) / kLayoutThreads;
     const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
     const int count = min(max(p.free_count[0], 0), p.free_cap);
@@ -152,6 +154,8 @@ __global__ void __launch_bounds__(kLayoutThreads) kv_layout(const LayoutParams p
 __global__ void __launch_bounds__(kLayoutThreads) kv_release(const ReleaseParams p) {
     extern __shared__ int32_t sm[];
     __shared__ uint32_t warp_sums[kLayoutThreads / 32];
+    ptx::griddep_wait();
+    ptx::griddep_launch();
     const int per = (p.batch + kLayoutThreads - 1) / kLayoutThreads;
     const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
     const int count = min(max(p.free_count[0], 0), p.free_cap);
@@ -283,6 +287,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
     const int lane = threadIdx.x % LANES;
     const long long items = (long long)p.rows * p.pool.kv_heads;
     const long long first = (long long)blockIdx.x * (GROUPS * kRowItems) + threadIdx.x / LANES;
+    ptx::griddep_wait();
+    ptx::griddep_launch();
     Item at[kRowItems];
     uint32_t k[kRowItems][4], v[kRowItems][4];
 #pragma unroll
@@ -363,6 +369,8 @@ __global__ void __launch_bounds__(kRowThreads) kv4_read(const RowsParams p) {
     const int lane = threadIdx.x % LANES;
     const long long items = (long long)p.rows * p.pool.kv_heads;
     const long long first = (long long)blockIdx.x * (GROUPS * kRowItems) + threadIdx.x / LANES;
+    ptx::griddep_wait();
+    ptx::griddep_launch();
     Item at[kRowItems];
     uint32_t k[kRowItems] = {}, v[kRowItems] = {}, kw[kRowItems] = {}, vw[kRowItems] = {};
 #pragma unroll
@@ -394,21 +402,16 @@ unsigned row_blocks(int d, const RowsParams& p) {
 }
 
 template <int D, typename T>
-void append_of(bool vector, const RowsParams& p, cudaStream_t stream) {
-    if (vector)
-        kv4_append<D, T, true><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
-    else
-        kv4_append<D, T, false><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+cudaError_t append_of(bool vector, const RowsParams& p, cudaStream_t stream) {
+    return launch_early(vector ? kv4_append<D, T, true> : kv4_append<D, T, false>, dim3(row_blocks(D, p)), kRowThreads, 0,
+                        stream, p);
 }
 
 template <int D>
-void read_of(int out_dtype, const RowsParams& p, cudaStream_t stream) {
-    if (out_dtype == LCA_DTYPE_F32)
-        kv4_read<D, float><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
-    else if (out_dtype == LCA_DTYPE_F16)
-        kv4_read<D, __half><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
-    else
-        kv4_read<D, __nv_bfloat16><<<row_blocks(D, p), kRowThreads, 0, stream>>>(p);
+cudaError_t read_of(int out_dtype, const RowsParams& p, cudaStream_t stream) {
+    auto kernel = out_dtype == LCA_DTYPE_F32 ? kv4_read<D, float>
+                                             : (out_dtype == LCA_DTYPE_F16 ? kv4_read<D, __half> : kv4_read<D, __nv_bfloat16>);
+    return launch_early(kernel, dim3(row_blocks(D, p)), kRowThreads, 0, stream, p);
 }
 
 }  // namespace
@@ -422,29 +425,25 @@ cudaError_t launch_layout(const LayoutParams& p, cudaStream_t stream) {
         cudaError_t e = cudaFuncSetAttribute(kv_layout, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
         if (e != cudaSuccess) return e;
     }
-    kv_layout<<<blocks, kLayoutThreads, smem, stream>>>(p);
-    return cudaGetLastError();
+    return launch_early(kv_layout, dim3(blocks), kLayoutThreads, smem, stream, p);
 }
 
 cudaError_t launch_release(const ReleaseParams& p, cudaStream_t stream) {
     const int blocks = std::max(1, std::min(148, (p.batch + kLayoutThreads / 32 - 1) / (kLayoutThreads / 32)));
     static_assert(sizeof(int32_t) * kMaxRequests <= 40 * 1024, "shared memory of the scan");
-    kv_release<<<blocks, kLayoutThreads, sizeof(int32_t) * (size_t)p.batch, stream>>>(p);
-    return cudaGetLastError();
+    return launch_early(kv_release, dim3(blocks), kLayoutThreads, sizeof(int32_t) * (size_t)p.batch, stream, p);
 }
 
 cudaError_t launch_append(int d, int dtype, bool vector, const RowsParams& p, cudaStream_t stream) {
     if (d == 64)
-        dtype == LCA_DTYPE_F16 ? append_of<64, __half>(vector, p, stream) : append_of<64, __nv_bfloat16>(vector, p, stream);
-    else
-        dtype == LCA_DTYPE_F16 ? append_of<128, __half>(vector, p, stream)
-                               : append_of<128, __nv_bfloat16>(vector, p, stream);
-    return cudaGetLastError();
+        return dtype == LCA_DTYPE_F16 ? append_of<64, __half>(vector, p, stream)
+                                      : append_of<64, __nv_bfloat16>(vector, p, stream);
+    return dtype == LCA_DTYPE_F16 ? append_of<128, __half>(vector, p, stream)
+                                  : append_of<128, __nv_bfloat16>(vector, p, stream);
 }
 
 cudaError_t launch_read(int d, int out_dtype, const RowsParams& p, cudaStream_t stream) {
-    d == 64 ? read_of<64>(out_dtype, p, stream) : read_of<128>(out_dtype, p, stream);
-    return cudaGetLastError();
+    return d == 64 ? read_of<64>(out_dtype, p, stream) : read_of<128>(out_dtype, p, stream);
 }
 
 }  // namespace kv4

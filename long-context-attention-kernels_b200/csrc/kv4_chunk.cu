@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         s_abort = 0;
         ptx::fence_mbar_init();
     }
-    ptx::griddep_launch();
+    ptx::griddep_wait();
     Walk walk;
     {
         const Share share = share_of<kChunkRows, kKeys, kThreads>(p, g, scratch, &found);
@@ -668,8 +668,7 @@ cudaError_t chunk_of(const AttnParams& p, const Globals& g, cudaStream_t stream)
     static std::atomic<unsigned long long> done{0};
     cudaError_t e = allow_smem(kv4_chunk<D, BF16, SPLIT_W>, Cfg<D>::SMEM, done);
     if (e != cudaSuccess) return e;
-    kv4_chunk<D, BF16, SPLIT_W><<<p.ctas, kThreads, Cfg<D>::SMEM, stream>>>(p, g);
-    return cudaGetLastError();
+    return launch_early(kv4_chunk<D, BF16, SPLIT_W>, dim3(p.ctas), kThreads, Cfg<D>::SMEM, stream, p, g);
 }
 
 template <int D>
