@@ -9,6 +9,7 @@
 // bf16 inputs, head_dim 64 or 128, and launch/device errors are checked.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <vector>
@@ -211,6 +212,11 @@ int device_error() {
 // ------------------------------------------------------------------ paged 4-bit KV cache
 // (include/lca.h lca_kv_* / lca_kv4_* / lca_swa_forward_cached; no counterpart in the reference)
 
+// A new tensor without the dispatcher, which costs a small call a noticeable part of its host time.
+torch::Tensor new_tensor(at::IntArrayRef sizes, c10::ScalarType type, const torch::Device& device) {
+    return at::detail::empty_cuda(sizes, type, device, c10::nullopt);
+}
+
 void check_ints(const torch::Tensor& t, const char* name, int64_t dim, const torch::Device& device) {
     TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kInt32 && t.is_contiguous() && t.dim() == dim, name,
                 " must be a contiguous int32 CUDA tensor with ", dim, " dimension(s)");
@@ -261,7 +267,7 @@ std::vector<torch::Tensor> kv_cache_layout(const torch::Tensor& block_table, con
     TORCH_CHECK(num_tokens >= 0, "num_tokens must be >= 0 (got ", num_tokens, ")");
     c10::cuda::CUDAGuard guard(device);
     const int64_t pad = (num_tokens + 3) / 4 * 4;  // slots and positions on 16-byte boundaries
-    auto all = torch::empty({2 * pad + 4 * batch + 2}, block_table.options());
+    auto all = new_tensor({2 * pad + 4 * batch + 2}, torch::kInt32, device);
     int32_t* at = all.data_ptr<int32_t>();
     int32_t *slots = at, *positions = at + pad, *kv_lens = at + 2 * pad, *placed = kv_lens + batch,
             *next = placed + batch, *count = next + batch, *cu = count + 1;
@@ -291,7 +297,7 @@ std::vector<torch::Tensor> kv_cache_release(const torch::Tensor& block_table, co
                 "seq_lens and release need one value per row of block_table (", batch, ")");
     TORCH_CHECK(free_count.size(0) == 1, "free_count must hold one value");
     c10::cuda::CUDAGuard guard(device);
-    auto next = torch::empty({batch + 1}, block_table.options());
+    auto next = new_tensor({batch + 1}, torch::kInt32, device);
     int32_t* at = next.data_ptr<int32_t>();
     raise_status(lca_kv_release(block_table.data_ptr<int32_t>(), batch, block_table.size(1),
                                 seq_lens.data_ptr<int32_t>(), reinterpret_cast<const uint8_t*>(release.data_ptr<bool>()),
@@ -326,8 +332,8 @@ std::vector<torch::Tensor> kv_cache_read(const torch::Tensor& pool, const torch:
     check_ints(slots, "slots", 1, pool.device());
     const int code = type_code(out_dtype, "out_dtype");
     c10::cuda::CUDAGuard guard(pool.device());
-    auto k = torch::empty({slots.size(0), s.kv_heads, s.head_dim}, pool.options().dtype(out_dtype));
-    auto v = torch::empty_like(k);
+    auto k = new_tensor({slots.size(0), s.kv_heads, s.head_dim}, out_dtype, pool.device());
+    auto v = new_tensor({slots.size(0), s.kv_heads, s.head_dim}, out_dtype, pool.device());
     raise_status(lca_kv4_read(pool.data_ptr(), s.pages, s.kv_heads, s.page_size, s.head_dim, slots.data_ptr<int32_t>(),
                               slots.size(0), k.data_ptr(), v.data_ptr(), code, current_stream()),
                  "kv_cache_read");
@@ -363,17 +369,17 @@ std::vector<torch::Tensor> sliding_window_attention_cached(const torch::Tensor& 
                         O.scalar_type() == out_dtype,
                     "out must be a contiguous tensor of Q's shape and out_dtype on the pool's device");
     } else {
-        O = torch::empty(Q.sizes(), Q.options().dtype(out_dtype));
+        O = new_tensor(Q.sizes(), out_dtype, device);
     }
     torch::Tensor L;
-    if (want_lse) L = torch::empty({heads, rows}, Q.options().dtype(torch::kFloat32));
+    if (want_lse) L = new_tensor({heads, rows}, torch::kFloat32, device);
     const int64_t capacity = block_table.size(1) * s.page_size;
     size_t bytes = 0;
     raise_status(lca_swa_cached_workspace_size(rows, heads, s.kv_heads, s.head_dim, batch, capacity, window_size,
                                                (int64_t)global_tokens.size(), &bytes),
                  "sliding_window_attention_cached");
     torch::Tensor ws;
-    if (bytes > 0) ws = torch::empty({(int64_t)bytes}, pool.options());
+    if (bytes > 0) ws = new_tensor({(int64_t)bytes}, torch::kUInt8, device);
     raise_status(lca_swa_forward_cached(Q.data_ptr(), type_code(Q.scalar_type(), "Q"), Q.stride(0), Q.stride(1), rows,
                                         heads, pool.data_ptr(), s.pages, s.kv_heads, s.page_size, s.head_dim,
                                         block_table.data_ptr<int32_t>(), batch, block_table.size(1),
