@@ -85,6 +85,13 @@ struct Globals {
     int32_t at[kMaxGlobals];  // sorted, unique
 };
 
+// An item that its first CTA could not finish: what the merge has to know of it.
+struct Cut {
+    long long end, per;    // the end of the item on the line of tiles, and a CTA's share of that; end 0: no item
+    int slot;              // of the first part, in the first CTA's two
+    int q0, rows, head, q_tile;
+};
+
 struct AttnParams {
     Pool pool;
     const void* q;
@@ -103,6 +110,7 @@ struct AttnParams {
     long long items;  // at most this many items
     float* part_o;    // [ctas][2][tile rows][d]: the parts of cut items, and
     float2* part_ml;  // [ctas][2][tile rows]: their maxima and sums
+    Cut* cuts;        // [ctas], or NULL: the merge finds the items itself
     int* err_word;
     unsigned long long wait_ns;
 };
@@ -113,7 +121,7 @@ struct AttnPlan {
     int ctas, min_tiles;
     bool split;
     int64_t items;
-    size_t part_o, part_ml;  // bytes
+    size_t part_o, part_ml, cuts;  // bytes
 };
 
 cudaError_t launch_layout(const LayoutParams& p, cudaStream_t stream);

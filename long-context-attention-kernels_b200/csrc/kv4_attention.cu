@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
     ptx::griddep_wait();
 
     const Share share = share_of<C::ROWS, C::TILE, kThreads>(p, g, scratch, &found);
+    if (p.cuts != nullptr && threadIdx.x == 0) p.cuts[blockIdx.x].end = 0;  // until it cuts one off
     if (share.at >= share.end) return;
     const long long end = share.end;
     long long at = share.at;
@@ -550,6 +551,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
             __syncthreads();
             const bool whole = t0 == 0 && t1 == r.tiles;
             const int part = (int)(2 * blockIdx.x) + (at != share.at);
+            if (p.cuts != nullptr && t0 == 0 && t1 < r.tiles && threadIdx.x == 0)
+                p.cuts[blockIdx.x] = {at + r.tiles, share.per, at != share.at, r.q0, r.rows, head, q_tile};
             for (int x = threadIdx.x; x < C::ROWS * (D / 4); x += kThreads) {
                 const int row = x / (D / 4), d = 4 * (x - row * (D / 4));
                 const int of = q_tile * C::ROWS + row;
@@ -596,7 +599,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 
 // The parts of the items that several CTAs shared: one CTA per (item, row), a warp per eighth of the
 // parts.  Parts are summed in the order of the line, so a call's result does not depend on timing.
-// Starts while the attention drains (programmatic launch) and finds its item meanwhile.
+// Starts while the attention drains (programmatic launch).  Where there are fewer items than CTAs of the
+// attention, a CTA finds its item from the lengths meanwhile; else it takes the item that its namesake cut.
 constexpr int kMergeWarps = 8;
 
 template <int D, int ROWS, int TILE>
@@ -607,33 +611,48 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     __shared__ int found_item;
     __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
     const int id = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) found.b = -1;
-    long long line = 0, items = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
-        const Request r = request_of<ROWS, TILE>(p, g, b0 + (int)threadIdx.x);
-        const long long mine = line_of(p, r), count = (long long)r.q_tiles * p.pool.kv_heads;
-        long long before, items_before;
-        const long long all = block_scan<THREADS>(mine, scratch, &before);
-        const long long all_items = block_scan<THREADS>(count, scratch, &items_before);
-        if (items + items_before <= id && id < items + items_before + count) {
-            found = {b0 + (int)threadIdx.x, line + before, r};
-            found_item = (int)(id - items - items_before);
+    Cut cut = {};
+    int c0 = id, c1;
+    if (p.cuts != nullptr) {  // a CTA per CTA of the attention
+        ptx::griddep_wait();
+        cut = p.cuts[id];
+        if (cut.end == 0) return;
+        c1 = (int)divide64(cut.end - 1, cut.per);
+    } else {  // a CTA per item: few of them, so few lengths too
+        if (threadIdx.x == 0) found.b = -1;
+        long long line = 0, items = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += THREADS) {
+            const Request r = request_of<ROWS, TILE>(p, g, b0 + (int)threadIdx.x);
+            const long long mine = line_of(p, r), count = (long long)r.q_tiles * p.pool.kv_heads;
+            long long before, items_before;
+            const long long all = block_scan<THREADS>(mine, scratch, &before);
+            const long long all_items = block_scan<THREADS>(count, scratch, &items_before);
+            if (items + items_before <= id && id < items + items_before + count) {
+                found = {b0 + (int)threadIdx.x, line + before, r};
+                found_item = (int)(id - items - items_before);
+            }
+            line += all;
+            items += all_items;
         }
-        line += all;
-        items += all_items;
+        __syncthreads();
+        if (found.b < 0) return;
+        const Request r = found.r;
+        const long long per = max(divide(line + p.ctas - 1, p.ctas), (long long)p.min_tiles);
+        const long long s = found.start + (long long)found_item * r.tiles;
+        c0 = (int)divide64(s, per);
+        c1 = (int)divide64(s + r.tiles - 1, per);
+        cut.slot = s > c0 * per;
+        cut.q0 = r.q0;
+        cut.rows = r.rows;
+        cut.head = found_item / r.q_tiles;
+        cut.q_tile = found_item - cut.head * r.q_tiles;
+        if (c0 == c1) return;  // one CTA had it all and wrote the output
+        ptx::griddep_wait();
     }
-    __syncthreads();
-    if (found.b < 0) return;
-    const Request r = found.r;
-    const int head = found_item / r.q_tiles, q_tile = found_item - head * r.q_tiles, of = q_tile * ROWS + row;
-    if (of >= r.rows) return;
-    const long long per = max(divide(line + p.ctas - 1, p.ctas), (long long)p.min_tiles);
-    const long long s = found.start + (long long)found_item * r.tiles, e = s + r.tiles;
-    const int c0 = (int)(s / per), c1 = (int)((e - 1) / per);
-    if (c0 == c1) return;  // one CTA had it all and wrote the output
-    ptx::griddep_wait();
+    const int of = cut.q_tile * ROWS + row;
+    if (of >= cut.rows) return;
 
-    auto part_of = [&](int c) { return ((long long)2 * c + (s > c * per)) * ROWS + row; };
+    auto part_of = [&](int c) { return (2ll * c + (c == c0 ? cut.slot : 0)) * ROWS + row; };
     float m = -INFINITY, l = 0.f, o[PER] = {};
     for (int c = c0 + warp; c <= c1; c += kMergeWarps) m = fmaxf(m, p.part_ml[part_of(c)].x);
     const float ref = m == -INFINITY ? 0.f : m;
@@ -671,15 +690,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = sum == 0.f ? 0.f : v[i] * inv;
-    const int token = p.per_group(of), h = head * p.group + of - token * p.group;
-    store_out(p, p.out_dtype, ((long long)(r.q0 + token) * p.heads + h) * D + 4 * threadIdx.x, v);
+    const int token = p.per_group(of), h = cut.head * p.group + of - token * p.group;
+    store_out(p, p.out_dtype, ((long long)(cut.q0 + token) * p.heads + h) * D + 4 * threadIdx.x, v);
     if (p.lse != nullptr && threadIdx.x == 0)
-        p.lse[(long long)h * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        p.lse[(long long)h * p.rows + cut.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 template <int D, int ROWS, int TILE>
 cudaError_t merge_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
-    return launch_early(kv4_attention_merge<D, ROWS, TILE>, dim3((unsigned)p.items, ROWS), 32 * kMergeWarps, 0, stream, p, g);
+    return launch_early(kv4_attention_merge<D, ROWS, TILE>, dim3(p.cuts != nullptr ? p.ctas : (unsigned)p.items, ROWS), 32 * kMergeWarps, 0, stream, p, g);
 }
 
 template <int D, int NT, int KB, bool SPLIT_W>
@@ -737,10 +756,11 @@ AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t h
     a.min_tiles = 256 / a.tile_keys;
     const int per_sm = chunk ? 1 : ctas_per_sm((int)head_dim, a.tile_rows, a.tile_keys);
     a.items = std::min<int64_t>(items, 0x7fffffff);
-    a.ctas = (int)(a.split || chunk ? kSms * per_sm : std::min<int64_t>(items, (int64_t)kSms * per_sm * 16));
+    a.ctas = (int)(a.split || chunk ? kSms * per_sm : std::min<int64_t>(items, (int64_t)kSms * per_sm));
     if (a.split) {
         a.part_o = (size_t)a.ctas * 2 * a.tile_rows * head_dim * sizeof(float);
         a.part_ml = (size_t)a.ctas * 2 * a.tile_rows * sizeof(float2);
+        a.cuts = items > a.ctas ? (size_t)a.ctas * sizeof(Cut) : 0;
     }
     return a;
 }

@@ -154,6 +154,10 @@ __device__ __forceinline__ long long divide(long long a, int b) {
     return (a >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
+__device__ __forceinline__ long long divide64(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 __device__ __forceinline__ long long line_of(const AttnParams& p, const Request& r) {
     return (long long)r.q_tiles * p.pool.kv_heads * r.tiles;
 }

@@ -236,7 +236,7 @@ int lca_swa_cached_workspace_size(int64_t num_rows, int64_t heads, int64_t kv_he
     if (int st = check_heads(num_rows, heads, kv_heads)) return st;
     const lca::kv4::AttnPlan a =
         lca::kv4::plan_attention(num_rows, heads, kv_heads, head_dim, batch, capacity, window_size, num_unique_global);
-    *out_bytes = round256(a.part_o) + a.part_ml;
+    *out_bytes = round256(a.part_o) + round256(a.part_ml) + a.cuts;
     return LCA_OK;
 }
 
@@ -283,7 +283,7 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     if (!aligned(lse, 4)) return report_error(LCA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
     const lca::kv4::AttnPlan a =
         lca::kv4::plan_attention(num_rows, heads, kv_heads, head_dim, batch, capacity, window_size, n);
-    const size_t need = round256(a.part_o) + a.part_ml;
+    const size_t need = round256(a.part_o) + round256(a.part_ml) + a.cuts;
     if (need > 0 && (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need))
         return report_error(LCA_ERR_WORKSPACE, "workspace needs %zu bytes, non-NULL and 256-byte aligned (got %zu)", need,
                             workspace_bytes);
@@ -293,7 +293,9 @@ int lca_swa_forward_cached(const void* q, int dtype, int64_t q_row_stride, int64
     p.split = a.split;
     p.items = a.items;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + round256(a.part_o));
+    uint8_t* at = static_cast<uint8_t*>(workspace) + round256(a.part_o);
+    p.part_ml = reinterpret_cast<float2*>(at);
+    p.cuts = a.cuts > 0 ? reinterpret_cast<lca::kv4::Cut*>(at + round256(a.part_ml)) : nullptr;
     p.bf16 = dtype == LCA_DTYPE_BF16;
     p.out_dtype = out_dtype;
     p.q = q;

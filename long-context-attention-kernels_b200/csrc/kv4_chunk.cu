@@ -181,9 +181,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     }
     ptx::griddep_wait();
     Walk walk;
+    long long per;
     {
         const Share share = share_of<kChunkRows, kKeys, kThreads>(p, g, scratch, &found);
+        if (p.cuts != nullptr && threadIdx.x == 32 * (kMmaWarp + 1)) p.cuts[blockIdx.x].end = 0;  // until it cuts one off
         if (share.at >= share.end) return;
+        per = share.per;
         walk.at = share.at;
         walk.end = share.end;
         walk.here = share.here;
@@ -229,6 +232,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         while (ok && next_item(p, g, walk)) {
             Span span;
             const int tiles = tiles_of(span);
+            if (p.cuts != nullptr && walk.t0 == 0 && walk.t1 < walk.r.tiles && warp == kMmaWarp + 1 && lane == 0)
+                p.cuts[blockIdx.x] = {walk.at + walk.r.tiles, per, walk.at != line_at, walk.r.q0, walk.r.rows, walk.head, walk.q_tile};
             walk.at += walk.t1 - walk.t0;
             if (tiles == 0) continue;
             const int buf = items & 1;

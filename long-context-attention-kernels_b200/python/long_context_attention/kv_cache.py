@@ -10,6 +10,7 @@ captured into a CUDA graph and replayed.  The format of a pool is in include/lca
 from __future__ import annotations
 
 import math
+import operator
 from typing import NamedTuple, Sequence
 
 import torch
@@ -123,8 +124,10 @@ def sliding_window_attention_cached(
     """
     _need_cuda(Q, "Q")
     _no_grad(Q)
-    if not isinstance(window_size, int):
-        raise TypeError("long_context_attention: attention over a cache takes one window_size, an int")
+    try:
+        window_size = operator.index(window_size)
+    except TypeError:
+        raise TypeError("long_context_attention: attention over a cache takes one window_size, an int") from None
     if out_dtype is None:
         out_dtype = torch.float32 if out is None else out.dtype
     got = extension().sliding_window_attention_cached(

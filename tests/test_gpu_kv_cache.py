@@ -275,12 +275,58 @@ def test_many_requests_and_long_lengths():
     check_attention(rng, [20000], [1], 2, 2, 128, 64, 300, list(range(10, 19000, 300)), torch.bfloat16, torch.bfloat16)
 
 
+@pytest.mark.parametrize("lens,new,heads,kv_heads,d,out_dtype", [
+    ([20000, 300], [20, 20], 8, 2, 128, torch.bfloat16),        # few long items of many rows, cut
+    ([2500] * 24, [17] * 24, 32, 8, 64, torch.float32),         # more of them than CTAs
+    ([1700, 2300, 5] * 5, [40, 2, 5] * 5, 6, 6, 64, torch.float16),
+])
+def test_long_chunks_that_are_cut(lens, new, heads, kv_heads, d, out_dtype):
+    check_attention(np.random.default_rng(len(lens)), lens, new, heads, kv_heads, d, 64, 10 ** 5, [3], torch.bfloat16,
+                    out_dtype)
+
+
+def test_more_items_than_ctas():
+    """Hundreds of requests of any length, cut wherever a CTA's share ends."""
+    rng = np.random.default_rng(31)
+    lens = np.concatenate([rng.integers(0, 60, 250), rng.integers(1000, 2500, 20), [0, 0, 1, 2000]])
+    rng.shuffle(lens)
+    check_attention(rng, lens.tolist(), [min(int(n), 1) for n in lens], 6, 3, 64, 64, 10 ** 5, [], torch.float16,
+                    torch.float16)
+    lens = rng.integers(0, 40, 5000)
+    check_attention(rng, lens.tolist(), [min(int(n), 1) for n in lens], 1, 1, 64, 16, 20, [0], torch.bfloat16, torch.float32)
+
+
+def test_a_pool_past_32_bit_offsets():
+    """Pages at the end of a 4.7 GB pool, for every operator that addresses it."""
+    kv_heads, d, page = 16, 128, 128
+    pages = 17000
+    pool = torch.empty(pages, kv_heads, page, d + 8, dtype=torch.uint8, device="cuda")
+    assert pool.numel() > 2 ** 32
+    rng = np.random.default_rng(32)
+    n = 300
+    table = np.array([[pages - 1, 3, pages - 2]])
+    k, v = (torch.tensor(rng.standard_normal((n, kv_heads, d)), dtype=torch.float32).half() for _ in range(2))
+    pos = np.arange(n)
+    slots = ints(table[0, pos // page] * page + pos % page)
+    lca.kv_cache_append(pool, k.cuda(), v.cuda(), slots)
+    values = [swa_oracle.kv4_values(x.float().numpy()) for x in (k, v)]
+    for got, want in zip(lca.kv_cache_read(pool, slots), values):
+        np.testing.assert_array_equal(got.cpu().numpy(), want.astype(np.float32))
+    for new, window in ((1, 200), (1, 10 ** 4), (80, 50)):
+        q = torch.tensor(rng.standard_normal((new, kv_heads, d)), dtype=torch.float32).bfloat16()
+        got, lse = lca.sliding_window_attention_cached(q.cuda(), pool, ints(table), ints([n]), ints([0, new]), window, [2],
+                                                       return_lse=True)
+        want = swa_oracle.cached_attention(q.float().numpy(), *values, window, [2], d ** -0.5)
+        check_rows(got, lse, *want, d, f"{new} new, window {window}")
+
+
 def test_rising_scores_and_scales_of_every_size():
     """Scores that grow along the keys (the running maximum moves all the time), queries far from 1, and a
     negative and a zero scale."""
     rng = np.random.default_rng(10)
     for q_std, scale in ((8.0, 0.05), (2.0 ** -20, 0.1), (2000.0, 1e-4), (1.0, -0.1), (1.0, 0.0)):
-        check_attention(rng, [700], [2], 4, 2, 64, 16, 500, [0], torch.bfloat16, torch.float32, q_std, scale)
+        for new in (2, 70):  # one kernel and the other
+            check_attention(rng, [700], [new], 4, 2, 64, 16, 500, [0], torch.bfloat16, torch.float32, q_std, scale)
     lens, d = [500], 64
     pool, table, _ = filled_cache(rng, lens, 1, d, 16)
     ramp = np.linspace(0, 20, 500)[:, None, None] * np.ones((1, 1, d)) + 0.01
@@ -290,9 +336,9 @@ def test_rising_scores_and_scales_of_every_size():
     slots = table[0, torch.arange(500) // 16].cpu().numpy() * 16 + np.arange(500) % 16
     lca.kv_cache_append(pool, k.cuda(), v.cuda(), ints(slots))
     values = [swa_oracle.kv4_values(x.float().numpy()) for x in (k, v)]
-    q = torch.full((1, 2, d), 0.25, dtype=torch.float16)
-    for out_dtype in (torch.float32, torch.float16):
-        got, lse = lca.sliding_window_attention_cached(q.cuda(), pool, table, ints(lens), ints([0, 1]), 1000, [], 0.2,
+    for out_dtype, new in ((torch.float32, 1), (torch.float16, 1), (torch.float32, 100), (torch.bfloat16, 100)):
+        q = torch.full((new, 2, d), 0.25, dtype=torch.float16)
+        got, lse = lca.sliding_window_attention_cached(q.cuda(), pool, table, ints(lens), ints([0, new]), 1000, [], 0.2,
                                                        out_dtype=out_dtype, return_lse=True)
         check_rows(got, lse, *swa_oracle.cached_attention(q.float().numpy(), *values, 1000, [], 0.2), d, "ramp")
 
@@ -322,6 +368,35 @@ def test_masked_infinities_and_nans_do_not_matter_and_visible_ones_do():
     q[0, 1, 7] = float("inf")  # and a query that is not finite
     got = lca.sliding_window_attention_cached(q.cuda(), pool, *args)
     assert got[0, 1].isnan().all() and got[0, 0].isfinite().all()
+
+
+def test_chunks_with_masked_and_visible_nans():
+    """The same of the kernel for many rows: rows that do not see a NaN key are what they were, those that see
+    it in K or V, or whose query is not finite, are NaN, and no other."""
+    rng = np.random.default_rng(14)
+    n, new, d, page = 400, 100, 128, 16
+    pool, table, _ = filled_cache(rng, [n], 1, d, page)
+    q = torch.tensor(rng.standard_normal((new, 2, d)), dtype=torch.float32).bfloat16()
+    args = (table, ints([n]), ints([0, new]), 60, [5])
+    want, lse = lca.sliding_window_attention_cached(q.cuda(), pool, *args, return_lse=True)
+    bad = torch.full((1, 1, d), float("nan"), device="cuda").half()
+    for which in range(2):
+        hurt = pool.clone()
+        for pos in (100, 350):  # one that no row sees, one that rows 50 to 99 see
+            slot = int(table[0, pos // page]) * page + pos % page
+            lca.kv_cache_append(hurt, *((bad, torch.ones_like(bad)) if which else (torch.ones_like(bad), bad)), ints([slot]))
+        got = lca.sliding_window_attention_cached(q.cuda(), hurt, *args)
+        assert torch.equal(got[:50], want[:50]) and got[50:].isnan().all()
+    q[7, 1, 3], q[8, 0, 0], q[9, 0, 5] = float("inf"), float("nan"), -float("inf")
+    got, got_lse = lca.sliding_window_attention_cached(q.cuda(), pool, *args, return_lse=True)
+    hit = torch.zeros(new, 2, dtype=torch.bool)
+    hit[7, 1], hit[8, 0], hit[9, 0] = True, True, True
+    assert got[hit].isnan().all() and got_lse.t()[hit].isnan().all()
+    assert torch.equal(got[~hit], want[~hit]) and torch.equal(got_lse.t()[~hit], lse.t()[~hit])
+    # more rows than tokens: the first ones see nothing
+    got, got_lse = lca.sliding_window_attention_cached(q[10:].cuda(), pool, table, ints([30]), ints([0, 90]), 60, [5],
+                                                       return_lse=True)
+    assert not got[:60].any() and (got_lse[:, :60] == -math.inf).all() and got[60:].isfinite().all()
 
 
 def test_rows_that_see_nothing():

@@ -133,6 +133,29 @@ def test_cached_attention_refusals():
     assert _cached(c, **{**full, "q": 24}) == c.ERR_INVALID_ARGUMENT and "aligned" in c.last_error()
     assert _cached(c, **full, qhead=68) == c.ERR_INVALID_ARGUMENT
     assert _cached(c, **{**full, "out": 20}) == c.ERR_INVALID_ARGUMENT
+    # long items are cut and need scratch
+    assert _cached(c, **full, width=1000, window=10 ** 6) == c.ERR_WORKSPACE and "workspace" in c.last_error()
+    assert _cached(c, **full, width=1 << 27) == c.ERR_UNSUPPORTED
+
+
+def test_cached_workspace_size():
+    c = _native.cabi()
+    size = ctypes.c_size_t(7)
+
+    def need(rows=64, heads=32, kv_heads=8, d=128, batch=64, capacity=131072, window=256, tokens=0):
+        st = c.lib.lca_swa_cached_workspace_size(rows, heads, kv_heads, d, batch, capacity, window, tokens, ctypes.byref(size))
+        return st, size.value
+
+    assert need() == (c.OK, 0)  # a band stays whole
+    st, one = need(window=131072)
+    assert st == c.OK and one > 0
+    assert need(window=131072, rows=64 * 500)[1] == 0  # many long items of many rows stay whole too
+    assert need(rows=0) == (c.OK, 0) and need(batch=0) == (c.OK, 0)
+    assert need(window=-1)[0] == c.ERR_INVALID_ARGUMENT
+    assert need(heads=12)[0] == c.ERR_INVALID_ARGUMENT
+    assert need(kv_heads=0)[0] == c.ERR_INVALID_ARGUMENT
+    assert need(capacity=-5)[0] == c.ERR_INVALID_ARGUMENT
+    assert c.lib.lca_swa_cached_workspace_size(1, 1, 1, 64, 1, 64, 1, 0, None) == c.ERR_INVALID_ARGUMENT
 
 
 def test_python_refusals():
