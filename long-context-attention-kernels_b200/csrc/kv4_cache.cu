@@ -209,8 +209,8 @@ struct Half<__nv_bfloat16> {
     }
 };
 
-// Quantises one row held by LANES lanes, 8 elements (four pairs) a lane: the lane's word of codes,
-// and the row's word of scale and zero point.  With lo = min(row, 0) and hi = max(row, 0): scale =
+// Quantises one row held by LANES lanes, kPieces pieces of 8 elements (four pairs) a lane: the lane's
+// words of codes, and the row's word of scale and zero point.  With lo = min(row, 0) and hi = max(row, 0): scale =
 // hi/15 - lo/15 (products with fp32 1/15, so that opposite extremes of bf16 do not overflow) with
 // its low four bits cleared, z = rint(-lo / scale), code = clamp(rint(x / scale) + z, 0, 15);
 // quotients are fp32 products with 1 / scale.  Every operation is the IEEE one (no contraction), so
@@ -220,11 +220,17 @@ struct Half<__nv_bfloat16> {
 // The extremes are found on the 16-bit pairs, (max x, max -x) in one word across the lanes, so a
 // step takes one shuffle and one instruction.  rint(y) for |y| < 2^22 is the sum with 1.5 * 2^23, whose
 // low bits are the integer (rint and the conversion to int run at a quarter of that rate).
+constexpr int kPieces = 2;
+
 template <int LANES, typename T>
-__device__ __forceinline__ void quantise(const uint32_t (&x)[4], uint32_t* codes, uint32_t* word) {
+__device__ __forceinline__ void quantise(const uint32_t (&x)[4 * kPieces], uint32_t (&codes)[kPieces], uint32_t* word) {
     using H = Half<T>;
-    const uint32_t up = H::max2(H::max2(x[0], x[1]), H::max2(x[2], x[3]));
-    const uint32_t down = H::max2(H::max2(x[0] ^ H::kSign, x[1] ^ H::kSign), H::max2(x[2] ^ H::kSign, x[3] ^ H::kSign));
+    uint32_t up = x[0], down = x[0] ^ H::kSign;
+#pragma unroll
+    for (int i = 1; i < 4 * kPieces; ++i) {
+        up = H::max2(up, x[i]);
+        down = H::max2(down, x[i] ^ H::kSign);
+    }
     uint32_t ends = H::max2(__byte_perm(up, down, 0x5410), __byte_perm(up, down, 0x7632));
     ends = H::max2(ends, 0u);
 #pragma unroll
@@ -239,23 +245,24 @@ __device__ __forceinline__ void quantise(const uint32_t (&x)[4], uint32_t* codes
     const float zm = normal ? __fadd_rn(__fmul_rn(minus_lo, inv), kMagic) : kMagic;  // kMagic + z
     const float z = __fsub_rn(zm, kMagic);
     const uint64_t magic2 = ptx::f2_pack(kMagic, kMagic), z2 = ptx::f2_pack(z, z);
-    uint32_t w = 0;
 #pragma unroll
-    for (int i = 3; i >= 0; --i) {
-        // the products one by one: a packed product and sum would be contracted into one operation
-        const uint64_t y = ptx::f2_pack(__fmul_rn(H::low(x[i]), inv), __fmul_rn(H::high(x[i]), inv));
-        const uint64_t c = ptx::f2_add(ptx::f2_add(y, magic2), z2);
-        // never below 0: the least element rounds to -z itself
-        w = w * 16u + __float_as_uint(fminf(ptx::f2_hi(c), kMagic + 15.f));
-        w = w * 16u + __float_as_uint(fminf(ptx::f2_lo(c), kMagic + 15.f));
+    for (int piece = 0; piece < kPieces; ++piece) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 4 * piece + 3; i >= 4 * piece; --i) {
+            // the products one by one: a packed product and sum would be contracted into one operation
+            const uint64_t y = ptx::f2_pack(__fmul_rn(H::low(x[i]), inv), __fmul_rn(H::high(x[i]), inv));
+            const uint64_t c = ptx::f2_add(ptx::f2_add(y, magic2), z2);
+            // never below 0: the least element rounds to -z itself
+            w = w * 16u + __float_as_uint(fminf(ptx::f2_hi(c), kMagic + 15.f));
+            w = w * 16u + __float_as_uint(fminf(ptx::f2_lo(c), kMagic + 15.f));
+        }
+        codes[piece] = normal ? w - 0x11111111u * 0x4b400000u : 0u;  // less the bits of kMagic in each
     }
-    *codes = normal ? w - 0x11111111u * 0x4b400000u : 0u;  // less the bits of kMagic in each
     *word = normal ? __float_as_uint(scale) | (__float_as_uint(zm) & 15u) : (finite ? 0u : 0x7fc00000u);
 }
 
 constexpr int kRowThreads = 256;
-constexpr int kRowItems = 2;  // (token, head) pairs of a group of lanes, whose loads are in flight together
-
 struct Item {
     int token, head, row;
     uint8_t* block;  // NULL: a slot outside the pool
@@ -278,51 +285,49 @@ __device__ __forceinline__ Item item_of(const RowsParams& p, long long item, lon
     return r;
 }
 
-// One group of d / 8 lanes per (token, head), kRowItems of them at a time: a lane loads 16 bytes of
-// the K and of the V row and stores one 32-bit word of codes of each.  Bound by memory: 4d
-// bytes read and d + 8 written a pair.
+// One group of d / 16 lanes per (token, head): a lane loads two pieces of 16 bytes of the K and of the V
+// row and stores two 32-bit words of codes of each.  Bound by memory, 4d bytes read and d + 8 written
+// a pair, as long as a row's reductions and its reciprocal are shared by 16 elements of a
+// lane (with 8, the instructions bounded it: 128K tokens of 8 heads of 128 in 162 us, now 124).
 template <int D, typename T, bool VECTOR>
 __global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
-    constexpr int LANES = D / 8, GROUPS = kRowThreads / LANES;
+    constexpr int LANES = D / (8 * kPieces), GROUPS = kRowThreads / LANES;
     const int lane = threadIdx.x % LANES;
     const long long items = (long long)p.rows * p.pool.kv_heads;
-    const long long first = (long long)blockIdx.x * (GROUPS * kRowItems) + threadIdx.x / LANES;
+    const long long item = (long long)blockIdx.x * GROUPS + threadIdx.x / LANES;
     ptx::griddep_wait();
     ptx::griddep_launch();
-    Item at[kRowItems];
-    uint32_t k[kRowItems][4], v[kRowItems][4];
+    const Item at = item_of<D>(p, item, items);
+    uint32_t x[2][4 * kPieces];
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) at[j] = item_of<D>(p, first + j * GROUPS, items);
+    for (int side = 0; side < 2; ++side) {
+        const T* src = side == 0 ? static_cast<const T*>(p.k) + at.token * p.k_token + at.head * p.k_head
+                                 : static_cast<const T*>(p.v) + at.token * p.v_token + at.head * p.v_head;
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) {
-        const T* kp = static_cast<const T*>(p.k) + at[j].token * p.k_token + at[j].head * p.k_head + lane * 8;
-        const T* vp = static_cast<const T*>(p.v) + at[j].token * p.v_token + at[j].head * p.v_head + lane * 8;
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
-        if (at[j].block != nullptr) {
-            if (VECTOR) {
-                a = *reinterpret_cast<const uint4*>(kp);
-                b = *reinterpret_cast<const uint4*>(vp);
-            } else {
-                const uint16_t *k16 = reinterpret_cast<const uint16_t*>(kp), *v16 = reinterpret_cast<const uint16_t*>(vp);
-                a = make_uint4(k16[0] | k16[1] << 16, k16[2] | k16[3] << 16, k16[4] | k16[5] << 16, k16[6] | k16[7] << 16);
-                b = make_uint4(v16[0] | v16[1] << 16, v16[2] | v16[3] << 16, v16[4] | v16[5] << 16, v16[6] | v16[7] << 16);
+        for (int j = 0; j < kPieces; ++j) {
+            uint4 a = make_uint4(0, 0, 0, 0);
+            if (at.block != nullptr) {
+                const T* from = src + 8 * (lane + LANES * j);
+                if (VECTOR) {
+                    a = *reinterpret_cast<const uint4*>(from);
+                } else {
+                    const uint16_t* e = reinterpret_cast<const uint16_t*>(from);
+                    a = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                                   e[6] | (uint32_t)e[7] << 16);
+                }
             }
+            x[side][4 * j] = a.x, x[side][4 * j + 1] = a.y, x[side][4 * j + 2] = a.z, x[side][4 * j + 3] = a.w;
         }
-        k[j][0] = a.x, k[j][1] = a.y, k[j][2] = a.z, k[j][3] = a.w;
-        v[j][0] = b.x, v[j][1] = b.y, v[j][2] = b.z, v[j][3] = b.w;
     }
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) {
-        uint32_t k_codes, k_word, v_codes, v_word;  // every lane takes part in the shuffles
-        quantise<LANES, T>(k[j], &k_codes, &k_word);
-        quantise<LANES, T>(v[j], &v_codes, &v_word);
-        if (at[j].block == nullptr) continue;
-        const int row = at[j].row;
-        uint8_t* block = at[j].block;
-        reinterpret_cast<uint32_t*>(block + row * row_bytes(D))[lane] = k_codes;
-        reinterpret_cast<uint32_t*>(block + v_codes_at(D) + row * row_bytes(D))[lane] = v_codes;
-        if (lane == 0) *reinterpret_cast<uint32_t*>(block + k_words_at(D) + 4 * row) = k_word;
-        if (lane == 1) *reinterpret_cast<uint32_t*>(block + v_words_at(D) + 4 * row) = v_word;
+    for (int side = 0; side < 2; ++side) {
+        uint32_t codes[kPieces], word;  // every lane takes part in the shuffles
+        quantise<LANES, T>(x[side], codes, &word);
+        if (at.block == nullptr) continue;
+        uint32_t* to = reinterpret_cast<uint32_t*>(at.block + (side ? v_codes_at(D) : 0) + at.row * row_bytes(D)) + lane;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) to[LANES * j] = codes[j];
+        if (lane == side) *reinterpret_cast<uint32_t*>(at.block + (side ? v_words_at(D) : k_words_at(D)) + 4 * at.row) = word;
     }
 }
 
@@ -363,47 +368,58 @@ __device__ __forceinline__ void values_of(uint32_t codes, uint32_t word, float (
 
 // The rows of `slots` as values, rounded once to the output's type; a slot outside the pool reads
 // as zeros.  The inverse of kv4_append, with the same lanes; bound by the bytes it writes.
+constexpr int kReadItems = 2;  // pairs of a group of lanes, whose loads are in flight together
+
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowThreads) kv4_read(const RowsParams p) {
-    constexpr int LANES = D / 8, GROUPS = kRowThreads / LANES;
+    constexpr int LANES = D / (8 * kPieces), GROUPS = kRowThreads / LANES;
     const int lane = threadIdx.x % LANES;
     const long long items = (long long)p.rows * p.pool.kv_heads;
-    const long long first = (long long)blockIdx.x * (GROUPS * kRowItems) + threadIdx.x / LANES;
+    const long long first = (long long)blockIdx.x * (GROUPS * kReadItems) + threadIdx.x / LANES;
     ptx::griddep_wait();
     ptx::griddep_launch();
-    Item at[kRowItems];
-    uint32_t k[kRowItems] = {}, v[kRowItems] = {}, kw[kRowItems] = {}, vw[kRowItems] = {};
+    Item at[kReadItems];
+    uint32_t codes[kReadItems][2][kPieces] = {}, words[kReadItems][2] = {};
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) at[j] = item_of<D>(p, first + j * GROUPS, items);
+    for (int i = 0; i < kReadItems; ++i) at[i] = item_of<D>(p, first + i * GROUPS, items);
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) {
-        if (at[j].block == nullptr) continue;
-        const int row = at[j].row;
-        const uint8_t* block = at[j].block;
-        k[j] = reinterpret_cast<const uint32_t*>(block + row * row_bytes(D))[lane];
-        v[j] = reinterpret_cast<const uint32_t*>(block + v_codes_at(D) + row * row_bytes(D))[lane];
-        kw[j] = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row);
-        vw[j] = *reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row);
+    for (int i = 0; i < kReadItems; ++i) {
+        if (at[i].block == nullptr) continue;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const uint8_t* block = at[i].block;
+            const uint32_t* from =
+                reinterpret_cast<const uint32_t*>(block + (side ? v_codes_at(D) : 0) + at[i].row * row_bytes(D)) + lane;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) codes[i][side][j] = from[LANES * j];
+            words[i][side] = *reinterpret_cast<const uint32_t*>(block + (side ? v_words_at(D) : k_words_at(D)) + 4 * at[i].row);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < kRowItems; ++j) {
-        if (first + j * GROUPS >= items) continue;
-        float x[8];
-        values_of(k[j], kw[j], x);
-        store8<T>(static_cast<T*>(p.k) + at[j].token * p.k_token + at[j].head * p.k_head + lane * 8, x);
-        values_of(v[j], vw[j], x);
-        store8<T>(static_cast<T*>(p.v) + at[j].token * p.v_token + at[j].head * p.v_head + lane * 8, x);
+    for (int i = 0; i < kReadItems; ++i) {
+        if (first + i * GROUPS >= items) continue;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            T* to = side == 0 ? static_cast<T*>(p.k) + at[i].token * p.k_token + at[i].head * p.k_head
+                              : static_cast<T*>(p.v) + at[i].token * p.v_token + at[i].head * p.v_head;
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                float x[8];
+                values_of(codes[i][side][j], words[i][side], x);
+                store8<T>(to + 8 * (lane + LANES * j), x);
+            }
+        }
     }
 }
 
-unsigned row_blocks(int d, const RowsParams& p) {
-    const long long groups = kRowThreads / (d / 8) * kRowItems;
-    return (unsigned)(((long long)p.rows * p.pool.kv_heads + groups - 1) / groups);
+unsigned row_blocks(int d, int each, const RowsParams& p) {
+    const long long pairs = kRowThreads / (d / (8 * kPieces)) * each;
+    return (unsigned)(((long long)p.rows * p.pool.kv_heads + pairs - 1) / pairs);
 }
 
 template <int D, typename T>
 cudaError_t append_of(bool vector, const RowsParams& p, cudaStream_t stream) {
-    return launch_early(vector ? kv4_append<D, T, true> : kv4_append<D, T, false>, dim3(row_blocks(D, p)), kRowThreads, 0,
+    return launch_early(vector ? kv4_append<D, T, true> : kv4_append<D, T, false>, dim3(row_blocks(D, 1, p)), kRowThreads, 0,
                         stream, p);
 }
 
@@ -411,7 +427,7 @@ template <int D>
 cudaError_t read_of(int out_dtype, const RowsParams& p, cudaStream_t stream) {
     auto kernel = out_dtype == LCA_DTYPE_F32 ? kv4_read<D, float>
                                              : (out_dtype == LCA_DTYPE_F16 ? kv4_read<D, __half> : kv4_read<D, __nv_bfloat16>);
-    return launch_early(kernel, dim3(row_blocks(D, p)), kRowThreads, 0, stream, p);
+    return launch_early(kernel, dim3(row_blocks(D, kReadItems, p)), kRowThreads, 0, stream, p);
 }
 
 }  // namespace
