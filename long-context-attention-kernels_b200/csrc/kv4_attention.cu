@@ -9,7 +9,12 @@
 //
 // The integers c - z are exact in fp16, so both products run on the tensor cores over them
 // (mma.sync m16n8k16, keys by queries and elements by queries, fp32 sums) and the scales stay in
-// fp32, outside the products: sk multiplies a finished score, sv the weight of its key.
+// fp32, outside the products: sk multiplies a finished score, sv the weight of its key.  For bf16
+// outputs the scores take the codes unconverted: bits 0 .. 3 of an fp16 that is otherwise 0 are the
+// subnormal c 2^-24, bits 4 .. 7 are c 2^-20, both exact operands, and zk_j sum_d q_d is taken off the sum.
+// (That rounds to 2^-24 of sum |q_d| c_jd rather than of sum |q_d (c_jd - zk_j)|, which is too
+// coarse for fp32 outputs; done to V, it would turn elements that are exactly 0 into such a
+// remainder.)
 #include <algorithm>
 
 #include "kv4_attention.cuh"
@@ -37,6 +42,17 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two codes of a word as fp16 subnormals: nibbles 0 and 4 (k = 0), 1 and 5 (16 times larger), 2 and 6, 3 and 7 (16
+// times larger).
+__device__ __forceinline__ uint32_t codes_raw(uint32_t w, int k) {
+    const uint32_t v = k >= 2 ? w >> 8 : w;
+    return v & ((k & 1) ? 0x00f000f0u : 0x000f000fu);
+}
+
+__device__ __forceinline__ float zero_of(uint32_t word) {  // 2^23 + z less 2^23
+    return __uint_as_float((word & 15u) | 0x4b000000u) - 8388608.f;
 }
 
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
@@ -82,6 +98,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
     kv4_attention(const AttnParams p, const __grid_constant__ Globals g) {
     using C = Cfg<D, NT, KB_>;
     constexpr int STEPS = D / 16;  // products over d of a score, and 16-element tiles of O
+    constexpr bool RAW_K = !SPLIT_W;  // scores over the codes as they are
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::MAIN);
     uint64_t* masks = bars + kWarps * C::STAGES;
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 
             // ---- queries: rows of the tile as the second operand, in the order of the K codes
             uint32_t q[NT][STEPS][2];
-            float q_scale[NT][2];             // of this thread's two columns
+            float q_scale[NT][2], q_total[NT][2];  // of this thread's two columns
             int row_hi[NT][2], row_lo[NT][2];  // their positions and band starts
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -254,45 +271,65 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i) raw[i] = 0;
                 }
-                // fp16 as it is; bf16 moved by a power of two that takes the row's largest element to
-                // [2^14, 2^15), where fp16 holds 8 bits of every element down to 2^-31 of it
+                // moved by a power of two that takes the row's largest element to [2^14, 2^15), where fp16 holds
+                // every bit of elements down to 2^-25 of it (2^-21 of a quarter of them below)
                 float mult = fabsf(p.scale) * kLog2e;
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) top = max(top, max(raw[i] & 0x7fffu, (raw[i] >> 16) & 0x7fffu));
                 top = max(top, __shfl_xor_sync(kAll, top, 1));
                 top = max(top, __shfl_xor_sync(kAll, top, 2));
-                if (p.bf16) {
-                    const int e = max((int)(top >> 7) - 127, -100);  // above 2^-100; smaller rows score 0
+                float total = 0.f;  // of the row's elements, as they enter the product
+                {
+                    const int e = p.bf16 ? max((int)(top >> 7) - 127, -100)  // above 2^-100; smaller rows score 0
+                                         : max((int)(top >> 10) - 15, -14);
                     const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
                     mult *= __uint_as_float((uint32_t)max(e - 14 + 127, 0) << 23);
+                    if (p.scale < 0.f) mult = -mult;
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        raw[i] = ptx::pack_f16x2(__uint_as_float(raw[i] << 16) * up,
-                                                 __uint_as_float(raw[i] & 0xffff0000u) * up);
+                    for (int i = 0; i < D / 8; ++i) {
+                        float2 x;
+                        if (p.bf16)
+                            x = make_float2(__uint_as_float(raw[i] << 16), __uint_as_float(raw[i] & 0xffff0000u));
+                        else
+                            x = __half22float2(*reinterpret_cast<const __half2*>(&raw[i]));
+                        raw[i] = ptx::pack_f16x2(x.x * up, x.y * up);
+                    }
                 }
                 // The factor of a score is positive and finite, so that it leaves the -inf of a masked
                 // one alone: the scale's sign goes to the row, a factor of 0 makes it a row of zeros,
                 // and a row that is not finite, or a scale that is not, a row of NaN.
-                const bool finite = top < (p.bf16 ? 0x7f80u : 0x7c00u) && mult < INFINITY;
-                const bool zero = mult < 1.17549435e-38f;
-                if (!finite || zero) mult = 1.f;
+                const bool finite = top < (p.bf16 ? 0x7f80u : 0x7c00u) && fabsf(mult) < INFINITY;
+                const bool zero = fabsf(mult) < 1.17549435e-38f;
+                const uint32_t flip = mult < 0.f ? 0x80008000u : 0u;
+                mult = !finite || zero ? 1.f : fabsf(mult);
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
-                    if (p.scale < 0.f) raw[i] ^= 0x80008000u;
+                    raw[i] ^= flip;
                     if (zero) raw[i] = 0;
                     if (!finite) raw[i] = 0x7e007e00u;
+                    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&raw[i]));
+                    total += x.x + x.y;
                 }
+                if (RAW_K) mult *= 16777216.f;  // the codes are 2^-24 of themselves
 #pragma unroll
                 for (int w = 0; w < D / 32; ++w) {  // elements 8w .. 8w + 7 of this thread's chunk
                     q[nt][2 * w][0] = __byte_perm(raw[4 * w], raw[4 * w + 2], 0x5410);
                     q[nt][2 * w][1] = __byte_perm(raw[4 * w], raw[4 * w + 2], 0x7632);
                     q[nt][2 * w + 1][0] = __byte_perm(raw[4 * w + 1], raw[4 * w + 3], 0x5410);
                     q[nt][2 * w + 1][1] = __byte_perm(raw[4 * w + 1], raw[4 * w + 3], 0x7632);
+                    if (RAW_K) {  // against codes that are 16 times larger
+                        q[nt][2 * w][1] = hmul2(q[nt][2 * w][1], 0x2c002c00u);
+                        q[nt][2 * w + 1][1] = hmul2(q[nt][2 * w + 1][1], 0x2c002c00u);
+                    }
                 }
+                total += __shfl_xor_sync(kAll, total, 1);
+                total += __shfl_xor_sync(kAll, total, 2);
+                total *= 1.f / 16777216.f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     q_scale[nt][e] = __shfl_sync(kAll, mult, 4 * (2 * t + e));
+                    q_total[nt][e] = __shfl_sync(kAll, total, 4 * (2 * t + e));
                     const int col = q_tile * C::ROWS + 8 * nt + 2 * t + e;
                     const int pos = col < r.rows ? r.len - p.per_group(r.rows) + p.per_group(col) : -1;
                     row_hi[nt][e] = pos;
@@ -331,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 
                 // ---- scores
                 float s[KB][NT][4];
-                float sk[2 * KB], sv[2 * KB];
+                float sk[2 * KB], sv[2 * KB], zk[2 * KB];
 #pragma unroll
                 for (int m = 0; m < KB; ++m) {
                     const uint8_t* block = stage + m * block_bytes(D);
@@ -341,9 +378,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                     const uint32_t w1 = *reinterpret_cast<const uint32_t*>(block + k_words_at(D) + 4 * row0 + 32);
                     sk[2 * m] = __uint_as_float(w0 & ~15u);
                     sk[2 * m + 1] = __uint_as_float(w1 & ~15u);
-                    sv[2 * m] = __uint_as_float(*reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0) & ~15u);
-                    sv[2 * m + 1] =
-                        __uint_as_float(*reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0 + 32) & ~15u);
+                    const uint32_t w2 = *reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0);
+                    const uint32_t w3 = *reinterpret_cast<const uint32_t*>(block + v_words_at(D) + 4 * row0 + 32);
+                    sv[2 * m] = __uint_as_float(w2 & ~15u);
+                    sv[2 * m + 1] = __uint_as_float(w3 & ~15u);
+                    zk[2 * m] = zero_of(w0);
+                    zk[2 * m + 1] = zero_of(w1);
                     const Zero z0 = zero_pair((w0 & 15u) * 0x10001u), z1 = zero_pair((w1 & 15u) * 0x10001u);
                     uint32_t c0[D / 32], c1[D / 32];
                     const uint8_t* at0 = block + row0 * row_bytes(D) + t * (D / 8);
@@ -359,8 +399,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                     for (int w = 0; w < D / 32; ++w) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t a0 = codes_pair(c0[w], 2 * h, z0), a1 = codes_pair(c1[w], 2 * h, z1);
-                            const uint32_t a2 = codes_pair(c0[w], 2 * h + 1, z0), a3 = codes_pair(c1[w], 2 * h + 1, z1);
+                            const uint32_t a0 = RAW_K ? codes_raw(c0[w], 2 * h) : codes_pair(c0[w], 2 * h, z0);
+                            const uint32_t a1 = RAW_K ? codes_raw(c1[w], 2 * h) : codes_pair(c1[w], 2 * h, z1);
+                            const uint32_t a2 = RAW_K ? codes_raw(c0[w], 2 * h + 1) : codes_pair(c0[w], 2 * h + 1, z0);
+                            const uint32_t a3 = RAW_K ? codes_raw(c1[w], 2 * h + 1) : codes_pair(c1[w], 2 * h + 1, z1);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
                                 mma(s[m][nt], a0, a1, a2, a3, q[nt][2 * w + h][0], q[nt][2 * w + h][1]);
@@ -405,7 +447,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int c = 0; c < 4 * KB; ++c) s[c >> 2][nt][c & 3] *= sk[c >> 1];
+                    for (int c = 0; c < 4 * KB; ++c) {
+                        float& x = s[c >> 2][nt][c & 3];
+                        if (RAW_K) x -= zk[c >> 1] * q_total[nt][c & 1];
+                        x *= sk[c >> 1];
+                    }
                     if (!full) {
 #pragma unroll
                         for (int c = 0; c < 4 * KB; ++c)
