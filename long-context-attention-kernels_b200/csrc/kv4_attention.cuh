@@ -35,7 +35,7 @@ __device__ __forceinline__ int lower_bound(const int32_t* a, int n, int v) {
 
 __device__ __forceinline__ float lg2(float x) {
     float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 

@@ -39,9 +39,10 @@ struct Cfg {
     static constexpr int Q_PANEL = kHalfRows * 128, KV_PANEL = kKeys * 128;  // 64 elements of every row
     static constexpr int Q_BYTES = D / 64 * Q_PANEL, KV_BYTES = D / 64 * KV_PANEL;
     static constexpr int OFF_KV = 4 * Q_BYTES;  // two buffers of A and B
-    static constexpr int OFF_TABLE = OFF_KV + kRing * 2 * KV_BYTES;  // [kRing][3][kKeys] sk, log2 sv, sv
+    static constexpr int OFF_TABLE = OFF_KV + kRing * 2 * KV_BYTES;  // [kRing][3][kKeys] sk scale log2(e), log2 sv, sv
     static constexpr int OFF_HAVE = OFF_TABLE + kRing * 3 * kKeys * 4;  // [kRing][4] keys that are there, and global ones
-    static constexpr int OFF_BAR = OFF_HAVE + kRing * 16;
+    static constexpr int OFF_ENDS = OFF_HAVE + kRing * 16;  // [kRing][4][2] greatest and least log2 sv of a block
+    static constexpr int OFF_BAR = OFF_ENDS + kRing * 32;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;  // and the alignment of the panels
 };
 
@@ -123,6 +124,12 @@ __device__ __forceinline__ uint4 codes_in_order(uint32_t w, uint32_t zero) {  //
     return make_uint4(pair(a), pair(a >> 8), pair(b), pair(b >> 8));
 }
 
+__device__ __forceinline__ float max_of_warp(float x) {
+    float y;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // 16 bytes to shared memory; `valid` false writes zeros and reads nothing.
 __device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0)
@@ -152,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
     float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
     volatile uint32_t* have_at = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_HAVE);
+    float2* ends = reinterpret_cast<float2*>(smem + C::OFF_ENDS);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t *q_full = bars, *q_free = bars + 2, *kv_full = bars + 4, *kv_free = kv_full + kRing, *s_full = kv_free + kRing,
              *p_full = s_full + 4, *pv_done = p_full + 4, *drain = pv_done + 4;
@@ -319,10 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     } else if (warp >= kSoftmaxWarps) {
         // ============================================================ unpacking
         const int w = warp - kSoftmaxWarps, row = lane & 15, side = lane >> 4;
-        // the factor of the scores is positive and finite (`factor` of the softmax), so that it leaves the -inf of a
-        // masked one alone: the softmax scale's sign, a zero and a NaN go with the scales of K
-        const float mult = fabsf(p.scale) * kLog2e;
-        const float sign = !(mult < INFINITY) ? NAN : (mult < 1.17549435e-38f ? 0.f : copysignf(1.f, p.scale));
+        const float factor = p.scale * kLog2e;
         constexpr int CHUNKS = D / 64;  // 16-byte pieces of a code row per lane
         struct Raw {
             uint4 k[CHUNKS], v[CHUNKS];
@@ -385,12 +390,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 if (!ok) return;
                 float* sk = table + slot * 3 * kKeys;
                 const float scale = __uint_as_float(x.word & ~15u);
+                float lam = 0.f;
                 if (side == 0) {
-                    sk[kBlock * w + row] = scale * sign;
+                    sk[kBlock * w + row] = scale * factor;
                 } else {
-                    sk[kKeys + kBlock * w + row] = fmaxf(lg2(fabsf(scale)), -100.f);
+                    lam = fmaxf(lg2(fabsf(scale)), -100.f);
+                    sk[kKeys + kBlock * w + row] = lam;
                     sk[2 * kKeys + kBlock * w + row] = scale;
                 }
+                const bool counts = side == 1 && ((x.have >> row) & 1);
+                const float most = max_of_warp(counts ? lam : -INFINITY), least = -max_of_warp(counts ? -lam : -INFINITY);
+                if (lane == 0) ends[slot * 4 + w] = make_float2(most, least);
                 if (lane == 0) have_at[slot * 4 + w] = x.have;
                 const uint32_t word_k = __shfl_sync(kAll, x.word, row), word_v = __shfl_sync(kAll, x.word, row + 16);
                 const Zero zv = zero_pair((word_v & 15u) * 0x10001u);
@@ -420,18 +430,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             load(0, a);
             load(1, b);
 #pragma unroll 1
-            for (int i = 0; i < tiles && ok; i += 2) {
+            for (int i = 0; i < tiles && ok; ++i) {  // (two copies of this in one turn cost more in fetching code)
                 store(i, a);
-                load(i + 2, a);
-                store(i + 1, b);
-                load(i + 3, b);
+                a = b;
+                load(i + 2, b);
             }
         }
     } else {
         // ============================================================ softmax
         const int h = warp >> 2, in_half = 32 * (warp & 3) + lane;
-        const float mult = fabsf(p.scale) * kLog2e, factor = mult >= 1.17549435e-38f && mult < INFINITY ? mult : 1.f;
-        const uint64_t factor2 = ptx::f2_pack(factor, factor);
         const uint32_t mine = tmem + 256 * h + ((uint32_t)(32 * (warp & 3)) << 16);
         while (ok && next_item(p, g, walk)) {
             Span span;
@@ -515,16 +522,29 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     }
                 }
 
-                // ---- running maximum of x log2(e) + log2(sv)
+                // ---- running maximum of x + log2(sv): where the scales of V lie within 2^8 of one another, the
+                // sum of the two maxima does as well (the weights come out up to 2^8 smaller, well above
+                // what fp16 holds in full), at a third of the instructions
+                const float4 e0 = *reinterpret_cast<const float4*>(ends + slot * 4), e1 = *reinterpret_cast<const float4*>(ends + slot * 4 + 2);
+                const float most = fmaxf(ptx::fmax3(e0.x, e0.z, e1.x), e1.z), least = fminf(ptx::fmin3(e0.y, e0.w, e1.y), e1.w);
                 float peak = -INFINITY, peak1 = -INFINITY;
+                if (most - least <= 8.f) {
 #pragma unroll
-                for (int j = 0; j < kKeys / 4; ++j) {
-                    const ulonglong2 a = lam[j];
-                    const uint64_t u = ptx::f2_fma(s[2 * j], factor2, a.x), v = ptx::f2_fma(s[2 * j + 1], factor2, a.y);
-                    peak = ptx::fmax3(peak, ptx::f2_lo(u), ptx::f2_hi(u));
-                    peak1 = ptx::fmax3(peak1, ptx::f2_lo(v), ptx::f2_hi(v));
+                    for (int j = 0; j < kKeys / 4; ++j) {
+                        peak = ptx::fmax3(peak, ptx::f2_lo(s[2 * j]), ptx::f2_hi(s[2 * j]));
+                        peak1 = ptx::fmax3(peak1, ptx::f2_lo(s[2 * j + 1]), ptx::f2_hi(s[2 * j + 1]));
+                    }
+                    peak = fmaxf(peak, peak1) + most;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kKeys / 4; ++j) {
+                        const ulonglong2 a = lam[j];
+                        const uint64_t u = ptx::f2_add(s[2 * j], a.x), v = ptx::f2_add(s[2 * j + 1], a.y);
+                        peak = ptx::fmax3(peak, ptx::f2_lo(u), ptx::f2_hi(u));
+                        peak1 = ptx::fmax3(peak1, ptx::f2_lo(v), ptx::f2_hi(v));
+                    }
+                    peak = fmaxf(peak, peak1);
                 }
-                peak = fmaxf(peak, peak1);
                 if (__any_sync(kAll, peak > top + 8.f)) {
                     const float to = fmaxf(peak, top);
                     const float f = to == -INFINITY ? 1.f : ptx::ex2(top - to);
@@ -556,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 #pragma unroll
                     for (int k = 0; k < kKeys / 4; ++k) {
                         const int j = half * (kKeys / 4) + k;
-                        const uint64_t x = ptx::f2_fma(s[j], factor2, ref2);
+                        const uint64_t x = ptx::f2_add(s[j], ref2);
                         const uint64_t e = ptx::f2_pack(ptx::ex2(ptx::f2_lo(x)), ptx::ex2(ptx::f2_hi(x)));
                         sum2 = ptx::f2_add(sum2, e);
                         const ulonglong2 v4 = sv[j >> 1];
