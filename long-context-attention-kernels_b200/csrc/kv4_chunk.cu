@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     extern __shared__ uint8_t raw_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
     float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
-    volatile uint32_t* have_at = reinterpret_cast<volatile uint32_t*>(smem + C::OFF_HAVE);
+    uint32_t* have_at = reinterpret_cast<uint32_t*>(smem + C::OFF_HAVE);
     float2* ends = reinterpret_cast<float2*>(smem + C::OFF_ENDS);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t *q_full = bars, *q_free = bars + 2, *kv_full = bars + 4, *kv_free = kv_full + kRing, *s_full = kv_free + kRing,
@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         if (ok) ok = ptx::mbar_wait(bar, (uint32_t)parity & 1u, &s_abort, p.err_word, LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
     };
     auto wait_all = [&](uint64_t* bar, int parity) {  // for a whole warp: every lane learns the same
+        if (__all_sync(kAll, ok && ptx::mbar_test(bar, (uint32_t)parity & 1u))) return;  // a third of a wait's time
         wait(bar, parity);
         ok = __all_sync(kAll, ok);
     };
@@ -451,12 +452,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             int row_lo = max(0, pos - p.window);
             float top = -INFINITY;
             bool finite = true, any = false;  // the row of q; whether it sees a key
+            int from_key = 0, to_key = 0;  // tiles that begin here are visible to all rows of the warp
             uint64_t sum2 = ptx::f2_pack(0.f, 0.f);
             if (tiles > 0) {
                 if (p.num_globals > 0 && span.first == 0 && valid) {
                     const int k = lower_bound(g.at, p.num_globals, pos);
                     if (k < p.num_globals && g.at[k] == pos) row_lo = 0;
                 }
+                from_key = __reduce_max_sync(kAll, valid ? row_lo : 0);
+                to_key = __reduce_min_sync(kAll, valid ? pos : 0x7fffffff) - kKeys + 1;
                 wait_all(&q_full[items & 1], items >> 1);
                 const uint8_t* q_row = smem + (2 * (items & 1) + h) * C::Q_BYTES + in_half * 128;
                 uint32_t most = 0;
@@ -500,14 +504,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // ---- visibility
                 const bool in_band = tile < span.band;
                 const int key0 = (span.first + tile) * kKeys;
-                const uint32_t h0 = have_at[slot * 4], h1 = have_at[slot * 4 + 1], h2 = have_at[slot * 4 + 2], h3 = have_at[slot * 4 + 3];
-                const uint64_t have = (uint64_t)__byte_perm(h0, h1, 0x5410) | ((uint64_t)__byte_perm(h2, h3, 0x5410) << 32);
-                const bool full = __all_sync(kAll, have == ~0ull && (!valid || !in_band || (row_lo <= key0 && pos >= key0 + kKeys - 1)));
+                const uint4 hs = *reinterpret_cast<const uint4*>(have_at + slot * 4);
+                const uint64_t have = (uint64_t)__byte_perm(hs.x, hs.y, 0x5410) | ((uint64_t)__byte_perm(hs.z, hs.w, 0x5410) << 32);
+                const bool full = have == ~0ull && (!in_band || (key0 >= from_key && key0 <= to_key));
                 uint64_t seen = ~0ull;
                 if (full) {
                     any = true;
                 } else {
-                    const uint64_t glob = (uint64_t)__byte_perm(h0, h1, 0x7632) | ((uint64_t)__byte_perm(h2, h3, 0x7632) << 32);
+                    const uint64_t glob = (uint64_t)__byte_perm(hs.x, hs.y, 0x7632) | ((uint64_t)__byte_perm(hs.z, hs.w, 0x7632) << 32);
                     if (in_band)
                         seen = bits_below(pos - key0 + 1) & (~bits_below(row_lo - key0) | glob);
                     else
