@@ -42,7 +42,8 @@ struct Cfg {
     static constexpr int OFF_TABLE = OFF_KV + kRing * 2 * KV_BYTES;  // [kRing][3][kKeys] sk scale log2(e), log2 sv, sv
     static constexpr int OFF_HAVE = OFF_TABLE + kRing * 3 * kKeys * 4;  // [kRing][4] keys that are there, and global ones
     static constexpr int OFF_ENDS = OFF_HAVE + kRing * 16;  // [kRing][4][2] greatest and least log2 sv of a block
-    static constexpr int OFF_BAR = OFF_ENDS + kRing * 32;
+    static constexpr int OFF_LOST = OFF_ENDS + kRing * 32;  // [kRing][4] keys whose scale of V is not finite
+    static constexpr int OFF_BAR = OFF_LOST + kRing * 16;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;  // and the alignment of the panels
 };
 
@@ -159,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
     float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
     uint32_t* have_at = reinterpret_cast<uint32_t*>(smem + C::OFF_HAVE);
+    uint32_t* lost_at = reinterpret_cast<uint32_t*>(smem + C::OFF_LOST);
     float2* ends = reinterpret_cast<float2*>(smem + C::OFF_ENDS);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t *q_full = bars, *q_free = bars + 2, *kv_full = bars + 4, *kv_free = kv_full + kRing, *s_full = kv_free + kRing,
@@ -397,11 +399,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 } else {
                     lam = fmaxf(lg2(fabsf(scale)), -100.f);
                     sk[kKeys + kBlock * w + row] = lam;
-                    sk[2 * kKeys + kBlock * w + row] = scale;
+                    sk[2 * kKeys + kBlock * w + row] = fabsf(scale) < INFINITY ? scale : 0.f;
                 }
+                // a weight of 0 times such a scale would not be 0, so it is kept out of the products
+                const uint32_t lost = __ballot_sync(kAll, side == 1 && ((x.have >> row) & 1) && !(fabsf(scale) < INFINITY)) >> 16;
                 const bool counts = side == 1 && ((x.have >> row) & 1);
-                const float most = max_of_warp(counts ? lam : -INFINITY), least = -max_of_warp(counts ? -lam : -INFINITY);
-                if (lane == 0) ends[slot * 4 + w] = make_float2(most, least);
+                const float most = lost ? INFINITY : max_of_warp(counts ? lam : -INFINITY), least = -max_of_warp(counts ? -lam : -INFINITY);
+                if (lane == 0) {
+                    ends[slot * 4 + w] = make_float2(most, least);
+                    lost_at[slot * 4 + w] = lost;
+                }
                 if (lane == 0) have_at[slot * 4 + w] = x.have;
                 const uint32_t word_k = __shfl_sync(kAll, x.word, row), word_v = __shfl_sync(kAll, x.word, row + 16);
                 const Zero zv = zero_pair((word_v & 15u) * 0x10001u);
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             const int pos = valid ? r.len - p.per_group(r.rows) + token : -1;
             int row_lo = max(0, pos - p.window);
             float top = -INFINITY;
-            bool finite = true, any = false;  // the row of q; whether it sees a key
+            bool finite = true, any = false, lost = false;  // the row of q; whether it sees a key, and one of V lost
             int from_key = 0, to_key = 0;  // tiles that begin here are visible to all rows of the warp
             uint64_t sum2 = ptx::f2_pack(0.f, 0.f);
             if (tiles > 0) {
@@ -540,6 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     }
                     peak = fmaxf(peak, peak1) + most;
                 } else {
+                    const uint4 ls = *reinterpret_cast<const uint4*>(lost_at + slot * 4);
+                    lost |= (seen & ((uint64_t)(ls.x | ls.y << 16) | ((uint64_t)(ls.z | ls.w << 16) << 32))) != 0;
 #pragma unroll
                     for (int j = 0; j < kKeys / 4; ++j) {
                         const ulonglong2 a = lam[j];
@@ -585,11 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                         sum2 = ptx::f2_add(sum2, e);
                         const ulonglong2 v4 = sv[j >> 1];
                         const uint64_t w = ptx::f2_mul(e, (j & 1) ? v4.y : v4.x);
-                        float w0 = ptx::f2_lo(w), w1 = ptx::f2_hi(w);
-                        if (!full) {  // 0 also where the scale of a key out of sight is not finite
-                            if (!((seen >> (2 * j)) & 1)) w0 = 0.f;
-                            if (!((seen >> (2 * j + 1)) & 1)) w1 = 0.f;
-                        }
+                        const float w0 = ptx::f2_lo(w), w1 = ptx::f2_hi(w);
                         hi[k] = ptx::pack_f16x2(w0, w1);
                         if (SPLIT_W) {
                             const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             float sum = ptx::f2_lo(sum2) + ptx::f2_hi(sum2);
             if (any && !finite) sum = NAN;
             const bool whole = walk.t0 == 0 && walk.t1 == r.tiles;
-            const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
+            const float inv = lost ? NAN : (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f);
             const long long part = (long long)(2 * blockIdx.x + (walk.at != line_at)) * kChunkRows + h * kHalfRows + in_half;
             const long long out_at = ((long long)(r.q0 + token) * p.heads + head) * D;
             if (valid) {
