@@ -25,6 +25,9 @@ __device__ __forceinline__ int uniform(int v) { return __shfl_sync(kAll, v, 0); 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int lower_bound(const int32_t* a, int n, int v) {
+    // the usual answers first: the globals lie at the start of long contexts
+    if (n == 0 || v <= a[0]) return 0;
+    if (v > a[n - 1]) return n;
     int lo = 0;
     while (lo < n) {
         const int mid = (lo + n) >> 1;

@@ -656,11 +656,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 #pragma unroll 4
                 for (int i = 0; i < LANES; ++i) {
                     const int row = AT_ONCE * i + lane / LANES, piece = lane % LANES;
-                    const int x = walk.q_tile * kChunkRows + h * kHalfRows + 32 * (warp & 3) + row, tok = p.per_group(x);
-                    if (x < r.rows)
-                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
-                                                  ((long long)(r.q0 + tok) * p.heads + walk.head * p.group + x - tok * p.group) * D +
-                                                  8 * piece) = *stage(row, piece);
+                    const int to = __shfl_sync(kAll, valid ? (r.q0 + token) * p.heads + head : -1, row);
+                    if (to >= 0)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (long long)to * D + 8 * piece) = *stage(row, piece);
                 }
                 __syncwarp();
             } else {
