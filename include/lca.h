@@ -378,7 +378,7 @@ LCA_API int lca_swa_backward(const void* q, const void* k, const void* v, const 
  * and replayed with other lengths.
  */
 
-/* Most requests of one layout or release call. */
+/* Most requests of one lca_kv_layout, lca_kv_release or lca_swa_forward_cached call. */
 #define LCA_MAX_REQUESTS 8192
 /* Most distinct global tokens of one lca_swa_forward_cached call. */
 #define LCA_MAX_CACHED_GLOBALS 1024
@@ -445,7 +445,7 @@ LCA_API int lca_kv4_read(const void* pool, int64_t num_pages, int64_t kv_heads, 
  *   out     [num_rows][heads][head_dim] contiguous, out_dtype, 16-byte aligned
  *   lse     [heads][num_rows] fp32 natural-log log-sum-exp, or NULL
  * A row that sees nothing (its position is negative) gets zeros and an LSE of -inf.  Rows outside
- * [cu_seqlens[0], cu_seqlens[batch]) are left as they were.  Lengths are clamped to the table's
+ * [cu_seqlens[0], cu_seqlens[batch]) are left as they were, in out and in lse.  Lengths are clamped to the table's
  * capacity (table_width * page_size); a key whose page id is outside the pool is not visible.
  * global_tokens: HOST array of positions in [0, capacity), any order, duplicates allowed, at most
  * LCA_MAX_CACHED_GLOBALS distinct ones; one at or behind a request's length has no effect yet.

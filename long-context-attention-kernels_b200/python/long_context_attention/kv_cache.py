@@ -120,7 +120,7 @@ def sliding_window_attention_cached(
     window of the longest length or more is plain causal attention.  Returns O [rows, heads,
     head_dim] in ``out_dtype`` (default float32), and with ``return_lse`` also the natural-log LSE
     [heads, rows].  A row that sees nothing gets zeros and -inf.  Rows behind the last request are
-    left as they were in ``out`` (without ``out`` they are not initialised).
+    left as they were in ``out``; in the LSE, and in O without ``out``, they are not initialised.
     """
     _need_cuda(Q, "Q")
     _no_grad(Q)
