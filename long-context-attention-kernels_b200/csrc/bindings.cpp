@@ -361,6 +361,8 @@ std::vector<torch::Tensor> sliding_window_attention_cached(const torch::Tensor& 
                 s.head_dim);
     TORCH_CHECK(Q.numel() == 0 || Q.stride(2) == 1, "the last dimension of Q must be contiguous");
     const int64_t rows = Q.size(0), heads = Q.size(1);
+    // a dimension of one has any stride, and none that matters
+    const int64_t row_stride = rows == 1 ? 0 : Q.stride(0), head_stride = heads == 1 ? 0 : Q.stride(1);
     c10::cuda::CUDAGuard guard(device);
     torch::Tensor O;
     if (out.has_value()) {
@@ -380,7 +382,7 @@ std::vector<torch::Tensor> sliding_window_attention_cached(const torch::Tensor& 
                  "sliding_window_attention_cached");
     torch::Tensor ws;
     if (bytes > 0) ws = new_tensor({(int64_t)bytes}, torch::kUInt8, device);
-    raise_status(lca_swa_forward_cached(Q.data_ptr(), type_code(Q.scalar_type(), "Q"), Q.stride(0), Q.stride(1), rows,
+    raise_status(lca_swa_forward_cached(Q.data_ptr(), type_code(Q.scalar_type(), "Q"), row_stride, head_stride, rows,
                                         heads, pool.data_ptr(), s.pages, s.kv_heads, s.page_size, s.head_dim,
                                         block_table.data_ptr<int32_t>(), batch, block_table.size(1),
                                         kv_lens.data_ptr<int32_t>(), cu_seqlens.data_ptr<int32_t>(), window_size,

@@ -112,7 +112,8 @@ def sliding_window_attention_cached(
 ):
     """Causal sliding-window + global-token attention of new tokens over a paged 4-bit cache.
 
-    Q: [rows, heads, head_dim] fp16 or bf16 (last dimension contiguous); request b's rows are
+    Q: [rows, heads, head_dim] fp16 or bf16 (last dimension contiguous, every row of a head on a
+    16-byte boundary); request b's rows are
     ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]`` and are the last of its ``kv_lens[b]`` cached tokens.
     heads is a multiple of the pool's kv_heads.  The mask is that of ``sliding_window_attention(...,
     causal=True)``: key j is visible to the row at position p iff j <= p and (p - j <= window_size, or

@@ -462,6 +462,21 @@ def test_strided_queries_streams_and_graphs():
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
 
 
+def test_strides_of_dimensions_of_one_do_not_matter():
+    rng = np.random.default_rng(14)
+    pool, table, _ = filled_cache(rng, [90], 2, 64, 32)
+    row = torch.randn(1, 4 * 64 + 5, device="cuda").half()
+    args = (pool, table, ints([90]), ints([0, 1]), 40)
+    q = row[:, :4 * 64].view(1, 4, 64)  # one token: the row's stride is odd
+    assert torch.equal(lca.sliding_window_attention_cached(q, *args),
+                       lca.sliding_window_attention_cached(q.clone(), *args))
+    pool, table, _ = filled_cache(rng, [90, 31], 1, 64, 32)
+    args = (pool, table, ints([90, 31]), ints([0, 1, 2]), 40)
+    q = torch.randn(2, 1, 64, device="cuda").half()
+    odd = q.as_strided((2, 1, 64), (64, 5, 1))  # one head
+    assert torch.equal(lca.sliding_window_attention_cached(odd, *args), lca.sliding_window_attention_cached(q, *args))
+
+
 def test_refusals_on_the_device():
     pool = lca.kv_cache_pool(4, 2, 16, 64)
     table, lens, cu = ints([[0, 1]]), ints([5]), ints([0, 1])
