@@ -132,8 +132,8 @@ __device__ __forceinline__ float max_of_warp(float x) {
 }
 
 // 16 bytes to shared memory; `valid` false writes zeros and reads nothing.
-__device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ptx::smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0)
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0)
                  : "memory");
 }
 
@@ -237,7 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     int items = 0;  // items with tiles since the start: query buffer items & 1, the same in every role
     if (warp > kMmaWarp) {
         // ============================================================ queries
-        // D / 8 lanes a row, 16 bytes each, copied asynchronously into the swizzled tile.
+        // D / 8 lanes a row, 16 bytes each, copied asynchronously into the swizzled tile.  The rows' addresses
+        // are found 32 at a time, a lane each (row by row in every lane they took 16000 cycles, which the
+        // first item waits for).
         constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
         const int piece = lane % LANES, sub = lane / LANES;
         while (ok && next_item(p, g, walk)) {
@@ -250,15 +252,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             const int buf = items & 1;
             if (items >= 2) wait_all(&q_free[buf], items / 2 - 1);
             if (!ok) break;
-            uint8_t* to = smem + 2 * buf * C::Q_BYTES + (piece >> 3) * C::Q_PANEL;
+            const uint32_t to = ptx::smem_u32(smem + 2 * buf * C::Q_BYTES + (piece >> 3) * C::Q_PANEL);
             const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)walk.r.q0 * p.q_token +
-                                  (long long)walk.head * p.group * p.q_head + 8 * piece;
-#pragma unroll 4
-            for (int row = (warp - kMmaWarp - 1) * AT_ONCE + sub; row < kChunkRows; row += kQueryWarps * AT_ONCE) {
-                const int x = walk.q_tile * kChunkRows + row, tok = p.per_group(x), in = row & (kHalfRows - 1);
-                const bool there = x < walk.r.rows;
-                cp_async_16(to + (row / kHalfRows) * C::Q_BYTES + in * 128 + (((piece & 7) ^ (in & 7)) << 4),
-                            there ? src + tok * p.q_token + (x - tok * p.group) * p.q_head : p.q, there);
+                                  (long long)walk.head * p.group * p.q_head;
+#pragma unroll 1
+            for (int row0 = 0; row0 < kChunkRows; row0 += 32 * kQueryWarps) {
+                // a lane finds one row, number lane of this warp's 32
+                const int mine = row0 + 32 * (warp - kMmaWarp - 1) + lane, x = walk.q_tile * kChunkRows + mine;
+                const int tok = p.per_group(x);
+                const unsigned long long from =
+                    x < walk.r.rows ? reinterpret_cast<unsigned long long>(src + tok * p.q_token + (x - tok * p.group) * p.q_head) : 0;
+                if (mine - lane >= kChunkRows) break;  // the same in the whole warp
+#pragma unroll 8
+                for (int k = 0; k < LANES; ++k) {
+                    const int which = AT_ONCE * k + sub, row = mine - lane + which, in = row & (kHalfRows - 1);
+                    const unsigned long long at = __shfl_sync(kAll, from, which);
+                    cp_async_16(to + (row / kHalfRows) * C::Q_BYTES + in * 128 + (((piece & 7) ^ (in & 7)) << 4),
+                                at != 0 ? reinterpret_cast<const void*>(at + 16 * piece) : p.q, at != 0);
+                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             ptx::fence_proxy_async_smem();
