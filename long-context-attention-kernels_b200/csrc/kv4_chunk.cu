@@ -10,7 +10,9 @@
 //   MMA warp (1 lane)  S = Q K^T into one of two buffers in TMEM, then O += W V of the tile before, W
 //                      read from TMEM where it lies over its S
 //   softmax warps (8)  a thread per row: scores times scales, the running maximum, weights to fp16
-//   query warps (3)    the next item's query rows into the other of two buffers
+//   query warps (3)    the next item's query rows into the other of two buffers, and what the softmax
+//                      warps need to know of the item (found by themselves it took them 2800 cycles an item,
+//                      and registers of their loop: 2K chunks of 128K contexts in 198 us, now 189)
 // Barriers with one phase per tile of one parity (n & 1), so that a wait for tile n - 1 cannot be
 // answered by a phase before or after it.
 // A tile of codes is unpacked once for 256 rows, and the products of one tile run under
@@ -47,12 +49,21 @@ struct Cfg {
     static constexpr int SMEM = OFF_BAR + 256 + 1024;  // and the alignment of the panels
 };
 
-// The items of this CTA, in order; every warp walks them for itself.
+// The items of this CTA, in order; the warps that feed the others walk them for themselves, the softmax
+// warps get each from the query warps with its queries.
 struct Walk {
     Place here;
     Request r;
     long long at, end;
     int head, q_tile, t0, t1;
+};
+
+struct Item {
+    int q0, rows, first_pos;            // the request's first row, rows, and position of the first
+    int head, q_tile, t0, tiles, whole; // this one's KV head, rows and tiles [t0, t0 + tiles)
+    int first, band;                    // first tile of its band, and tiles of that
+    int part;                           // where its part goes: 0 or 1
+    int there;                          // 0: no more items
 };
 
 template <int ROWS, int TILE>
@@ -167,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
              *p_full = s_full + 4, *pv_done = p_full + 4, *drain = pv_done + 4;
     __shared__ long long scratch[kThreads / 32];
     __shared__ Place found;
+    __shared__ __align__(16) Item s_items[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -174,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&q_full[i], kQueryWarps);
-            ptx::mbar_init(&q_free[i], kSoftmaxWarps);
+            ptx::mbar_init(&q_free[i], kSoftmaxWarps + 1);  // and the MMA warp
         }
         for (int i = 0; i < kRing; ++i) {
             ptx::mbar_init(&kv_full[i], kUnpackWarps);
@@ -234,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     } else {
         ptx::setmaxnreg_inc<kSoftmaxRegs>();
     }
-    int items = 0;  // items with tiles since the start: query buffer items & 1, the same in every role
+    int items = 0;  // items since the start: query buffer items & 1, the same in every role
     if (warp > kMmaWarp) {
         // ============================================================ queries
         // D / 8 lanes a row, 16 bytes each, copied asynchronously into the swizzled tile.  The rows' addresses
@@ -247,16 +259,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             const int tiles = tiles_of(span);
             if (p.cuts != nullptr && walk.t0 == 0 && walk.t1 < walk.r.tiles && warp == kMmaWarp + 1 && lane == 0)
                 p.cuts[blockIdx.x] = {walk.at + walk.r.tiles, per, walk.at != line_at, walk.r.q0, walk.r.rows, walk.head, walk.q_tile};
+            const int part = walk.at != line_at;
             walk.at += walk.t1 - walk.t0;
-            if (tiles == 0) continue;
             const int buf = items & 1;
             if (items >= 2) wait_all(&q_free[buf], items / 2 - 1);
             if (!ok) break;
+            if (warp == kMmaWarp + 1 && lane == 0)
+                s_items[buf] = {walk.r.q0, walk.r.rows, walk.r.len - p.per_group(walk.r.rows), walk.head, walk.q_tile, walk.t0, tiles,
+                                walk.t0 == 0 && walk.t1 == walk.r.tiles, span.first, span.band, part, 1};
             const uint32_t to = ptx::smem_u32(smem + 2 * buf * C::Q_BYTES + (piece >> 3) * C::Q_PANEL);
             const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)walk.r.q0 * p.q_token +
                                   (long long)walk.head * p.group * p.q_head;
 #pragma unroll 1
-            for (int row0 = 0; row0 < kChunkRows; row0 += 32 * kQueryWarps) {
+            for (int row0 = 0; row0 < kChunkRows && tiles > 0; row0 += 32 * kQueryWarps) {
                 // a lane finds one row, number lane of this warp's 32
                 const int mine = row0 + 32 * (warp - kMmaWarp - 1) + lane, x = walk.q_tile * kChunkRows + mine;
                 const int tok = p.per_group(x);
@@ -276,6 +291,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&q_full[buf]);
             ++items;
+        }
+        if (items >= 2) wait_all(&q_free[items & 1], items / 2 - 1);
+        if (ok) {
+            if (warp == kMmaWarp + 1 && lane == 0) s_items[items & 1].there = 0;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&q_full[items & 1]);
         }
     } else if (warp == kMmaWarp) {
         // ============================================================ products
@@ -305,10 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             Span span;
             const int tiles = tiles_of(span);
             walk.at += walk.t1 - walk.t0;
-            if (tiles == 0) continue;
             if (lane == 0) {
                 const uint8_t* q_tile = smem + 2 * (items & 1) * C::Q_BYTES;
                 wait(&q_full[items & 1], items >> 1);
+                if (ok) ptx::mbar_arrive(&q_free[items & 1]);  // seen: no later phase can complete before it was
                 for (int i = 0; i < tiles && ok; ++i, ++n) {
                     wait(&kv_full[n % kRing], n / kRing);
                     if (!ok) break;
@@ -328,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     }
                     if (i > 0) accumulate(n - 1, i == 1);
                 }
-                if (ok) accumulate(n - 1, tiles == 1);
+                if (ok && tiles > 0) accumulate(n - 1, tiles == 1);
             }
             ++items;
             ok = __shfl_sync(kAll, (int)ok, 0) != 0;
@@ -459,27 +480,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         // ============================================================ softmax
         const int h = warp >> 2, in_half = 32 * (warp & 3) + lane;
         const uint32_t mine = tmem + 256 * h + ((uint32_t)(32 * (warp & 3)) << 16);
-        while (ok && next_item(p, g, walk)) {
-            Span span;
-            const int tiles = uniform(tiles_of(span));
-            const Request& r = walk.r;
-            const int of = walk.q_tile * kChunkRows + h * kHalfRows + in_half;
-            const bool valid = of < r.rows;
-            const int token = p.per_group(of), head = walk.head * p.group + of - token * p.group;
-            const int pos = valid ? r.len - p.per_group(r.rows) + token : -1;
+        while (true) {
+            wait_all(&q_full[items & 1], items >> 1);
+            if (!ok) break;
+            const Item& it = s_items[items & 1];  // and its queries' buffer: this warp's until it arrives at q_free
+            if (!it.there) break;
+            const int tiles = uniform(it.tiles), t0 = uniform(it.t0), first = uniform(it.first), band = uniform(it.band);
+            const int of = it.q_tile * kChunkRows + h * kHalfRows + in_half;
+            const bool valid = of < it.rows;
+            const int pos = valid ? it.first_pos + p.per_group(of) : -1;
             int row_lo = max(0, pos - p.window);
             float top = -INFINITY;
             bool finite = true, any = false, lost = false;  // the row of q; whether it sees a key, and one of V lost
             int from_key = 0, to_key = 0;  // tiles that begin here are visible to all rows of the warp
             uint64_t sum2 = ptx::f2_pack(0.f, 0.f);
             if (tiles > 0) {
-                if (p.num_globals > 0 && span.first == 0 && valid) {
+                if (p.num_globals > 0 && first == 0 && valid) {
                     const int k = lower_bound(g.at, p.num_globals, pos);
                     if (k < p.num_globals && g.at[k] == pos) row_lo = 0;
                 }
                 from_key = __reduce_max_sync(kAll, valid ? row_lo : 0);
                 to_key = __reduce_min_sync(kAll, valid ? pos : 0x7fffffff) - kKeys + 1;
-                wait_all(&q_full[items & 1], items >> 1);
                 const uint8_t* q_row = smem + (2 * (items & 1) + h) * C::Q_BYTES + in_half * 128;
                 uint32_t most = 0;
 #pragma unroll
@@ -493,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 
 #pragma unroll 1
             for (int i = 0; i < tiles; ++i, ++n) {
-                const int slot = n % kRing, buf = n & 1, tile = walk.t0 + i;
+                const int slot = n % kRing, buf = n & 1, tile = t0 + i;
                 wait_all(&kv_full[slot], n / kRing);  // complete since its scores are: makes the table visible here
                 wait_all(&s_full[2 * h + buf], n >> 1);
                 if (!ok) break;
@@ -520,8 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 }
 
                 // ---- visibility
-                const bool in_band = tile < span.band;
-                const int key0 = (span.first + tile) * kKeys;
+                const bool in_band = tile < band;
+                const int key0 = (first + tile) * kKeys;
                 const uint4 hs = *reinterpret_cast<const uint4*>(have_at + slot * 4);
                 const uint64_t have = (uint64_t)__byte_perm(hs.x, hs.y, 0x5410) | ((uint64_t)__byte_perm(hs.z, hs.w, 0x5410) << 32);
                 const bool full = have == ~0ull && (!in_band || (key0 >= from_key && key0 <= to_key));
@@ -629,15 +650,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             if (!ok) break;
             float sum = ptx::f2_lo(sum2) + ptx::f2_hi(sum2);
             if (any && !finite) sum = NAN;
-            const bool whole = walk.t0 == 0 && walk.t1 == r.tiles;
+            const bool whole = it.whole;
+            const int token = p.per_group(of), head = it.head * p.group + of - token * p.group, q0 = it.q0;
             const float inv = lost ? NAN : (whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f);
-            const long long part = (long long)(2 * blockIdx.x + (walk.at != line_at)) * kChunkRows + h * kHalfRows + in_half;
-            const long long out_at = ((long long)(r.q0 + token) * p.heads + head) * D;
+            const long long part = (long long)(2 * blockIdx.x + it.part) * kChunkRows + h * kHalfRows + in_half;
+            const long long out_at = ((long long)(q0 + token) * p.heads + head) * D;
             if (valid) {
                 if (!whole) {
                     p.part_ml[part] = make_float2(top, sum);
                 } else if (p.lse != nullptr) {
-                    p.lse[(long long)head * p.rows + r.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+                    p.lse[(long long)head * p.rows + q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
                 }
             }
             if (whole && p.out_dtype != LCA_DTYPE_F32) {
@@ -667,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 #pragma unroll 4
                 for (int i = 0; i < LANES; ++i) {
                     const int row = AT_ONCE * i + lane / LANES, piece = lane % LANES;
-                    const int to = __shfl_sync(kAll, valid ? (r.q0 + token) * p.heads + head : -1, row);
+                    const int to = __shfl_sync(kAll, valid ? (q0 + token) * p.heads + head : -1, row);
                     if (to >= 0)
                         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (long long)to * D + 8 * piece) = *stage(row, piece);
                 }
@@ -690,12 +712,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 }
             }
             ptx::tc_fence_before();  // the next item's products overwrite what was read here
-            if (tiles > 0) {
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(&q_free[items & 1]);
-                ++items;
-            }
-            walk.at += walk.t1 - walk.t0;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&q_free[items & 1]);
+            ++items;
         }
     }
     ptx::tc_fence_before();

@@ -19,7 +19,7 @@ class Cta:
     def __init__(self, items, ring, rng, warps=2, unpackers=2, skip=()):
         self.items, self.ring, self.rng, self.W, self.U = items, ring, rng, warps, unpackers  # tiles of each item
         self.skip = set(skip)
-        self.q_full, self.q_free = ([Bar(n) for _ in range(2)] for n in (1, 2 * warps))
+        self.q_full, self.q_free = ([Bar(n) for _ in range(2)] for n in (1, 2 * warps + 1))
         self.kv_full, self.kv_free = ([Bar(n) for _ in range(ring)] for n in (unpackers, 1))
         self.s_full, self.p_full, self.pv_done = ({(h, b): Bar(n) for h in (0, 1) for b in (0, 1)} for n in (1, warps, 1))
         self.queue = []
@@ -44,6 +44,8 @@ class Cta:
         n = 0
         for k, tiles in enumerate(self.items):
             yield from self.wait(self.q_full[k & 1], k >> 1, "mma: q_full")
+            if "mma: q_free" not in self.skip:
+                self.q_free[k & 1].arrive()
             for i in range(tiles):
                 yield from self.wait(self.kv_full[n % self.ring], n // self.ring, "mma: kv_full")
                 for h in (0, 1):
@@ -51,7 +53,8 @@ class Cta:
                 if i > 0:
                     yield from self.accumulate(n - 1, i == 1)
                 n += 1
-            yield from self.accumulate(n - 1, tiles == 1)
+            if tiles > 0:
+                yield from self.accumulate(n - 1, tiles == 1)
 
     def unpack(self, w):
         n = 0
@@ -67,7 +70,7 @@ class Cta:
                 n += 1
 
     def query(self):
-        for k in range(len(self.items)):
+        for k in range(len(self.items) + 1):  # the last one says that there are no more
             if k >= 2:
                 yield from self.wait(self.q_free[k & 1], (k >> 1) - 1, "query: q_free")
                 assert len(self.left_q.get(k - 2, ())) == 2 * self.W, "query buffer replaced while in use"
@@ -96,12 +99,16 @@ class Cta:
                 self.wrote_p.setdefault((n, h), set()).add(w)
                 self.p_full[h, n & 1].arrive()
                 n += 1
-            yield from self.wait(self.pv_done[h, (n - 1) & 1], (n - 1) >> 1, "softmax: pv_done (output)")
-            assert (n - 1, h) in self.pv, "output read before the last product"
+            if tiles > 0:
+                yield from self.wait(self.pv_done[h, (n - 1) & 1], (n - 1) >> 1, "softmax: pv_done (output)")
+                assert (n - 1, h) in self.pv, "output read before the last product"
             yield None
             self.read_o.setdefault((k, h), set()).add(w)  # rows staged in the item's own query buffer
             self.left_q.setdefault(k, set()).add((h, w))
             self.q_free[k & 1].arrive()
+        k = len(self.items)
+        yield from self.wait(self.q_full[k & 1], k >> 1, "softmax: q_full")
+        assert k in self.q_loaded, "end read before it is there"
 
     # ------------------------------------------------------------ products
     def run_mma(self):
@@ -152,7 +159,7 @@ class Cta:
 
 
 def _items(rng, least=1):
-    return [rng.choice([1, 1, 2, 3, 5, 11]) for _ in range(rng.randint(least, 6))]
+    return [rng.choice([0, 0, 1, 1, 2, 3, 5, 11]) for _ in range(rng.randint(least, 6))]
 
 
 @pytest.mark.parametrize("ring", [2, 3])
@@ -162,10 +169,24 @@ def test_chunk_barrier_protocol(ring):
         Cta(_items(rng), ring, rng).simulate()
 
 
-# The softmax's waits for q_full and kv_full follow from its wait for the scores, whose operands these are;
-# they are there so that the reading threads have themselves seen the writes.
+def test_items_without_tiles_need_the_products_to_keep_up():
+    """Without the MMA warp's arrival at q_free, a query buffer could pass two phases while it waits for one."""
+    rng, caught = random.Random(5), 0
+    for _ in range(300):
+        cta = Cta([0] * 6 + [1, 0, 0, 2], 2, rng, skip={"mma: q_free"})
+        for bar in cta.q_free:
+            bar.count -= 1
+        try:
+            cta.simulate()
+        except AssertionError:
+            caught += 1
+    assert caught > 0
+
+
+# The softmax's wait for kv_full follows from its wait for the scores, whose operand that is;
+# it is there so that the reading threads have themselves seen the writes.
 @pytest.mark.parametrize("what", ["mma: p_full", "mma: q_full", "mma: kv_full", "unpack: kv_free", "query: q_free",
-                                  "softmax: s_full", "softmax: pv_done (rescale)", "softmax: pv_done (output)"])
+                                  "softmax: q_full", "softmax: s_full", "softmax: pv_done (rescale)", "softmax: pv_done (output)"])
 def test_the_model_notices_a_missing_wait(what):
     rng = random.Random(sum(map(ord, what)))
     caught = 0

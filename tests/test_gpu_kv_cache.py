@@ -426,6 +426,28 @@ def test_rows_that_see_nothing():
     torch.testing.assert_close(a, b, rtol=0, atol=0, equal_nan=True)
 
 
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_chunks_that_see_nothing_between_others(out_dtype):
+    """Every other chunk has no cached tokens (a request that was not placed): its rows are zeros, and
+    the rows of the others are those that they are without it."""
+    rng = np.random.default_rng(15)
+    lens = [600 + 7 * b for b in range(20)]
+    pool, table, values = filled_cache(rng, lens, 8, 64, 32)
+    q = torch.randn(20 * 600, 8, 64, device="cuda").bfloat16()
+    kept = [n if b % 2 else 0 for b, n in enumerate(lens)]
+    cu = ints(range(0, 20 * 600 + 1, 600))
+    got, lse = lca.sliding_window_attention_cached(q, pool, table, ints(kept), cu, 100, [3], out_dtype=out_dtype, return_lse=True)
+    got, lse = got.view(20, 600, 8, 64), lse.view(8, 20, 600)
+    assert not got[::2].any() and (lse[:, ::2] == -math.inf).all()
+    want, want_lse = lca.sliding_window_attention_cached(
+        q.view(20, 600, 8, 64)[1::2].reshape(-1, 8, 64), pool, table[1::2].contiguous(), ints(kept[1::2]),
+        ints(range(0, 10 * 600 + 1, 600)), 100, [3], out_dtype=out_dtype, return_lse=True)
+    assert torch.equal(got[1::2], want.view(10, 600, 8, 64)) and torch.equal(lse[:, 1::2], want_lse.view(8, 10, 600))
+    for b in (1, 19):
+        one = swa_oracle.cached_attention(to_np(q[600 * b:600 * (b + 1)]), *values[b], 100, [3], 0.125)
+        check_rows(got[b], lse[:, b], *one, 64, f"request {b}")
+
+
 def test_strided_queries_streams_and_graphs():
     rng = np.random.default_rng(13)
     lens = [900, 40]
