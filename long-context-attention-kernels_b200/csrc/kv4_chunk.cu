@@ -29,7 +29,9 @@ namespace {
 
 constexpr int kHalfRows = 128;            // rows of a tile A or B
 constexpr int kKeys = kChunkKeys;         // keys of a tile
-constexpr int kRing = 2;                  // unpacked tiles
+// unpacked tiles: with two, a tile could only be unpacked once the product of the one before the last was
+// done, and the scores came late (2K chunks of 128K contexts 188 us, with three 157)
+constexpr int kRing = 3;
 constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4, kMmaWarp = kSoftmaxWarps + kUnpackWarps, kQueryWarps = 3;
 constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, products and queries
 // registers a thread of each: 2 * 184 + 80 + 64 = 4 * 128, what the block is launched with
@@ -46,7 +48,7 @@ struct Cfg {
     static constexpr int OFF_ENDS = OFF_HAVE + kRing * 16;  // [kRing][4][2] greatest and least log2 sv of a block
     static constexpr int OFF_LOST = OFF_ENDS + kRing * 32;  // [kRing][4] keys whose scale of V is not finite
     static constexpr int OFF_BAR = OFF_LOST + kRing * 16;
-    static constexpr int SMEM = OFF_BAR + 256 + 1024;  // and the alignment of the panels
+    static constexpr int OFF_REST = OFF_BAR + 8 * (17 + 2 * kRing);  // Rest, below
 };
 
 // The items of this CTA, in order; the warps that feed the others walk them for themselves, the softmax
@@ -65,6 +67,20 @@ struct Item {
     int part;                           // where its part goes: 0 or 1
     int there;                          // 0: no more items
 };
+
+// What else is in shared memory: all of it dynamic, as only so three tiles fit next to 256 rows of 128.
+struct Rest {
+    Item items[2];
+    long long scratch[kThreads / 32];
+    Place found;
+    uint32_t tmem;
+    int abort;
+};
+
+template <int D>
+constexpr int kSmem = Cfg<D>::OFF_REST + (int)sizeof(Rest);
+static_assert(Cfg<128>::OFF_REST % alignof(Rest) == 0 && Cfg<64>::OFF_REST % alignof(Rest) == 0, "alignment");
+static_assert(kSmem<128> <= 232448, "shared memory of a CTA");
 
 template <int ROWS, int TILE>
 __device__ __forceinline__ Place locate_warp(const AttnParams& p, const Globals& g, int from, long long start, long long at) {
@@ -167,8 +183,7 @@ __device__ __forceinline__ void read_out(float (&x)[32], uint32_t taddr, bool so
 template <int D, bool BF16, bool SPLIT_W>
 __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, const __grid_constant__ Globals g) {
     using C = Cfg<D>;
-    extern __shared__ uint8_t raw_smem[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) uint8_t smem[];
     float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
     uint32_t* have_at = reinterpret_cast<uint32_t*>(smem + C::OFF_HAVE);
     uint32_t* lost_at = reinterpret_cast<uint32_t*>(smem + C::OFF_LOST);
@@ -176,11 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t *q_full = bars, *q_free = bars + 2, *kv_full = bars + 4, *kv_free = kv_full + kRing, *s_full = kv_free + kRing,
              *p_full = s_full + 4, *pv_done = p_full + 4, *drain = pv_done + 4;
-    __shared__ long long scratch[kThreads / 32];
-    __shared__ Place found;
-    __shared__ __align__(16) Item s_items[2];
-    __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    Rest& rest = *reinterpret_cast<Rest*>(smem + C::OFF_REST);
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -198,14 +209,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             ptx::mbar_init(&pv_done[i], 1);
         }
         ptx::mbar_init(drain, 1);
-        s_abort = 0;
+        rest.abort = 0;
         ptx::fence_mbar_init();
     }
     ptx::griddep_wait();
     Walk walk;
     long long per;
     {
-        const Share share = share_of<kChunkRows, kKeys, kThreads>(p, g, scratch, &found);
+        const Share share = share_of<kChunkRows, kKeys, kThreads>(p, g, rest.scratch, &rest.found);
         if (p.cuts != nullptr && threadIdx.x == 32 * (kMmaWarp + 1)) p.cuts[blockIdx.x].end = 0;  // until it cuts one off
         if (share.at >= share.end) return;
         per = share.per;
@@ -216,17 +227,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     }
     const long long line_at = walk.at;
     if (warp == kMmaWarp) {
-        ptx::tmem_alloc(&s_tmem, kTmemCols);
+        ptx::tmem_alloc(&rest.tmem, kTmemCols);
         ptx::tmem_relinquish();
     }
     ptx::tc_fence_before();
     __syncthreads();
     ptx::tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = rest.tmem;
 
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity) {
-        if (ok) ok = ptx::mbar_wait(bar, (uint32_t)parity & 1u, &s_abort, p.err_word, LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
+        if (ok) ok = ptx::mbar_wait(bar, (uint32_t)parity & 1u, &rest.abort, p.err_word, LCA_DEVERR_TIMEOUT_CACHE, p.wait_ns);
     };
     auto wait_all = [&](uint64_t* bar, int parity) {  // for a whole warp: every lane learns the same
         if (__all_sync(kAll, ok && ptx::mbar_test(bar, (uint32_t)parity & 1u))) return;  // a third of a wait's time
@@ -265,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
             if (items >= 2) wait_all(&q_free[buf], items / 2 - 1);
             if (!ok) break;
             if (warp == kMmaWarp + 1 && lane == 0)
-                s_items[buf] = {walk.r.q0, walk.r.rows, walk.r.len - p.per_group(walk.r.rows), walk.head, walk.q_tile, walk.t0, tiles,
+                rest.items[buf] = {walk.r.q0, walk.r.rows, walk.r.len - p.per_group(walk.r.rows), walk.head, walk.q_tile, walk.t0, tiles,
                                 walk.t0 == 0 && walk.t1 == walk.r.tiles, span.first, span.band, part, 1};
             const uint32_t to = ptx::smem_u32(smem + 2 * buf * C::Q_BYTES + (piece >> 3) * C::Q_PANEL);
             const uint16_t* src = static_cast<const uint16_t*>(p.q) + (long long)walk.r.q0 * p.q_token +
@@ -294,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         }
         if (items >= 2) wait_all(&q_free[items & 1], items / 2 - 1);
         if (ok) {
-            if (warp == kMmaWarp + 1 && lane == 0) s_items[items & 1].there = 0;
+            if (warp == kMmaWarp + 1 && lane == 0) rest.items[items & 1].there = 0;
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&q_full[items & 1]);
         }
@@ -483,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         while (true) {
             wait_all(&q_full[items & 1], items >> 1);
             if (!ok) break;
-            const Item& it = s_items[items & 1];  // and its queries' buffer: this warp's until it arrives at q_free
+            const Item& it = rest.items[items & 1];  // and its queries' buffer: this warp's until it arrives at q_free
             if (!it.there) break;
             const int tiles = uniform(it.tiles), t0 = uniform(it.t0), first = uniform(it.first), band = uniform(it.band);
             const int of = it.q_tile * kChunkRows + h * kHalfRows + in_half;
@@ -728,9 +739,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 template <int D, bool BF16, bool SPLIT_W>
 cudaError_t chunk_of(const AttnParams& p, const Globals& g, cudaStream_t stream) {
     static std::atomic<unsigned long long> done{0};
-    cudaError_t e = allow_smem(kv4_chunk<D, BF16, SPLIT_W>, Cfg<D>::SMEM, done);
+    cudaError_t e = allow_smem(kv4_chunk<D, BF16, SPLIT_W>, kSmem<D>, done);
     if (e != cudaSuccess) return e;
-    return launch_early(kv4_chunk<D, BF16, SPLIT_W>, dim3(p.ctas), kThreads, Cfg<D>::SMEM, stream, p, g);
+    return launch_early(kv4_chunk<D, BF16, SPLIT_W>, dim3(p.ctas), kThreads, kSmem<D>, stream, p, g);
 }
 
 template <int D>
