@@ -57,7 +57,7 @@ struct Walk {
     Place here;
     Request r;
     long long at, end;
-    int head, q_tile, t0, t1;
+    int head, q_tile, t0, t1;  // q_tile -1: not placed within the request yet
 };
 
 struct Item {
@@ -117,18 +117,27 @@ __device__ __forceinline__ bool next_item(const AttnParams& p, const Globals& g,
         if (w.at >= stop) {
             w.here = locate_warp<kChunkRows, kKeys>(p, g, w.here.b + 1, stop, w.at);
             w.r = w.here.r;
+            w.q_tile = -1;
             continue;
         }
-        const long long in = w.at - w.here.start;
-        const int item = (int)divide(in, w.r.tiles);
-        w.t0 = (int)(in - (long long)item * w.r.tiles);
-        if (!p.split && w.t0 > 0) {  // whole items only: this one belongs to the CTA before
-            w.at = w.here.start + (long long)(item + 1) * w.r.tiles;
-            continue;
+        if (w.q_tile >= 0) {  // the item after the last one, which ended where this one begins
+            w.t0 = 0;
+            if (++w.q_tile == w.r.q_tiles) {
+                w.q_tile = 0;
+                ++w.head;
+            }
+        } else {
+            const long long in = w.at - w.here.start;
+            const int item = in == 0 ? 0 : (int)divide(in, w.r.tiles);
+            w.t0 = (int)(in - (long long)item * w.r.tiles);
+            if (!p.split && w.t0 > 0) {  // whole items only: this one belongs to the CTA before
+                w.at = w.here.start + (long long)(item + 1) * w.r.tiles;
+                continue;
+            }
+            w.head = item == 0 ? 0 : item / w.r.q_tiles;
+            w.q_tile = item - w.head * w.r.q_tiles;
         }
         w.t1 = p.split ? (int)min((long long)w.r.tiles, w.t0 + (w.end - w.at)) : w.r.tiles;
-        w.head = item / w.r.q_tiles;
-        w.q_tile = item - w.head * w.r.q_tiles;
         return true;
     }
     return false;
@@ -224,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
         walk.end = share.end;
         walk.here = share.here;
         walk.r = share.here.r;
+        walk.q_tile = -1;
     }
     const long long line_at = walk.at;
     if (warp == kMmaWarp) {
@@ -526,21 +536,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
 #pragma unroll 1
             for (int i = 0; i < tiles; ++i, ++n) {
                 const int slot = n % kRing, buf = n & 1, tile = t0 + i;
-                wait_all(&kv_full[slot], n / kRing);  // complete since its scores are: makes the table visible here
-                wait_all(&s_full[2 * h + buf], n >> 1);
-                if (!ok) break;
+                // the tile's table is complete since its scores are; its barrier makes it visible here
+                const bool scores = ptx::mbar_test(&s_full[2 * h + buf], (uint32_t)(n >> 1) & 1u);
+                const bool tables = ptx::mbar_test(&kv_full[slot], (uint32_t)(n / kRing) & 1u);
+                if (!__all_sync(kAll, ok && scores && tables)) {
+                    wait_all(&s_full[2 * h + buf], n >> 1);
+                    wait_all(&kv_full[slot], n / kRing);
+                    if (!ok) break;
+                }
                 ptx::tc_fence_after();
                 uint64_t s[kKeys / 2];  // pairs of keys
                 const uint32_t s_at = mine + 128 + 64 * buf;
-                {
-                    float x[32];
+                float x0[32], x1[32];
+                ptx::tmem_ld32(s_at, x0);
+                ptx::tmem_ld32(s_at + 32, x1);
+                // what says which keys count comes while the scores do
+                const uint4 hs = *reinterpret_cast<const uint4*>(have_at + slot * 4);
+                const float4 e0 = *reinterpret_cast<const float4*>(ends + slot * 4), e1 = *reinterpret_cast<const float4*>(ends + slot * 4 + 2);
+                ptx::tmem_wait_ld();
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        ptx::tmem_ld32(s_at + 32 * half, x);
-                        ptx::tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) s[16 * half + j] = ptx::f2_pack(x[2 * j], x[2 * j + 1]);
-                    }
+                for (int j = 0; j < 16; ++j) {
+                    s[j] = ptx::f2_pack(x0[2 * j], x0[2 * j + 1]);
+                    s[16 + j] = ptx::f2_pack(x1[2 * j], x1[2 * j + 1]);
                 }
                 const ulonglong2* sk = reinterpret_cast<const ulonglong2*>(table + slot * 3 * kKeys);
                 const ulonglong2 *lam = sk + kKeys / 4, *sv = lam + kKeys / 4;
@@ -554,7 +571,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // ---- visibility
                 const bool in_band = tile < band;
                 const int key0 = (first + tile) * kKeys;
-                const uint4 hs = *reinterpret_cast<const uint4*>(have_at + slot * 4);
                 const uint64_t have = (uint64_t)__byte_perm(hs.x, hs.y, 0x5410) | ((uint64_t)__byte_perm(hs.z, hs.w, 0x5410) << 32);
                 const bool full = have == ~0ull && (!in_band || (key0 >= from_key && key0 <= to_key));
                 uint64_t seen = ~0ull;
@@ -579,7 +595,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // ---- running maximum of x + log2(sv): where the scales of V lie within 2^8 of one another, the
                 // sum of the two maxima does as well (the weights come out up to 2^8 smaller, well above
                 // what fp16 holds in full), at a third of the instructions
-                const float4 e0 = *reinterpret_cast<const float4*>(ends + slot * 4), e1 = *reinterpret_cast<const float4*>(ends + slot * 4 + 2);
                 const float most = fmaxf(ptx::fmax3(e0.x, e0.z, e1.x), e1.z), least = fminf(ptx::fmin3(e0.y, e0.w, e1.y), e1.w);
                 float peak = -INFINITY, peak1 = -INFINITY;
                 if (most - least <= 8.f) {
