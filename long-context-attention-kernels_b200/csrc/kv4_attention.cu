@@ -645,8 +645,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 
 // The parts of the items that several CTAs shared: one CTA per (item, row), a warp per eighth of the
 // parts.  Parts are summed in the order of the line, so a call's result does not depend on timing.
-// Starts while the attention drains (programmatic launch).  Where there are fewer items than CTAs of the
-// attention, a CTA finds its item from the lengths meanwhile; else it takes the item that its namesake cut.
+// Where there are fewer items than CTAs of the attention, a CTA finds its item from the lengths; else it
+// takes the item that its namesake cut.  Set up while the attention drains (programmatic launch), but every
+// CTA waits for it first, also one that has nothing to merge: what follows in the stream is ordered behind
+// this grid alone, which must not complete before the attention has.
 constexpr int kMergeWarps = 8;
 
 template <int D, int ROWS, int TILE>
@@ -657,10 +659,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     __shared__ int found_item;
     __shared__ float s_m[kMergeWarps], s_l[kMergeWarps], s_o[kMergeWarps][D];
     const int id = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    ptx::griddep_wait();
     Cut cut = {};
     int c0 = id, c1;
     if (p.cuts != nullptr) {  // a CTA per CTA of the attention
-        ptx::griddep_wait();
         cut = p.cuts[id];
         if (cut.end == 0) return;
         c1 = (int)divide64(cut.end - 1, cut.per);
@@ -693,7 +695,6 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
         cut.head = found_item / r.q_tiles;
         cut.q_tile = found_item - cut.head * r.q_tiles;
         if (c0 == c1) return;  // one CTA had it all and wrote the output
-        ptx::griddep_wait();
     }
     const int of = cut.q_tile * ROWS + row;
     if (of >= cut.rows) return;

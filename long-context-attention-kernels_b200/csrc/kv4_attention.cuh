@@ -258,8 +258,8 @@ __device__ __forceinline__ Share share_of(const AttnParams& p, const Globals& g,
 }
 
 // Launch with programmatic stream serialisation: the kernel may be set up while the one before it in
-// the stream drains.  Every kernel launched so calls griddep_wait before it touches memory, so the order
-// of the stream's effects is unchanged.  LCA_PDL=0 in the environment launches in plain order.
+// the stream drains.  Every CTA of a kernel launched so calls griddep_wait before it touches memory and
+// before it returns, so the order of the stream's effects is unchanged.  LCA_PDL=0 in the environment launches in plain order.
 template <typename... K, typename... A>
 inline cudaError_t launch_early(void (*kernel)(K...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream,
                                 A&&... args) {
