@@ -89,10 +89,9 @@ __device__ __forceinline__ int slot_row(int s) { return s ^ ((s >> 1) & 1); }
 // its 8 columns), weights, then O^T += V^T P^T.  The score fragment of a thread holds two
 // queries of a key; transposed 8 x 8 it is the second product's operand.
 //
-// M is the running maximum of x_j log2(e) + log2(sv_j), so that the weights w = p sv that enter the second
-// product as fp16 are at most 1 (2^8 between rescalings) whatever the sizes of V; p itself, which the
-// sum l takes, stays within 2^100 of it because log2(sv) is cut at -100.  Rounding: w to fp16
-// (2^-11); with an fp32 output the remainder w - fp16(w) goes through a second product (2^-22).
+// The weights w = p sv enter the second product as fp16 whatever the sizes of V, moved to the upper part of
+// its range (kv4_attention.cuh, kHead); with an output finer than bf16 the remainder w - fp16(w) goes through
+// a second product.
 template <int D, int NT, int KB_, bool SPLIT_W>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
     kv4_attention(const AttnParams p, const __grid_constant__ Globals g) {
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                 // ---- softmax
                 float lam[2 * KB];
 #pragma unroll
-                for (int c = 0; c < 2 * KB; ++c) lam[c] = fmaxf(lg2(fabsf(sv[c])), -100.f);
+                for (int c = 0; c < 2 * KB; ++c) lam[c] = fmaxf(lg2(fabsf(sv[c])), kLeast);
                 bool raise = false;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -467,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                     return m;
                 };
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) raise |= peaks(nt, 0) > top[nt][0] + 8.f || peaks(nt, 1) > top[nt][1] + 8.f;
+                for (int nt = 0; nt < NT; ++nt) raise |= peaks(nt, 0) > top[nt][0] + kRise || peaks(nt, 1) > top[nt][1] + kRise;
                 if (__any_sync(kAll, raise)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
@@ -477,8 +476,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                             float to = peaks(nt, e);
 #pragma unroll
                             for (int m = 4; m < 32; m *= 2) to = fmaxf(to, __shfl_xor_sync(kAll, to, m));
-                            to = fmaxf(to, top[nt][e]);
-                            f[e] = to == -INFINITY ? 1.f : ptx::ex2(top[nt][e] - to);
+                            const bool rise = to > top[nt][e] + kRise;
+                            to = rise ? to - kHead : top[nt][e];
+                            f[e] = rise ? ptx::ex2(top[nt][e] - to) : 1.f;
                             top[nt][e] = to;
                             sum[nt][e] *= f[e];
                         }
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                     v[0] *= inv, v[1] *= inv, v[2] *= inv, v[3] *= inv;
                     store_out(p, p.out_dtype, ((long long)(r.q0 + token) * p.heads + h) * D + d, v);
                     if (p.lse != nullptr && d == 0)
-                        p.lse[(long long)h * p.rows + r.q0 + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+                        p.lse[(long long)h * p.rows + r.q0 + token] = lse_of(m, l);
                 } else {
                     const long long to = (long long)part * C::ROWS + row;
                     *reinterpret_cast<float4*>(p.part_o + to * D + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -740,7 +740,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     const int token = p.per_group(of), h = cut.head * p.group + of - token * p.group;
     store_out(p, p.out_dtype, ((long long)(cut.q0 + token) * p.heads + h) * D + 4 * threadIdx.x, v);
     if (p.lse != nullptr && threadIdx.x == 0)
-        p.lse[(long long)h * p.rows + cut.q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+        p.lse[(long long)h * p.rows + cut.q0 + token] = lse_of(top, sum);
 }
 
 template <int D, int ROWS, int TILE>

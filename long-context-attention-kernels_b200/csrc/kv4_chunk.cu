@@ -37,6 +37,7 @@ constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, p
 // registers a thread of each: 2 * 184 + 80 + 64 = 4 * 128, what the block is launched with
 constexpr int kSoftmaxRegs = 184, kUnpackRegs = 80, kMmaRegs = 64;
 constexpr uint32_t kTmemCols = 512;
+constexpr float kSpan = 3.f;  // log2 of how far V's scales in a tile may differ for the quick maximum
 
 template <int D>
 struct Cfg {
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 if (side == 0) {
                     sk[kBlock * w + row] = scale * factor;
                 } else {
-                    lam = fmaxf(lg2(fabsf(scale)), -100.f);
+                    lam = fmaxf(lg2(fabsf(scale)), kLeast);
                     sk[kKeys + kBlock * w + row] = lam;
                     sk[2 * kKeys + kBlock * w + row] = fabsf(scale) < INFINITY ? scale : 0.f;
                 }
@@ -592,12 +593,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     }
                 }
 
-                // ---- running maximum of x + log2(sv): where the scales of V lie within 2^8 of one another, the
-                // sum of the two maxima does as well (the weights come out up to 2^8 smaller, well above
-                // what fp16 holds in full), at a third of the instructions
+                // ---- running maximum of x + log2(sv): where the scales of V lie within 2^kSpan of one another, the
+                // sum of the two maxima does as well (the weights come out up to 2^kSpan smaller), at a third of
+                // the instructions
                 const float most = fmaxf(ptx::fmax3(e0.x, e0.z, e1.x), e1.z), least = fminf(ptx::fmin3(e0.y, e0.w, e1.y), e1.w);
                 float peak = -INFINITY, peak1 = -INFINITY;
-                if (most - least <= 8.f) {
+                if (most - least <= kSpan) {
 #pragma unroll
                     for (int j = 0; j < kKeys / 4; ++j) {
                         peak = ptx::fmax3(peak, ptx::f2_lo(s[2 * j]), ptx::f2_hi(s[2 * j]));
@@ -616,9 +617,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     }
                     peak = fmaxf(peak, peak1);
                 }
-                if (__any_sync(kAll, peak > top + 8.f)) {
-                    const float to = fmaxf(peak, top);
-                    const float f = to == -INFINITY ? 1.f : ptx::ex2(top - to);
+                const bool rise = peak > top + kRise;
+                if (__any_sync(kAll, rise)) {
+                    const float to = rise ? peak - kHead : top;
+                    const float f = rise ? ptx::ex2(top - to) : 1.f;
                     top = to;
                     sum2 = ptx::f2_mul(sum2, ptx::f2_pack(f, f));
                     if (i > 0) {
@@ -641,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // ---- weights
                 const float ref = top == -INFINITY ? 0.f : -top;
                 const uint64_t ref2 = ptx::f2_pack(ref, ref);
+                uint64_t tile2 = ptx::f2_pack(0.f, 0.f);  // the tile's own sum first: a chain of 32 + tiles, not of 32 tiles
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t hi[kKeys / 4], lo[kKeys / 4];
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                         const int j = half * (kKeys / 4) + k;
                         const uint64_t x = ptx::f2_add(s[j], ref2);
                         const uint64_t e = ptx::f2_pack(ptx::ex2(ptx::f2_lo(x)), ptx::ex2(ptx::f2_hi(x)));
-                        sum2 = ptx::f2_add(sum2, e);
+                        tile2 = ptx::f2_add(tile2, e);
                         const ulonglong2 v4 = sv[j >> 1];
                         const uint64_t w = ptx::f2_mul(e, (j & 1) ? v4.y : v4.x);
                         const float w0 = ptx::f2_lo(w), w1 = ptx::f2_hi(w);
@@ -662,6 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     ptx::tmem_st16u(s_at + kKeys / 4 * half, hi);
                     if constexpr (SPLIT_W) ptx::tmem_st16u(s_at + kKeys / 2 + kKeys / 4 * half, lo);
                 }
+                sum2 = ptx::f2_add(sum2, tile2);
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before();
                 __syncwarp();
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 if (!whole) {
                     p.part_ml[part] = make_float2(top, sum);
                 } else if (p.lse != nullptr) {
-                    p.lse[(long long)head * p.rows + q0 + token] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+                    p.lse[(long long)head * p.rows + q0 + token] = lse_of(top, sum);
                 }
             }
             if (whole && p.out_dtype != LCA_DTYPE_F32) {
