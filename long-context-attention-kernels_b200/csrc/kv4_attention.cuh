@@ -29,19 +29,16 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // another fp16.  fp16 has no step below 2^-24, so a long tail of small weights would vanish if the largest
 // were 1: M is taken kHead below the running maximum of y, and moves once y has passed it by kRise, so the
 // largest weight of a row is at least 2^kHead and none passes 2^kRise = 61147 of fp16's 65504.  Two halves are
-// off by at most 2^-22 of w_j, or 2^-34 of the row's largest weight where that is more (in the chunk kernel,
-// whose maximum may be 2^kSpan too large, 2^-31); one half by 2^-11 of w_j instead of the 2^-22.  With M the maximum
-// itself (kHead 0, kRise 8, kSpan 8), 100000 equal keys 2^16.7 below a sink beside a row of V 200 times
-// larger came out 0.13 of |v| wrong.  A greater kHead leaves less room before M has to move: 11 and 15, which
-// would gain a factor 4, take 161 us instead of 156 for four chunks of 2K (bf16, 32 / 8 heads of 128,
-// window 512).
+// off by at most 2^-22 of w_j, or 2^-33 of the row's largest weight where that is more; one half by 2^-11 of w_j
+// instead of the 2^-22.  A greater kHead leaves less room before M has to move: 9 gains a factor 2 and takes
+// 157 us instead of 154 for four chunks of 2K (bf16, 32 / 8 heads of 128, window 512).
 // The sum takes p_j = w_j / sv_j; log2(sv) is cut off at kLeast, so that 2^30 of them stay in fp32's range.
-constexpr float kHead = 9.f, kRise = 15.9f, kLeast = -80.f;
+constexpr float kHead = 8.f, kRise = 15.9f, kLeast = -80.f;
 
 // The natural logarithm of a row's sum l 2^m.
 __device__ __forceinline__ float lse_of(float m, float l) {
-    constexpr float kTakeOff = 1.f / 512.f;
-    static_assert(kHead == 9.f, "kTakeOff is 2^-kHead");
+    constexpr float kTakeOff = 1.f / 256.f;
+    static_assert(kHead == 8.f, "kTakeOff is 2^-kHead");
     return l == 0.f ? -INFINITY : ((m + kHead) + log2f(l * kTakeOff)) * kLn2;
 }
 

@@ -37,7 +37,6 @@ constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, p
 // registers a thread of each: 2 * 184 + 80 + 64 = 4 * 128, what the block is launched with
 constexpr int kSoftmaxRegs = 184, kUnpackRegs = 80, kMmaRegs = 64;
 constexpr uint32_t kTmemCols = 512;
-constexpr float kSpan = 3.f;  // log2 of how far V's scales in a tile may differ for the quick maximum
 
 template <int D>
 struct Cfg {
@@ -46,8 +45,8 @@ struct Cfg {
     static constexpr int OFF_KV = 4 * Q_BYTES;  // two buffers of A and B
     static constexpr int OFF_TABLE = OFF_KV + kRing * 2 * KV_BYTES;  // [kRing][3][kKeys] sk scale log2(e), log2 sv, sv
     static constexpr int OFF_HAVE = OFF_TABLE + kRing * 3 * kKeys * 4;  // [kRing][4] keys that are there, and global ones
-    static constexpr int OFF_ENDS = OFF_HAVE + kRing * 16;  // [kRing][4][2] greatest and least log2 sv of a block
-    static constexpr int OFF_LOST = OFF_ENDS + kRing * 32;  // [kRing][4] keys whose scale of V is not finite
+    static constexpr int OFF_MOST = OFF_HAVE + kRing * 16;  // [kRing][4] greatest log2 sv of a block
+    static constexpr int OFF_LOST = OFF_MOST + kRing * 16;  // [kRing][4] keys whose scale of V is not finite
     static constexpr int OFF_BAR = OFF_LOST + kRing * 16;
     static constexpr int OFF_REST = OFF_BAR + 8 * (17 + 2 * kRing);  // Rest, below
 };
@@ -197,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
     float* table = reinterpret_cast<float*>(smem + C::OFF_TABLE);
     uint32_t* have_at = reinterpret_cast<uint32_t*>(smem + C::OFF_HAVE);
     uint32_t* lost_at = reinterpret_cast<uint32_t*>(smem + C::OFF_LOST);
-    float2* ends = reinterpret_cast<float2*>(smem + C::OFF_ENDS);
+    float* most_at = reinterpret_cast<float*>(smem + C::OFF_MOST);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t *q_full = bars, *q_free = bars + 2, *kv_full = bars + 4, *kv_free = kv_full + kRing, *s_full = kv_free + kRing,
              *p_full = s_full + 4, *pv_done = p_full + 4, *drain = pv_done + 4;
@@ -458,12 +457,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 // a weight of 0 times such a scale would not be 0, so it is kept out of the products
                 const uint32_t lost = __ballot_sync(kAll, side == 1 && ((x.have >> row) & 1) && !(fabsf(scale) < INFINITY)) >> 16;
                 const bool counts = side == 1 && ((x.have >> row) & 1);
-                const float most = lost ? INFINITY : max_of_warp(counts ? lam : -INFINITY), least = -max_of_warp(counts ? -lam : -INFINITY);
+                const float most = lost ? INFINITY : max_of_warp(counts ? lam : -INFINITY);
                 if (lane == 0) {
-                    ends[slot * 4 + w] = make_float2(most, least);
+                    most_at[slot * 4 + w] = most;
                     lost_at[slot * 4 + w] = lost;
+                    have_at[slot * 4 + w] = x.have;
                 }
-                if (lane == 0) have_at[slot * 4 + w] = x.have;
                 const uint32_t word_k = __shfl_sync(kAll, x.word, row), word_v = __shfl_sync(kAll, x.word, row + 16);
                 const Zero zv = zero_pair((word_v & 15u) * 0x10001u);
                 uint8_t* k_tile = smem + C::OFF_KV + slot * 2 * C::KV_BYTES;
@@ -553,7 +552,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                 ptx::tmem_ld32(s_at + 32, x1);
                 // what says which keys count comes while the scores do
                 const uint4 hs = *reinterpret_cast<const uint4*>(have_at + slot * 4);
-                const float4 e0 = *reinterpret_cast<const float4*>(ends + slot * 4), e1 = *reinterpret_cast<const float4*>(ends + slot * 4 + 2);
                 ptx::tmem_wait_ld();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
@@ -593,21 +591,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     }
                 }
 
-                // ---- running maximum of x + log2(sv): where the scales of V lie within 2^kSpan of one another, the
-                // sum of the two maxima does as well (the weights come out up to 2^kSpan smaller), at a third of
-                // the instructions
-                const float most = fmaxf(ptx::fmax3(e0.x, e0.z, e1.x), e1.z), least = fminf(ptx::fmin3(e0.y, e0.w, e1.y), e1.w);
-                float peak = -INFINITY, peak1 = -INFINITY;
-                if (most - least <= kSpan) {
+                // ---- running maximum of x + log2(sv): the sum of the two maxima is no less, at a third of the
+                // instructions, and says whether any row may have to move.  Whether and where to is then
+                // found from the keys that the row sees, and from nothing else.
+                float peak = INFINITY, peak1 = -INFINITY;
+                if (i > 0) {  // the first tile always moves it
+                    const float4 most4 = *reinterpret_cast<const float4*>(most_at + slot * 4);
+                    peak = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < kKeys / 4; ++j) {
                         peak = ptx::fmax3(peak, ptx::f2_lo(s[2 * j]), ptx::f2_hi(s[2 * j]));
                         peak1 = ptx::fmax3(peak1, ptx::f2_lo(s[2 * j + 1]), ptx::f2_hi(s[2 * j + 1]));
                     }
-                    peak = fmaxf(peak, peak1) + most;
-                } else {
+                    peak = fmaxf(peak, peak1) + fmaxf(ptx::fmax3(most4.x, most4.y, most4.z), most4.w);
+                }
+                if (__any_sync(kAll, peak > top + kRise)) {
                     const uint4 ls = *reinterpret_cast<const uint4*>(lost_at + slot * 4);
                     lost |= (seen & ((uint64_t)(ls.x | ls.y << 16) | ((uint64_t)(ls.z | ls.w << 16) << 32))) != 0;
+                    peak = peak1 = -INFINITY;
 #pragma unroll
                     for (int j = 0; j < kKeys / 4; ++j) {
                         const ulonglong2 a = lam[j];
@@ -616,14 +617,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                         peak1 = ptx::fmax3(peak1, ptx::f2_lo(v), ptx::f2_hi(v));
                     }
                     peak = fmaxf(peak, peak1);
-                }
-                const bool rise = peak > top + kRise;
-                if (__any_sync(kAll, rise)) {
+                    const bool rise = peak > top + kRise;
                     const float to = rise ? peak - kHead : top;
                     const float f = rise ? ptx::ex2(top - to) : 1.f;
                     top = to;
                     sum2 = ptx::f2_mul(sum2, ptx::f2_pack(f, f));
-                    if (i > 0) {
+                    if (__any_sync(kAll, rise) && i > 0) {
                         wait_all(&pv_done[2 * h + ((n - 1) & 1)], (n - 1) >> 1);
                         if (!ok) break;
                         ptx::tc_fence_after();

@@ -7,9 +7,8 @@ all of one value, the query all ones.  Then, relative to the average of |v|, an 
   2 (G 2^-22 + 2^-21)   a weight: its argument of at most G (in units of log 2) after four roundings,
                         and the exponential; twice, for the normalisation
   2^-22                 the two fp16 halves of a weight (2^-11 for an output in bf16, which has one)
-  N 2^-34 w             half a step at the bottom of fp16 (2^-25) for each of N keys, where the row's largest
-                        weight is at least 2^9; of that weight's own |v|.  2^-31 in the kernel for chunks,
-                        whose largest weight may be 2^3 smaller
+  N 2^-33 w             half a step at the bottom of fp16 (2^-25) for each of N keys, where the row's largest
+                        weight is at least 2^8; of that weight's own |v|
   C 2^-23               a sum of C steps, each of which may truncate (C 2^-24 for one that rounds).  The keys
                         of a call of one request are shared out over the SMs: a warp (or a row's thread) adds up at
                         most 11 tiles of 64 keys, 16 at a time in O (twice, for the halves) and 2 by 2 in the
@@ -76,7 +75,7 @@ def check(k, v, gap, new, out_dtype, peak_at=0, batch=1):
         largest = np.abs(values[1][peak_at]).max() / np.exp(want_lse[0, 0] - gap * math.log(2))
         share = 2 * (gap * 2.0 ** -22 + 2.0 ** -21) + steps * 2.0 ** -23
         share += 2.0 ** -11 if out_dtype == torch.bfloat16 else 2.0 ** -22
-        bound = share * mean[0, 0] + length * (2.0 ** -34 if new < 64 else 2.0 ** -31) * largest + HALF[out_dtype] * np.abs(want[0, 0])
+        bound = share * mean[0, 0] + length * 2.0 ** -33 * largest + HALF[out_dtype] * np.abs(want[0, 0])
         err = np.abs(got[:, i] - want[0, 0])  # of every request and head
         assert (err <= bound).all(), f"row {i}: off by {err.max():.3e}, bound {bound.min():.3e}"
         lse_bound = gap * 2.0 ** -22 + 2.0 ** -21 + steps * 2.0 ** -23 + 2.0 ** -22 * abs(want_lse[0, 0])
