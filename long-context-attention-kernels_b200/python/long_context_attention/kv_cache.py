@@ -14,6 +14,7 @@ import operator
 from typing import NamedTuple, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from ._native import extension
 
@@ -51,6 +52,9 @@ def _need_cuda(t: torch.Tensor, what: str) -> None:
 def _no_grad(*tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise NotImplementedError("long_context_attention: the operators of the 4-bit cache have no backward")
+    # no tensor carries a forward-mode tangent outside a dual level, which is quicker to ask
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("long_context_attention: the operators of the 4-bit cache have no forward-mode derivative")
 
 
 def kv_cache_layout(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor,

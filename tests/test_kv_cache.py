@@ -188,3 +188,25 @@ def test_layout_oracle_takes_whole_requests_in_order():
     assert got["kv_lens"].tolist() == [13, 0, 5, 0]  # 49 tokens pass the table's row, which takes no pages
     got = swa_oracle.kv_layout(table, [10, 0, 0, 0], [3, 40, 5, 0], [0, 1, 2, 3], 3, 16, 42)
     assert got["kv_lens"].tolist() == [13, 0, 0, 0] and got["cu_seqlens"].tolist() == [0, 3, 42, 42, 42]
+
+
+def test_derivatives_are_refused():
+    """A gradient that is asked for, backward or forward, is refused and not dropped."""
+    from torch.autograd import forward_ad
+
+    from long_context_attention import kv_cache
+
+    x, leaf = torch.zeros(2), torch.zeros(2, requires_grad=True)
+    kv_cache._no_grad(x, x)
+    with pytest.raises(NotImplementedError, match="backward"):
+        kv_cache._no_grad(x, leaf)
+    with torch.no_grad():
+        kv_cache._no_grad(leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(2))
+        kv_cache._no_grad(x)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            kv_cache._no_grad(x, dual)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: (kv_cache._no_grad(t), t)[1], (x,), (torch.ones(2),))
+    kv_cache._no_grad(x)
