@@ -128,7 +128,7 @@ def sliding_window_attention_cached(
     left as they were in ``out``; in the LSE, and in O without ``out``, they are not initialised.
     """
     _need_cuda(Q, "Q")
-    _no_grad(Q)
+    _no_grad(Q) if out is None else _no_grad(Q, out)
     try:
         window_size = operator.index(window_size)
     except TypeError:
