@@ -54,7 +54,7 @@ enum {
     LCA_DEVERR_TIMEOUT_DRAIN = 4,    /* main kernel: waiting for its own copies at exit */
     LCA_DEVERR_TIMEOUT_PEER = 5,     /* peer exchange: another rank's data did not arrive */
     LCA_DEVERR_TIMEOUT_BACKWARD = 6, /* backward kernel: waited for a tile or an MMA */
-    LCA_DEVERR_TIMEOUT_CACHE = 7     /* cached attention: a copy out of the pool did not arrive */
+    LCA_DEVERR_TIMEOUT_CACHE = 7     /* cached attention: waited for a copy or another role */
 };
 
 /* Element types: Q, K, V share LCA_DTYPE_F16 or LCA_DTYPE_BF16; the output is fp32
@@ -419,8 +419,8 @@ LCA_API int lca_kv_release(const int32_t* block_table, int64_t batch, int64_t ta
 /*
  * Quantise the rows k, v [num_tokens][kv_heads][head_dim] (fp16 or bf16; strides in elements, the
  * last dimension contiguous, any alignment of whole elements) into the slots given.  A slot
- * outside the pool (-1) is skipped.  Slots of one call are distinct; which row a slot given twice
- * holds afterwards is not specified.
+ * outside the pool (-1) is skipped.  Slots of one call are distinct; what a slot given twice holds
+ * afterwards is not specified (codes of one row under the scale of another, say).
  */
 LCA_API int lca_kv4_append(void* pool, int64_t num_pages, int64_t kv_heads, int64_t page_size, int64_t head_dim,
                            const void* k, const void* v, int dtype, int64_t k_token_stride, int64_t k_head_stride,

@@ -1,5 +1,5 @@
 // kv4.h -- internal interface between the C-ABI layer (kv4_capi.cpp) and the kernels of the
-// paged 4-bit KV cache (kv4_cache.cu, kv4_attention.cu).  Not part of the public ABI.
+// paged 4-bit KV cache (kv4_cache.cu, kv4_attention.cu, kv4_chunk.cu).  Not part of the public ABI.
 //
 // Cache format.  A pool is [pages][kv_heads] pieces of page_size tokens; a piece is
 // page_size / 16 blocks, and a block holds 16 tokens of one head contiguously:

@@ -26,7 +26,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kWholeKeys = 1536; // items of up to this many keys are not split
-constexpr int kChunkFrom = 64;   // mean rows a request from which the tcgen05 kernel takes the call
+constexpr int kChunkFrom = 64;   // mean rows a request from which the tcgen05 kernel takes the call (both: plan_attention)
 constexpr int kSms = 148;
 constexpr int kCtas64 = 6;
 
@@ -779,7 +779,9 @@ cudaError_t attention_rows(int tile_rows, int tile_keys, const AttnParams& p, co
 
 // Rows of an item: as many groups of 8 as an average request has, so that a tile of keys is
 // unpacked once for all of them, up to the 32 whose sums fit the registers of one warp; from
-// kChunkFrom rows on, 256 rows on tcgen05.
+// kChunkFrom rows on, 256 rows on tcgen05.  Measured with 32 / 8 heads of 128 (one kernel | the other, us), 48, 64 and
+// 96 rows a request over whole contexts of 16K to 32K: one request 62 | 63, 65 | 63, 83 | 66; 32 of them 899 | 1080,
+// 911 | 1086, 1336 | 1095; with a window of 512, 32 requests of 32, 48 and 64 rows 34 | 49, 62 | 48, 65 | 49.
 AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t batch, int64_t capacity,
                         int64_t window, int64_t num_globals) {
     AttnPlan a = {};
@@ -796,10 +798,17 @@ AttnPlan plan_attention(int64_t rows, int64_t heads, int64_t kv_heads, int64_t h
     // Long items are cut wherever a CTA's share of the line ends, and merged by a second kernel;
     // short ones (a band) stay whole, which saves that launch.
     // Many long items of many rows balance by themselves, and their parts are large.
+    // Measured (cut | whole, us; contexts of 16K, 32 / 8 heads of 128): one token of 1 request, window 1024, 1400
+    // and 2048: 16 | 14, 16 | 17, 16 | 22; of 8 requests 17 | 15, 18 | 18, 19 | 22; of 64 requests 39 | 26, 46 | 43, 54 | 45
+    // (from 4096 on 81 | 77).  Chunks, fewer items than 4 an SM, 32K contexts: 8 items of a window of 8192 76 | 209, 256
+    // items 461 | 412, of whole contexts 1483 | 1552; 1024 whole contexts 5404 | 5365.  A few chunks with a window
+    // little above kWholeKeys would be better whole (32 items, 2048: 148 | 65): their parts cost more than they save.
     a.split = longest > kWholeKeys && (!chunk || items < 4 * kSms);
     // A step of 64 keys shares what it costs besides its keys (waiting, issuing, the vote on the maximum),
     // where the scores of 64 leave the registers for it and items are long enough to fill the warps.
     a.tile_keys = chunk ? kChunkKeys : (a.tile_rows == 8 && a.split ? 64 : 32);
+    // Shares of at least 64, 256 and 1024 keys: one token of 4 requests of 2000 keys in 17, 13 and 16 us, of one of
+    // 8000 in 16, 15 and 18; of longer ones alike.
     a.min_tiles = 256 / a.tile_keys;
     const int per_sm = chunk ? 1 : ctas_per_sm((int)head_dim, a.tile_rows, a.tile_keys);
     a.items = std::min<int64_t>(items, 0x7fffffff);

@@ -288,7 +288,8 @@ __device__ __forceinline__ Item item_of(const RowsParams& p, long long item, lon
 // One group of d / 16 lanes per (token, head): a lane loads two pieces of 16 bytes of the K and of the V
 // row and stores two 32-bit words of codes of each.  Bound by memory, 4d bytes read and d + 8 written
 // a pair, as long as a row's reductions and its reciprocal are shared by 16 elements of a
-// lane (with 8, the instructions bounded it: 128K tokens of 8 heads of 128 in 162 us, now 124).
+// lane; with 8 the instructions bound it.  128K tokens of 8 heads of 128: 110 us, 94% of the copy rate;
+// 155 us where rows are not on 16-byte boundaries (2-byte loads).
 template <int D, typename T, bool VECTOR>
 __global__ void __launch_bounds__(kRowThreads) kv4_append(const RowsParams p) {
     constexpr int LANES = D / (8 * kPieces), GROUPS = kRowThreads / LANES;

@@ -12,7 +12,7 @@
 //   softmax warps (8)  a thread per row: scores times scales, the running maximum, weights to fp16
 //   query warps (3)    the next item's query rows into the other of two buffers, and what the softmax
 //                      warps need to know of the item (found by themselves it took them 2800 cycles an item,
-//                      and registers of their loop: 2K chunks of 128K contexts in 198 us, now 189)
+//                      and registers of their loop)
 // Barriers with one phase per tile of one parity (n & 1), so that a wait for tile n - 1 cannot be
 // answered by a phase before or after it.
 // A tile of codes is unpacked once for 256 rows, and the products of one tile run under
@@ -30,7 +30,7 @@ namespace {
 constexpr int kHalfRows = 128;            // rows of a tile A or B
 constexpr int kKeys = kChunkKeys;         // keys of a tile
 // unpacked tiles: with two, a tile could only be unpacked once the product of the one before the last was
-// done, and the scores came late (2K chunks of 128K contexts 188 us, with three 157)
+// done, and the scores came late (a fifth more time)
 constexpr int kRing = 3;
 constexpr int kSoftmaxWarps = 8, kUnpackWarps = 4, kMmaWarp = kSoftmaxWarps + kUnpackWarps, kQueryWarps = 3;
 constexpr int kThreads = 512;  // four warpgroups: softmax A and B, unpacking, products and queries

@@ -293,7 +293,7 @@ DEVICE_ERRORS = {
     4: "main kernel: waiting for its own copies at exit took too long",
     5: "peer exchange: another rank's halos, global rows or row partials did not arrive in time",
     6: "backward kernel: waited too long for a tile or an MMA",
-    7: "cached attention: a copy out of the pool did not arrive in time",
+    7: "cached attention: waited too long for a copy, or for another role of the kernel",
 }
 
 
