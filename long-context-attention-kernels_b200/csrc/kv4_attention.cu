@@ -478,9 +478,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
                             for (int m = 4; m < 32; m *= 2) to = fmaxf(to, __shfl_xor_sync(kAll, to, m));
                             const bool rise = to > top[nt][e] + kRise;
                             to = rise ? to - kHead : top[nt][e];
-                            f[e] = rise ? ptx::ex2(top[nt][e] - to) : 1.f;
+                            const float half = rise ? ex2_half(top[nt][e] - to) : 1.f;
                             top[nt][e] = to;
-                            sum[nt][e] *= f[e];
+                            sum[nt][e] = half * (half * sum[nt][e]);
+                            f[e] = half * half;
                         }
 #pragma unroll
                         for (int k = 0; k < STEPS; ++k) {
@@ -611,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, 8 * NT, 16 * KB_))
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     const float2 st = stats[w * C::ROWS + row];
-                    const float f = ptx::ex2(st.x - ref);
-                    l += f * st.y;
+                    const float half = ex2_half(st.x - ref), f = half * half;
+                    l += half * (half * st.y);
                     const float4 a = *reinterpret_cast<const float4*>(buf + (w * C::ROWS + row) * C::PITCH + d);
                     v[0] += f * a.x, v[1] += f * a.y, v[2] += f * a.z, v[3] += f * a.w;
                 }
@@ -707,8 +708,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
         const long long at = part_of(c);
         const float2 ml = p.part_ml[at];
-        const float f = ptx::ex2(ml.x - ref);
-        l += f * ml.y;
+        const float half = ex2_half(ml.x - ref), f = half * half;
+        l += half * (half * ml.y);
         const float* src = p.part_o + at * D + lane * PER;
         if (PER == 4) {
             const float4 v = *reinterpret_cast<const float4*>(src);
@@ -729,8 +730,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_attention_merge(const At
     const float ref_top = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int w = 0; w < kMergeWarps; ++w) {
-        const float f = ptx::ex2(s_m[w] - ref_top);
-        sum += f * s_l[w];
+        const float half = ex2_half(s_m[w] - ref_top), f = half * half;
+        sum += half * (half * s_l[w]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += f * s_o[w][4 * threadIdx.x + i];
     }

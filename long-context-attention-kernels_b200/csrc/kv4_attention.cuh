@@ -35,6 +35,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // The sum takes p_j = w_j / sv_j; log2(sv) is cut off at kLeast, so that 2^30 of them stay in fp32's range.
 constexpr float kHead = 8.f, kRise = 15.9f, kLeast = -80.f;
 
+// The square root of 2^d, d <= 0.  M is up to 200 apart between keys whose V is near zero and keys whose V is
+// large; 2^d itself would be 0 then, while a sum of the former, 2^80 times larger, still counts.
+__device__ __forceinline__ float ex2_half(float d) { return ptx::ex2(0.5f * d); }
+
 // The natural logarithm of a row's sum l 2^m.
 __device__ __forceinline__ float lse_of(float m, float l) {
     constexpr float kTakeOff = 1.f / 256.f;

@@ -619,9 +619,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_chunk(const AttnParams p, con
                     peak = fmaxf(peak, peak1);
                     const bool rise = peak > top + kRise;
                     const float to = rise ? peak - kHead : top;
-                    const float f = rise ? ptx::ex2(top - to) : 1.f;
+                    const float half = rise ? ex2_half(top - to) : 1.f, f = half * half;
+                    const uint64_t half2 = ptx::f2_pack(half, half);
                     top = to;
-                    sum2 = ptx::f2_mul(sum2, ptx::f2_pack(f, f));
+                    sum2 = ptx::f2_mul(ptx::f2_mul(sum2, half2), half2);
                     if (__any_sync(kAll, rise) && i > 0) {
                         wait_all(&pv_done[2 * h + ((n - 1) & 1)], (n - 1) >> 1);
                         if (!ok) break;

@@ -8,7 +8,7 @@ all of one value, the query all ones.  Then, relative to the average of |v|, an 
                         and the exponential; twice, for the normalisation
   2^-22                 the two fp16 halves of a weight (2^-11 for an output in bf16, which has one)
   N 2^-33 w             half a step at the bottom of fp16 (2^-25) for each of N keys, where the row's largest
-                        weight is at least 2^8; of that weight's own |v|
+                        weight (of the softmax, times its |v|) is at least 2^8
   C 2^-23               a sum of C steps, each of which may truncate (C 2^-24 for one that rounds).  The keys
                         of a call of one request are shared out over the SMs: a warp (or a row's thread) adds up at
                         most 11 tiles of 64 keys, 16 at a time in O (twice, for the halves) and 2 by 2 in the
@@ -51,7 +51,7 @@ def cache_of(k, v, heads, batch):
     return pool, table, [swa_oracle.kv4_values(x.float().numpy()) for x in rows]
 
 
-def check(k, v, gap, new, out_dtype, peak_at=0, batch=1):
+def check(k, v, gap, new, out_dtype, peak_at=0, batch=1, off=0.0):
     heads = 1 if batch == 1 else HEADS
     pool, table, values = cache_of(k, v, heads, batch)
     n = len(k)
@@ -66,19 +66,20 @@ def check(k, v, gap, new, out_dtype, peak_at=0, batch=1):
         steps = STEPS
     elif new < 64:  # two halves of four blocks a tile, and four warps to merge
         steps = -(-tiles // 4) * 8 + 4
-    else:           # O truncates, the sum of 32 pairs rounds
-        steps = max(tiles * 8, tiles * 32 / 2)
+    else:           # the sum takes fewer: 32 pairs a tile and then the tiles, and rounds
+        steps = tiles * 8
     for i in sorted({0, new // 2, new - 1}):  # the rows are alike but for a few keys at the end
         length = n - new + 1 + i
         want, want_lse, mean, _ = swa_oracle.cached_attention(np.ones((1, 1, D)), values[0][:length], values[1][:length], 2 * n,
                                                               [], scale)
-        largest = np.abs(values[1][peak_at]).max() / np.exp(want_lse[0, 0] - gap * math.log(2))
-        share = 2 * (gap * 2.0 ** -22 + 2.0 ** -21) + steps * 2.0 ** -23
+        share_of = np.exp(scale * values[0][:length, 0].sum(-1) - want_lse[0, 0])
+        largest = (share_of * np.abs(values[1][:length, 0]).max(-1)).max()
+        share = 2 * (gap * 2.0 ** -22 + 2.0 ** -21 + off) + steps * 2.0 ** -23
         share += 2.0 ** -11 if out_dtype == torch.bfloat16 else 2.0 ** -22
         bound = share * mean[0, 0] + length * 2.0 ** -33 * largest + HALF[out_dtype] * np.abs(want[0, 0])
         err = np.abs(got[:, i] - want[0, 0])  # of every request and head
         assert (err <= bound).all(), f"row {i}: off by {err.max():.3e}, bound {bound.min():.3e}"
-        lse_bound = gap * 2.0 ** -22 + 2.0 ** -21 + steps * 2.0 ** -23 + 2.0 ** -22 * abs(want_lse[0, 0])
+        lse_bound = gap * 2.0 ** -22 + 2.0 ** -21 + 3 * off + steps * 2.0 ** -23 + 2.0 ** -22 * abs(want_lse[0, 0])
         assert (np.abs(lse[:, :, i] - want_lse[0, 0]) <= lse_bound).all()
     assert lca.device_error() == 0
 
@@ -130,3 +131,18 @@ def test_values_of_every_size(size, new):
     k[0], k[20000:] = 1.875, 0.46875
     v = size * (np.abs(rng.standard_normal((n, D))) + 0.5)
     check(k, v, 14.2, new, torch.float32)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("new,batch", [(1, 1), (20, 1), (70, 1), (1, 64), (70, 75)])
+@pytest.mark.parametrize("sizes", [(0.0, 1e16), (1e16, 0.0), (1e-22, 1e25), (0.0, 1.0, 1e12, 1e-3, 1e28), (1e20, 0.0, 1e20)])
+def test_stretches_of_values_far_apart_in_size(sizes, new, batch, out_dtype):
+    """Even scores: every key counts in the sum, whatever the sizes of V before and behind it.  The sizes move
+    the reference of the weights by more than fp32's exponent holds.  It is then up to 128 away from the
+    scores, which are rounded to 2^-18 against it, as are it and the logarithm in the LSE."""
+    n = 9000 + new
+    k, v = np.full((n, D), 1.875), np.ones((n, D))
+    at = np.linspace(0, 9000, len(sizes) + 1).astype(int)
+    for size, a, b in zip(sizes, at, [*at[1:-1], n]):
+        v[a:b] *= size
+    check(k, v, 0.3, new, out_dtype, batch=batch, off=2.0 ** -18)
